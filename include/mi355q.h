@@ -490,6 +490,126 @@ extern "C"
     size_t mi355q_context_attention_workspace_size(const mi355q_context_attention_params* params);
     mi355q_status mi355q_context_attention(const mi355q_context_attention_params* params, void* stream);
 
+    /* ---- speculative decoding over the paged cache.  No counterpart among the reference's entry points (its Medusa
+     * attention is inside GPTAttention, is_medusa_enabled).  A step of a batch whose sequences each draft a tree of tokens:
+     *   mi355q_kv_block_tables      blocks, block pointers of every layer and slots for the drafted tokens
+     *   mi355q_tree_attention       per layer: K / V of the nodes into the cache, attention of the nodes
+     *   mi355q_draft_tree_accept    the path along which the model agrees with the drafts
+     *   mi355q_kv_commit_path       the path's keys and values to the end of the history, in every layer; new lengths
+     * All lengths, tables and results stay on the device; nothing synchronises and every call can be captured into a
+     * graph.  A workspace belongs to one call until that call has run on the GPU: two graphs, or two streams, that may
+     * run at the same time need one each. */
+
+    /* Attention of a tree of drafted tokens over the paged cache.  Node i of sequence b is row draft_offsets[b] + i of
+     * qkv; its position is past_lengths[b] + position_offsets[row] (NULL: + i), its cache slot past_lengths[b] + i (position
+     * t lives in block t / tokens_per_block: no window, no sink tokens, no beams).  The call rotates q and k, rounds K / V
+     * of every node once to the cache's type, stores them, and attends from every node to the past tokens and to the
+     * nodes j whose bit (word j / 32, bit j % 32 of the row of tree_mask) is set -- itself too only if its own bit is.  A row
+     * that sees nothing is 0.  What a row does not see does not reach it, infinities and NaN included.  K / V are read back
+     * from the cache, so an 8-bit cache attends to the quantised nodes.
+     * A sequence whose device-side lengths do not fit (past_lengths outside 0 .. max_past_length, more than
+     * max_draft_length nodes, rows outside num_tokens, keys beyond the block table) or whose table lacks a block (pointer 0)
+     * is skipped: its rows of out stay as they were.  Rows of qkv / out outside every sequence are not touched. */
+    typedef struct
+    {
+        const void* qkv;            /* [num_tokens, (Hq+2Hkv)*Dh] act type, row stride qkv_stride; q | k | v */
+        const void* qkv_bias;       /* [(Hq+2Hkv)*Dh] or NULL */
+        void* out;                  /* [num_tokens, Hq*Dh] */
+        const int32_t* past_lengths;   /* device [batch]: tokens in the cache */
+        const int32_t* draft_offsets;  /* device [batch + 1]: first row of each sequence */
+        const int32_t* position_offsets; /* device [num_tokens] (a node's depth in the tree) or NULL */
+        const uint32_t* tree_mask;  /* device [num_tokens, mask_words] */
+        const int64_t* block_pointers;   /* device [batch, 2, max_blocks_per_seq] block addresses */
+        const float* kv_scale_orig_quant; /* device [1], 8-bit caches */
+        const float* kv_scale_quant_orig;
+        void* workspace;            /* mi355q_tree_attention_workspace_size bytes; qkv, qkv_bias, out and it 16-byte aligned */
+        size_t workspace_bytes;
+        int64_t qkv_stride;         /* elements between rows of qkv, a multiple of 8; 0 = (Hq+2Hkv)*Dh */
+        int32_t batch, num_heads, num_kv_heads;
+        int32_t head_size;          /* a multiple of 8 (8-bit caches: of 16) up to 256 */
+        int32_t num_tokens;         /* rows of qkv and out */
+        int32_t max_draft_length;   /* host bound of a sequence's nodes, <= 1024 */
+        int32_t max_past_length;    /* host bound of past_lengths */
+        int32_t mask_words;         /* >= ceil(max_draft_length / 32) */
+        int32_t max_blocks_per_seq, tokens_per_block;
+        int32_t act_type;           /* MI355Q_HALF / MI355Q_BF16 */
+        int32_t kv_type;            /* act_type, MI355Q_INT8 or MI355Q_FP8 */
+        int32_t position_embedding_type; /* 0 none applied here, 1 RoPE GPT-J, 2 RoPE GPT-NeoX */
+        int32_t rotary_embedding_dim;
+        float rotary_embedding_base;
+        int32_t rotary_embedding_scale_type; /* 0 none, 1 linear, 2 dynamic (by the node's own position) */
+        float rotary_embedding_scale;
+        int32_t rotary_embedding_max_positions;
+        float q_scaling;
+        int32_t multi_block_mode;   /* 0: heuristic, > 0: that many key splits at most */
+    } mi355q_tree_attention_params;
+    size_t mi355q_tree_attention_workspace_size(const mi355q_tree_attention_params* params);
+    mi355q_status mi355q_tree_attention(const mi355q_tree_attention_params* params, void* stream);
+
+    /* Block tables, block pointers and slot maps on the device, from request lengths: what KVCacheManager does on the host
+     * (block_table holds block indices; a pool is all its K blocks, then all its V blocks).  Request b holds
+     * block_counts[b] blocks and past_lengths[b] tokens and is about to get new_lengths[b] more: the blocks it lacks come
+     * from the free ring, in request order.  new_lengths[b] < 0 ends the request: its blocks go to the ring's back (they can
+     * be handed out from the next call on).  status: 0 done; 1 the free blocks did not reach (nor for any later request
+     * that asked); 2 more than max_blocks_per_seq blocks; 3 lengths or counts out of range.  A refused request keeps what it
+     * has and its slots are -1.  Pointers are 0 where no block is held (all of an ended request's); so are those of a table
+     * or ring entry outside the pool. */
+    typedef struct
+    {
+        const int32_t* past_lengths; /* device [batch] */
+        const int32_t* new_lengths;  /* device [batch] */
+        int32_t* block_table;        /* device [batch, max_blocks_per_seq], updated in place */
+        const int32_t* block_counts; /* device [batch] */
+        int32_t* block_counts_out;   /* device [batch]; may be block_counts */
+        int32_t* free_blocks;        /* device [num_blocks]: the ring, updated in place behind the free ones */
+        const int32_t* free_state;   /* device [2]: first free entry of the ring, number of free blocks */
+        int32_t* free_state_out;     /* device [2]; may be free_state */
+        const int64_t* pool_bases;   /* device [num_pools]: address of each pool's first K block */
+        int64_t* block_pointers;     /* device [num_pools, batch, 2, max_blocks_per_seq] */
+        int32_t* token_offsets;      /* device [batch + 1]: first new token of each request (ended ones have none) */
+        int64_t* slot_map;           /* device [num_tokens]: block index * tokens_per_block + offset of every new token, -1 behind
+                                        the last one; NULL with num_tokens 0 */
+        int32_t* status;             /* device [batch] */
+        void* workspace;             /* mi355q_kv_block_tables_workspace_size bytes, 16-byte aligned */
+        size_t workspace_bytes;
+        int64_t block_bytes;         /* bytes of one K (or V) block */
+        int32_t batch, max_blocks_per_seq, num_blocks, num_pools, num_tokens, tokens_per_block;
+    } mi355q_kv_block_tables_params;
+    size_t mi355q_kv_block_tables_workspace_size(int32_t batch);
+    mi355q_status mi355q_kv_block_tables(const mi355q_kv_block_tables_params* params, void* stream);
+
+    /* The accepted path of every tree: from node 0 (the last token that is certain) on, the lowest child whose drafted token
+     * is the model's token after its parent.  Children stand behind their parents (parents[i] < i); others are not followed.
+     * accept_path [batch, max_path] and accepted_tokens (the model's token after each node of the path: what the step
+     * emits) are -1 behind accept_counts[b] entries; an empty tree has none. */
+    typedef struct
+    {
+        const int32_t* draft_tokens;  /* device [num_tokens] */
+        const int32_t* parents;       /* device [num_tokens]: index within the sequence's tree, -1 for the root */
+        const int32_t* target_tokens; /* device [num_tokens]: the model's token after each node */
+        const int32_t* draft_offsets; /* device [batch + 1] */
+        int32_t* accept_path;         /* device [batch, max_path] */
+        int32_t* accept_counts;       /* device [batch] */
+        int32_t* accepted_tokens;     /* device [batch, max_path] */
+        int32_t batch, num_tokens, max_path;
+    } mi355q_draft_tree_accept_params;
+    mi355q_status mi355q_draft_tree_accept(const mi355q_draft_tree_accept_params* params, void* stream);
+
+    /* Slot past_lengths[b] + i takes the keys and values of slot past_lengths[b] + accept_path[b][i], i < accept_counts[b], in
+     * every pool; new_lengths[b] = past_lengths[b] + accept_counts[b].  A path has to rise strictly and stay inside the
+     * sequence's blocks; otherwise nothing of that sequence moves and new_lengths[b] = past_lengths[b]. */
+    typedef struct
+    {
+        const int64_t* block_pointers; /* device [num_pools, batch, 2, max_blocks_per_seq] */
+        const int32_t* past_lengths;   /* device [batch] */
+        const int32_t* accept_path;    /* device [batch, max_path] */
+        const int32_t* accept_counts;  /* device [batch] */
+        int32_t* new_lengths;          /* device [batch]; not past_lengths itself */
+        int32_t batch, num_pools, max_blocks_per_seq, tokens_per_block, num_kv_heads, head_size, max_path;
+        int32_t kv_type;               /* MI355Q_HALF / MI355Q_BF16 / MI355Q_INT8 / MI355Q_FP8 */
+    } mi355q_kv_commit_path_params;
+    mi355q_status mi355q_kv_commit_path(const mi355q_kv_commit_path_params* params, void* stream);
+
     enum
     {
         MI355Q_AR_RING = 0,

@@ -1,0 +1,490 @@
+// draft_tree.hip -- what surrounds the attention of drafted tokens (tree_attn.hip) on the device, so that a speculative step
+// needs no host round trip: block tables and slot maps from request lengths, the accepted path of a tree, and the move of the
+// accepted keys and values to the end of the history.  All integer work and copies: results are exact and do not depend on
+// the order in which workgroups run.
+#include "kernels.h"
+
+namespace mi355q
+{
+namespace
+{
+
+// ---------------------------------------------------------------------------------------------- block tables
+// Every request holds block_counts[b] blocks; past + new tokens need ceil((past + new) / tokens_per_block).  The missing
+// ones come from the front of a ring of free block indices, in request order; a request that ends returns its blocks to
+// the ring's back.  Two launches: the plan (prefix sums over the requests, one workgroup) and the fill (tables, ring,
+// pointers of every pool, slots), which reads only what the plan does not write, so state updated in place is safe.
+struct TableArgs
+{
+    const int32_t* past_lengths;
+    const int32_t* new_lengths;
+    int32_t* block_table;
+    const int32_t* block_counts;
+    int32_t* block_counts_out;
+    int32_t* free_blocks;
+    const int32_t* free_state;
+    int32_t* free_state_out;
+    const int64_t* pool_bases;
+    int64_t* block_pointers;
+    int32_t* token_offsets;
+    int64_t* slot_map;
+    int32_t* status;
+    int4* rows; // workspace [batch]: blocks held before, blocks granted (-1: released), first ring position, status
+    int64_t block_bytes;
+    int batch, max_blocks, num_blocks, num_pools, num_tokens, tpb, tpb_log2;
+    int pools_per_wg;
+};
+
+constexpr int PLAN_THREADS = 1024;
+
+// exclusive prefix sum over the workgroup; `sum` receives the total.  lds: [17] int64
+__device__ __forceinline__ int64_t exclusive_scan(int64_t v, int64_t* lds, int64_t& sum)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int64_t x = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1)
+    {
+        const int64_t y = __shfl_up(x, o);
+        if (lane >= o)
+            x += y;
+    }
+    __syncthreads();
+    if (lane == 63)
+        lds[wave] = x;
+    __syncthreads();
+    int64_t base = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < PLAN_THREADS / 64; ++w)
+    {
+        if (w < wave)
+            base += lds[w];
+        total += lds[w];
+    }
+    sum = total;
+    return base + x - v;
+}
+
+__global__ __launch_bounds__(PLAN_THREADS) void table_plan_kernel(TableArgs p)
+{
+    __shared__ int64_t lds[PLAN_THREADS / 64];
+    const int64_t N = p.num_blocks;
+    const int64_t head = ((p.free_state[0] % N) + N) % N;
+    const int64_t avail = min((int64_t) max(p.free_state[1], 0), N);
+    int64_t demand = 0, granted = 0, returned = 0, tokens = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += PLAN_THREADS)
+    {
+        const int b = b0 + threadIdx.x;
+        int count = 0, status = 0;
+        int64_t need = 0, back = 0, fresh = 0;
+        bool release = false;
+        if (b < p.batch)
+        {
+            const int64_t past = p.past_lengths[b], add = p.new_lengths[b];
+            count = p.block_counts[b];
+            release = add < 0;
+            fresh = max(add, (int64_t) 0);
+            if (past < 0 || count < 0 || count > p.max_blocks)
+                status = 3;
+            else if (release)
+                back = count;
+            else
+            {
+                const int64_t total = (past + add + p.tpb - 1) >> p.tpb_log2;
+                if (total > p.max_blocks)
+                    status = 2;
+                else
+                    need = max(total - count, (int64_t) 0);
+            }
+        }
+        int64_t s_need, s_back, s_fresh, s_grant;
+        const int64_t need_from = demand + exclusive_scan(need, lds, s_need);
+        const int64_t back_from = returned + exclusive_scan(back, lds, s_back);
+        const int64_t tok_from = tokens + exclusive_scan(fresh, lds, s_fresh);
+        // first come, first served: a request that the blocks do not reach for gets none, nor does any behind it that asks
+        if (need > 0 && need_from + need > avail)
+        {
+            status = 1;
+            need = 0;
+        }
+        exclusive_scan(need, lds, s_grant);
+        if (b < p.batch)
+        {
+            const bool gives = release && status == 0;
+            const int64_t from = gives ? head + avail + back_from : head + need_from;
+            p.rows[b] = make_int4(count, gives ? -1 : (int) need, (int) (from % N), status);
+            p.token_offsets[b] = (int) min(tok_from, (int64_t) INT32_MAX);
+            p.status[b] = status;
+            p.block_counts_out[b] = gives ? 0 : count + (int) need;
+        }
+        demand += s_need;
+        returned += s_back;
+        tokens += s_fresh;
+        granted += s_grant;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0)
+    {
+        p.token_offsets[p.batch] = (int) min(tokens, (int64_t) INT32_MAX);
+        p.free_state_out[0] = (int) ((head + granted) % N);
+        p.free_state_out[1] = (int) min(avail - granted + returned, N);
+    }
+}
+
+// the index of block j of a request, from the table or, for a block granted in this call, from the ring; -1: none
+__device__ __forceinline__ int block_index(const TableArgs& p, int b, const int4& row, int j)
+{
+    int idx = -1;
+    if (row.y >= 0 && row.x >= 0 && row.x <= p.max_blocks && j < row.x + row.y)
+        idx = j < row.x ? p.block_table[(size_t) b * p.max_blocks + j]
+                        : p.free_blocks[(int) (((int64_t) row.z + j - row.x) % p.num_blocks)];
+    return idx >= 0 && idx < p.num_blocks ? idx : -1;
+}
+
+// grid (ceil(max_blocks / 512), batch, pool groups + 1), 256 threads, two blocks of the table per thread: bound by the
+// pointer stores.  The last z plane does the table and the ring.
+template <bool PAIRS>
+__global__ __launch_bounds__(256) void table_fill_kernel(TableArgs p)
+{
+    const int b = blockIdx.y, j = 2 * (blockIdx.x * 256 + threadIdx.x);
+    if (j >= p.max_blocks)
+        return;
+    const int4 row = p.rows[b];
+    if (blockIdx.z == gridDim.z - 1)
+    {
+        for (int k = j; k < min(j + 2, p.max_blocks); ++k)
+        {
+            int32_t* entry = p.block_table + (size_t) b * p.max_blocks + k;
+            if (row.y < 0 && k < row.x) // released
+                p.free_blocks[(int) (((int64_t) row.z + k) % p.num_blocks)] = *entry;
+            else if (row.y > 0 && k >= row.x && k < row.x + row.y) // granted
+                *entry = p.free_blocks[(int) (((int64_t) row.z + k - row.x) % p.num_blocks)];
+        }
+        return;
+    }
+    const int i0 = block_index(p, b, row, j), i1 = j + 1 < p.max_blocks ? block_index(p, b, row, j + 1) : -1;
+    const int64_t k0 = i0 * p.block_bytes, k1 = i1 * p.block_bytes, v = p.num_blocks * p.block_bytes;
+    const int lo = blockIdx.z * p.pools_per_wg, hi = min(lo + p.pools_per_wg, p.num_pools);
+    for (int pool = lo; pool < hi; ++pool)
+    {
+        const int64_t base = p.pool_bases[pool];
+        int64_t* out = p.block_pointers + (((size_t) pool * p.batch + b) * 2) * p.max_blocks + j;
+        const longlong2 kk = make_longlong2(i0 < 0 ? 0 : base + k0, i1 < 0 ? 0 : base + k1);
+        const longlong2 vv = make_longlong2(i0 < 0 ? 0 : base + k0 + v, i1 < 0 ? 0 : base + k1 + v);
+        if constexpr (PAIRS)
+        {
+            *reinterpret_cast<longlong2*>(out) = kk;
+            *reinterpret_cast<longlong2*>(out + p.max_blocks) = vv;
+        }
+        else
+        {
+            out[0] = kk.x;
+            out[p.max_blocks] = vv.x;
+            if (j + 1 < p.max_blocks)
+            {
+                out[1] = kk.y;
+                out[p.max_blocks + 1] = vv.y;
+            }
+        }
+    }
+}
+
+// one thread per new token: its request by bisection of the offsets
+__global__ __launch_bounds__(256) void table_slots_kernel(TableArgs p)
+{
+    const int t = blockIdx.x * 256 + threadIdx.x;
+    if (t >= p.num_tokens)
+        return;
+    int64_t slot = -1;
+    if (t < p.token_offsets[p.batch])
+    {
+        int lo = 0, hi = p.batch; // the last request whose first token is <= t and that has tokens
+        while (hi - lo > 1)
+        {
+            const int mid = (lo + hi) >> 1;
+            if (p.token_offsets[mid] <= t)
+                lo = mid;
+            else
+                hi = mid;
+        }
+        const int4 row = p.rows[lo];
+        if (row.w == 0)
+        {
+            const int64_t pos = (int64_t) p.past_lengths[lo] + (t - p.token_offsets[lo]);
+            const int idx = block_index(p, lo, row, (int) (pos >> p.tpb_log2));
+            if (idx >= 0)
+                slot = ((int64_t) idx << p.tpb_log2) + (pos & (p.tpb - 1));
+        }
+    }
+    p.slot_map[t] = slot;
+}
+
+// ---------------------------------------------------------------------------------------------- accepted path
+// One wave per sequence walks its tree from node 0: from node c it goes to the lowest child (parent c, index > c) whose drafted
+// token is the model's token after c.  The nodes sit in registers, 4 per lane (256 nodes; larger trees re-read memory): a step
+// is a compare, a ballot and a lane read, so the call costs one round trip to memory and a launch.
+__global__ __launch_bounds__(256) void tree_accept_kernel(const int32_t* draft_tokens, const int32_t* parents,
+    const int32_t* target_tokens, const int32_t* draft_offsets, int32_t* accept_path, int32_t* accept_counts,
+    int32_t* accepted_tokens, int batch, int num_tokens, int max_path)
+{
+    const int lane = threadIdx.x & 63;
+    const int b = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+    if (b >= batch)
+        return;
+    const int off = draft_offsets[b];
+    const int64_t n64 = (int64_t) draft_offsets[b + 1] - off;
+    const int n = off >= 0 && n64 > 0 && off + n64 <= num_tokens ? (int) n64 : 0;
+    constexpr int R = 4;
+    int tok[R], par[R], tgt[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+    {
+        const int i = lane + 64 * r;
+        const bool in = i < n;
+        tok[r] = in ? draft_tokens[off + i] : 0;
+        par[r] = in ? parents[off + i] : -1;
+        tgt[r] = in ? target_tokens[off + i] : 0;
+    }
+    int32_t* path = accept_path + (size_t) b * max_path;
+    int32_t* said = accepted_tokens + (size_t) b * max_path;
+    int cur = n > 0 ? 0 : -1, count = 0;
+    while (cur >= 0 && count < max_path)
+    {
+        int want = 0;
+        if (cur < 64 * R)
+        {
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+                want = cur >> 6 == r ? __builtin_amdgcn_readlane(tgt[r], cur & 63) : want;
+        }
+        else
+            want = target_tokens[off + cur];
+        if (lane == 0)
+        {
+            path[count] = cur;
+            said[count] = want;
+        }
+        ++count;
+        int next = -1;
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+        {
+            const int i = lane + 64 * r;
+            const uint64_t hit = __ballot(i < n && i > cur && par[r] == cur && tok[r] == want);
+            if (next < 0 && hit)
+                next = 64 * r + __builtin_ctzll(hit);
+        }
+        for (int i0 = 64 * R; next < 0 && i0 < n; i0 += 64)
+        {
+            const int i = i0 + lane;
+            const uint64_t hit = __ballot(i < n && i > cur && parents[off + min(i, n - 1)] == cur && draft_tokens[off + min(i, n - 1)] == want);
+            if (hit)
+                next = i0 + __builtin_ctzll(hit);
+        }
+        cur = __builtin_amdgcn_readfirstlane(next);
+    }
+    for (int i = count + lane; i < max_path; i += 64)
+    {
+        path[i] = -1;
+        said[i] = -1;
+    }
+    if (lane == 0)
+        accept_counts[b] = count;
+}
+
+// ---------------------------------------------------------------------------------------------- commit
+// Slot past + i of every pool takes the keys and values of slot past + path[i].  In place: paths rise strictly (a parent's
+// index is below its children's), so slot past + i is never a source of a later entry, and a thread owns the same bytes
+// of a row for all entries: it loads 8 entries, then stores them.
+// grid (batch, pools), 256 threads over K / V x heads x row chunks: bound by the rows it moves.
+template <typename V>
+__global__ __launch_bounds__(256) void commit_path_kernel(const int64_t* block_pointers, const int32_t* past_lengths,
+    const int32_t* accept_path, const int32_t* accept_counts, int32_t* new_lengths, int batch, int max_blocks, int tpb_log2,
+    int num_kv_heads, int row_bytes, int max_path)
+{
+    constexpr int E = 8; // entries per round
+    __shared__ int64_t src[2][E], dst[2][E];
+    const int b = blockIdx.x, pool = blockIdx.y, tid = threadIdx.x;
+    const int past = past_lengths[b];
+    const int count = min(accept_counts[b], max_path);
+    const int32_t* path = accept_path + (size_t) b * max_path;
+    const int64_t* kp = block_pointers + ((size_t) pool * batch + b) * 2 * max_blocks;
+    bool bad = past < 0 || count < 0;
+    for (int i = tid; i < count && !bad; i += 256)
+    {
+        const int node = path[i];
+        const int64_t pos = (int64_t) past + node;
+        bad = node < 0 || (i > 0 && path[i - 1] >= node) || (pos >> tpb_log2) >= max_blocks;
+        if (!bad)
+            for (int kv = 0; kv < 2; ++kv)
+                bad |= kp[kv * max_blocks + (pos >> tpb_log2)] == 0 || kp[kv * max_blocks + ((past + i) >> tpb_log2)] == 0;
+    }
+    bad = __syncthreads_or(bad);
+    if (pool == 0 && tid == 0)
+        new_lengths[b] = bad ? past : past + count;
+    if (bad)
+        return;
+    const int tpb_mask = (1 << tpb_log2) - 1;
+    const int chunks = row_bytes / (int) sizeof(V), work = 2 * num_kv_heads * chunks;
+    for (int i0 = 0; i0 < count; i0 += E)
+    {
+        __syncthreads(); // the previous round's addresses have been read
+        if (tid < 2 * E)
+        {
+            const int kv = tid / E, i = i0 + tid % E;
+            if (i < count)
+            {
+                const int s = past + path[i], d = past + i;
+                src[kv][tid % E] = kp[kv * max_blocks + (s >> tpb_log2)] + (int64_t) (s & tpb_mask) * row_bytes;
+                dst[kv][tid % E] = kp[kv * max_blocks + (d >> tpb_log2)] + (int64_t) (d & tpb_mask) * row_bytes;
+            }
+            else
+                src[kv][tid % E] = dst[kv][tid % E] = 0;
+        }
+        __syncthreads();
+        for (int w = tid; w < work; w += 256)
+        {
+            const int kv = w / (num_kv_heads * chunks), hc = w % (num_kv_heads * chunks), h = hc / chunks, c = hc % chunks;
+            const int64_t at = ((int64_t) h << tpb_log2) * row_bytes + (int64_t) c * sizeof(V);
+            V x[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (src[kv][e] != dst[kv][e])
+                    x[e] = *reinterpret_cast<const V*>(src[kv][e] + at);
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (src[kv][e] != dst[kv][e])
+                    *reinterpret_cast<V*>(dst[kv][e] + at) = x[e];
+        }
+    }
+}
+
+int log2_exact(int v, const char* what)
+{
+    MQ_CHECK(v > 0 && (v & (v - 1)) == 0 && v <= (1 << 20), "%s must be a power of 2, got %d", what, v);
+    int l = 0;
+    while ((1 << l) < v)
+        ++l;
+    return l;
+}
+
+// do [a, a + an) and [b, b + bn) share a byte
+bool overlap(const void* a, size_t an, const void* b, size_t bn)
+{
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return a && b && x < y + bn && y < x + an;
+}
+} // namespace
+
+size_t kv_block_tables_workspace_size(int batch)
+{
+    MQ_CHECK(batch >= 0 && batch <= 65535, "batch %d", batch);
+    return (size_t) batch * sizeof(int4);
+}
+
+void kv_block_tables(const mi355q_kv_block_tables_params& q, hipStream_t stream)
+{
+    MQ_CHECK(q.batch >= 0 && q.batch <= 65535, "batch %d", q.batch);
+    MQ_CHECK(q.max_blocks_per_seq > 0 && q.max_blocks_per_seq <= (1 << 24), "max_blocks_per_seq %d", q.max_blocks_per_seq);
+    MQ_CHECK(q.num_blocks > 0 && q.num_pools >= 0 && q.num_tokens >= 0, "num_blocks %d, num_pools %d, num_tokens %d", q.num_blocks,
+        q.num_pools, q.num_tokens);
+    MQ_CHECK(q.block_bytes > 0, "block_bytes %lld", (long long) q.block_bytes);
+    TableArgs a{};
+    a.tpb_log2 = log2_exact(q.tokens_per_block, "tokens_per_block");
+    if (q.batch == 0)
+        return;
+    MQ_CHECK(q.past_lengths && q.new_lengths && q.block_table && q.block_counts && q.block_counts_out && q.free_blocks && q.free_state
+            && q.free_state_out && q.token_offsets && q.status,
+        "null tensor");
+    MQ_CHECK(q.num_pools == 0 || (q.pool_bases && q.block_pointers), "null pool_bases / block_pointers");
+    MQ_CHECK(q.num_tokens == 0 || q.slot_map, "null slot_map");
+    MQ_CHECK(q.workspace && q.workspace_bytes >= kv_block_tables_workspace_size(q.batch) && (reinterpret_cast<uintptr_t>(q.workspace) & 15) == 0,
+        "workspace too small: %zu < %zu (or not 16-byte aligned)", q.workspace_bytes, kv_block_tables_workspace_size(q.batch));
+    const size_t rows = (size_t) q.batch * sizeof(int32_t);
+    MQ_CHECK(!overlap(q.past_lengths, rows, q.block_counts_out, rows) && !overlap(q.past_lengths, rows, q.token_offsets, rows + 4)
+            && !overlap(q.past_lengths, rows, q.status, rows),
+        "past_lengths overlaps an output");
+    MQ_CHECK(q.block_counts == q.block_counts_out || !overlap(q.block_counts, rows, q.block_counts_out, rows),
+        "block_counts_out overlaps block_counts without being it");
+    a.past_lengths = q.past_lengths;
+    a.new_lengths = q.new_lengths;
+    a.block_table = q.block_table;
+    a.block_counts = q.block_counts;
+    a.block_counts_out = q.block_counts_out;
+    a.free_blocks = q.free_blocks;
+    a.free_state = q.free_state;
+    a.free_state_out = q.free_state_out;
+    a.pool_bases = q.pool_bases;
+    a.block_pointers = q.block_pointers;
+    a.token_offsets = q.token_offsets;
+    a.slot_map = q.slot_map;
+    a.status = q.status;
+    a.rows = static_cast<int4*>(q.workspace);
+    a.block_bytes = q.block_bytes;
+    a.batch = q.batch;
+    a.max_blocks = q.max_blocks_per_seq;
+    a.num_blocks = q.num_blocks;
+    a.num_pools = q.num_pools;
+    a.num_tokens = q.num_tokens;
+    a.tpb = q.tokens_per_block;
+    hipLaunchKernelGGL(table_plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, stream, a);
+    MQ_HIP(hipGetLastError());
+    // the pools are dealt over enough workgroups to fill the chip (a table entry is read once per group)
+    const int per_pool = (q.max_blocks_per_seq + 511) / 512 * q.batch;
+    const int pool_groups = std::max(1, std::min(q.num_pools, (1024 + per_pool - 1) / per_pool));
+    a.pools_per_wg = std::max(1, (q.num_pools + pool_groups - 1) / pool_groups);
+    const int planes = q.num_pools ? (q.num_pools + a.pools_per_wg - 1) / a.pools_per_wg : 0;
+    const dim3 g((q.max_blocks_per_seq + 511) / 512, q.batch, planes + 1);
+    if (q.max_blocks_per_seq % 2 == 0 && (reinterpret_cast<uintptr_t>(q.block_pointers) & 15) == 0)
+        hipLaunchKernelGGL(table_fill_kernel<true>, g, dim3(256), 0, stream, a);
+    else
+        hipLaunchKernelGGL(table_fill_kernel<false>, g, dim3(256), 0, stream, a);
+    MQ_HIP(hipGetLastError());
+    if (q.num_tokens > 0)
+    {
+        hipLaunchKernelGGL(table_slots_kernel, dim3((q.num_tokens + 255) / 256), dim3(256), 0, stream, a);
+        MQ_HIP(hipGetLastError());
+    }
+}
+
+void draft_tree_accept(const mi355q_draft_tree_accept_params& q, hipStream_t stream)
+{
+    MQ_CHECK(q.batch >= 0 && q.num_tokens >= 0 && q.max_path > 0, "batch %d, num_tokens %d, max_path %d", q.batch, q.num_tokens, q.max_path);
+    if (q.batch == 0)
+        return;
+    MQ_CHECK(q.draft_offsets && q.accept_path && q.accept_counts && q.accepted_tokens, "null tensor");
+    MQ_CHECK(q.num_tokens == 0 || (q.draft_tokens && q.parents && q.target_tokens), "null tensor");
+    hipLaunchKernelGGL(tree_accept_kernel, dim3((q.batch + 3) / 4), dim3(256), 0, stream, q.draft_tokens, q.parents, q.target_tokens,
+        q.draft_offsets, q.accept_path, q.accept_counts, q.accepted_tokens, q.batch, q.num_tokens, q.max_path);
+    MQ_HIP(hipGetLastError());
+}
+
+void kv_commit_path(const mi355q_kv_commit_path_params& q, hipStream_t stream)
+{
+    MQ_CHECK(q.batch >= 0 && q.num_pools > 0 && q.num_pools <= 65535 && q.max_path > 0, "batch %d, num_pools %d, max_path %d", q.batch,
+        q.num_pools, q.max_path);
+    MQ_CHECK(q.max_blocks_per_seq > 0 && q.num_kv_heads > 0, "max_blocks_per_seq %d, num_kv_heads %d", q.max_blocks_per_seq, q.num_kv_heads);
+    MQ_CHECK(q.kv_type == MI355Q_HALF || q.kv_type == MI355Q_BF16 || q.kv_type == MI355Q_INT8 || q.kv_type == MI355Q_FP8, "kv cache type %d",
+        q.kv_type);
+    MQ_CHECK(q.head_size > 0 && q.head_size <= 4096 && q.head_size % 8 == 0, "head_size %d (multiples of 8)", q.head_size);
+    const int tpb_log2 = log2_exact(q.tokens_per_block, "tokens_per_block");
+    if (q.batch == 0)
+        return;
+    MQ_CHECK(q.block_pointers && q.past_lengths && q.accept_path && q.accept_counts && q.new_lengths, "null tensor");
+    const size_t rows = (size_t) q.batch * sizeof(int32_t);
+    // every pool's workgroups read the lengths that pool 0's replace
+    MQ_CHECK(!overlap(q.new_lengths, rows, q.past_lengths, rows) && !overlap(q.new_lengths, rows, q.accept_counts, rows)
+            && !overlap(q.new_lengths, rows, q.accept_path, rows * q.max_path),
+        "new_lengths overlaps an input");
+    const int row_bytes = q.head_size * (int) dtype_size(q.kv_type);
+    const dim3 g(q.batch, q.num_pools);
+    if (row_bytes % 16 == 0)
+        hipLaunchKernelGGL(commit_path_kernel<uint4>, g, dim3(256), 0, stream, q.block_pointers, q.past_lengths, q.accept_path,
+            q.accept_counts, q.new_lengths, q.batch, q.max_blocks_per_seq, tpb_log2, q.num_kv_heads, row_bytes, q.max_path);
+    else
+        hipLaunchKernelGGL(commit_path_kernel<uint2>, g, dim3(256), 0, stream, q.block_pointers, q.past_lengths, q.accept_path,
+            q.accept_counts, q.new_lengths, q.batch, q.max_blocks_per_seq, tpb_log2, q.num_kv_heads, row_bytes, q.max_path);
+    MQ_HIP(hipGetLastError());
+}
+
+} // namespace mi355q

@@ -135,4 +135,14 @@ void masked_multihead_attention_static(const mi355q_decode_attention_params& q, 
 size_t context_attention_workspace_size(const mi355q_context_attention_params& q);
 void context_attention(const mi355q_context_attention_params& q, hipStream_t stream);
 
+// tree_attn.hip
+size_t tree_attention_workspace_size(const mi355q_tree_attention_params& q);
+void tree_attention(const mi355q_tree_attention_params& q, hipStream_t stream);
+
+// draft_tree.hip
+size_t kv_block_tables_workspace_size(int batch);
+void kv_block_tables(const mi355q_kv_block_tables_params& q, hipStream_t stream);
+void draft_tree_accept(const mi355q_draft_tree_accept_params& q, hipStream_t stream);
+void kv_commit_path(const mi355q_kv_commit_path_params& q, hipStream_t stream);
+
 } // namespace mi355q

@@ -2226,6 +2226,65 @@ extern "C"
             });
     }
 
+    size_t mi355q_tree_attention_workspace_size(const mi355q_tree_attention_params* params)
+    {
+        size_t res = 0;
+        guarded(
+            [&]
+            {
+                MQ_CHECK(params, "null argument");
+                res = tree_attention_workspace_size(*params);
+            });
+        return res;
+    }
+
+    mi355q_status mi355q_tree_attention(const mi355q_tree_attention_params* params, void* stream)
+    {
+        return guarded(
+            [&]
+            {
+                MQ_CHECK(params, "null argument");
+                tree_attention(*params, static_cast<hipStream_t>(stream));
+            });
+    }
+
+    size_t mi355q_kv_block_tables_workspace_size(int32_t batch)
+    {
+        size_t res = 0;
+        guarded([&] { res = kv_block_tables_workspace_size(batch); });
+        return res;
+    }
+
+    mi355q_status mi355q_kv_block_tables(const mi355q_kv_block_tables_params* params, void* stream)
+    {
+        return guarded(
+            [&]
+            {
+                MQ_CHECK(params, "null argument");
+                kv_block_tables(*params, static_cast<hipStream_t>(stream));
+            });
+    }
+
+    mi355q_status mi355q_draft_tree_accept(const mi355q_draft_tree_accept_params* params, void* stream)
+    {
+        return guarded(
+            [&]
+            {
+                MQ_CHECK(params, "null argument");
+                draft_tree_accept(*params, static_cast<hipStream_t>(stream));
+            });
+    }
+
+    mi355q_status mi355q_kv_commit_path(const mi355q_kv_commit_path_params* params, void* stream)
+    {
+        return guarded(
+            [&]
+            {
+                MQ_CHECK(params, "null argument");
+                kv_commit_path(*params, static_cast<hipStream_t>(stream));
+            });
+    }
+
     size_t mi355q_allreduce_max_workspace_size(int32_t worldSize)
     {
         return worldSize <= 2 ? 16 * 1000 * 1000 : 8 * 1000 * 1000;

@@ -1,0 +1,973 @@
+// tree_attn.hip -- attention of a tree of drafted tokens over the paged cache: the generation step of speculative decoding,
+// where the model scores n candidate tokens (nodes) of a sequence at once.
+//
+// Node i of sequence b is row draft_offsets[b] + i of qkv, sits at position past + position_offsets[row] and owns the cache
+// slot past + i.  For every query head
+//     out[i] = sum_t softmax_t(q_i . k_t / (sqrt(Dh) q_scaling)) v_t   over t < past and the nodes t = past + j of i's mask,
+// and 0 where nothing is visible.  Three launches:
+//   1. tree_prepare_kernel: bias and rotation of q, k, v; K / V of every node rounded ONCE to the cache's type and stored
+//      in its slot; q, times the score scale, to the workspace.  One workgroup per sequence checks its lengths and blocks.
+//   2. tree_attn_kernel: flash attention of the nodes over the cache (K / V of the nodes come from the cache too, so a
+//      later step over the accepted tokens sees the values that were scored).
+//   3. tree_combine_kernel, where the keys of a sequence were split over workgroups: joins the partial states.
+#include "attn_mfma.h"
+#include "decode_common.h"
+
+namespace mi355q
+{
+namespace
+{
+
+constexpr int TREE_KT = 64;         // keys per tile
+constexpr int TREE_THREADS = 256;   // 4 waves
+constexpr int TREE_MAX_SPLITS = 64; // lane = split in the combine kernel
+constexpr int TREE_MAX_DRAFT = 1024;
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct TreeArgs
+{
+    const uint16_t* qkv;
+    const uint16_t* qkv_bias;
+    uint16_t* out;
+    const int32_t* past_lengths;
+    const int32_t* draft_offsets;
+    const int32_t* position_offsets; // or null: the node's index
+    const uint32_t* tree_mask;
+    const int64_t* block_ptrs;
+    const float* kv_scale_orig_quant;
+    const float* kv_scale_quant_orig;
+    uint16_t* q_ws;      // [tokens][Hq][DP] T: rotated, times the score scale (and the K dequantisation) and log2(e)
+    int32_t* seq_nodes;  // [batch]: nodes of the sequence, 0 if it is skipped
+    float* part_acc;     // [splits][tokens * Hq][DP]
+    float2* part_ml;     // [splits][tokens * Hq] (running maximum in the log2 domain, sum)
+    int64_t qkv_stride;
+    int batch, num_heads, num_kv_heads, group, hs;
+    int num_tokens, max_draft, max_past, mask_words;
+    int max_blocks, tpb_log2;
+    int mtiles, chunk_tiles, splits, groups; // groups = batch * kv heads * splits
+    int pos_type, rot_dim, rot_scale_type, rot_max_pos;
+    double rot_log2_base, rot_scale;
+    float score_scale;
+};
+
+// The sequence's rows, from device memory: false when the lengths do not fit what the host was told, so that nothing is
+// read or written outside the tensors (such a sequence is skipped).
+__device__ __forceinline__ bool tree_seq(const TreeArgs& p, int b, int& off, int& n, int& past)
+{
+    off = p.draft_offsets[b];
+    n = p.draft_offsets[b + 1] - off;
+    past = p.past_lengths[b];
+    const int64_t end = (int64_t) off + n, keys = (int64_t) past + n;
+    return off >= 0 && n > 0 && n <= p.max_draft && end <= p.num_tokens && past >= 0 && past <= p.max_past
+        && keys <= ((int64_t) p.max_blocks << p.tpb_log2);
+}
+
+// ---------------------------------------------------------------------------------------------- 1. prepare
+// grid (max_draft + 1, batch).  Rotation and quantisation of K / V run in 64 bits: the angle of a far position has no
+// correct digits left in fp32 (position 2^17, fp32 angle: error 2^-8 rad), and a value next to a rounding border of the
+// cache's type lands on the side the definition says.  It costs nothing that shows: 2 Hkv Dh values per token against the
+// whole history that the attention reads.
+template <typename T, int KVT>
+__global__ __launch_bounds__(TREE_THREADS) void tree_prepare_kernel(TreeArgs p, int dp)
+{
+    const int b = blockIdx.y, i = blockIdx.x;
+    int off, n, past;
+    const bool ok = tree_seq(p, b, off, n, past);
+    const int tpb = 1 << p.tpb_log2;
+    const int64_t* kp = p.block_ptrs + (size_t) b * 2 * p.max_blocks;
+    if (i == p.max_draft)
+    {
+        // every block the sequence's keys live in has to be there (0 = not allocated)
+        bool bad = !ok;
+        if (ok)
+            for (int j = threadIdx.x; j < (past + n + tpb - 1) >> p.tpb_log2; j += TREE_THREADS)
+                bad |= kp[j] == 0 || kp[p.max_blocks + j] == 0;
+        bad = __syncthreads_or(bad);
+        if (threadIdx.x == 0)
+            p.seq_nodes[b] = bad ? 0 : n;
+        return;
+    }
+    if (!ok || i >= n)
+        return;
+    const int row = off + i, hs = p.hs;
+    const int Hq = p.num_heads, Hkv = p.num_kv_heads;
+    const bool rope = p.pos_type == 1 || p.pos_type == 2;
+    const int half = p.rot_dim >> 1;
+    __shared__ double cs_tab[128], sn_tab[128];
+    if (rope && (int) threadIdx.x < half)
+    {
+        const int pos = past + (p.position_offsets ? p.position_offsets[row] : i);
+        double log2_base = p.rot_log2_base, scale = p.rot_scale;
+        if (p.rot_scale_type == 2) // dynamic NTK: the base grows with the length once that passes the trained one
+        {
+            if (pos > p.rot_max_pos)
+                log2_base += log2(pos * (scale / p.rot_max_pos) - (scale - 1.0)) * p.rot_dim / (p.rot_dim - 2);
+            scale = 1.0;
+        }
+        else if (p.rot_scale_type == 1)
+            scale = 1.0 / scale;
+        else
+            scale = 1.0;
+        const double turns = pos * scale * exp2(-log2_base * (2 * (int) threadIdx.x) / p.rot_dim) * 0.15915494309189535;
+        double sn, cs;
+        sincospi(2.0 * (turns - rint(turns)), &sn, &cs);
+        cs_tab[threadIdx.x] = cs;
+        sn_tab[threadIdx.x] = sn;
+    }
+    __syncthreads();
+    const uint16_t* src = p.qkv + (size_t) row * p.qkv_stride;
+    const int cpv = dp / 8, nvec = Hq + 2 * Hkv; // 8-element chunks per head
+    const float qscale = p.score_scale * LOG2E * (KVT ? p.kv_scale_quant_orig[0] : 1.f);
+    const double kvq = KVT ? (double) p.kv_scale_orig_quant[0] : 1.0;
+    const int slot = past + i, blk = slot >> p.tpb_log2, tin = slot & (tpb - 1);
+    char* const kdst = reinterpret_cast<char*>(kp[blk]);
+    char* const vdst = reinterpret_cast<char*>(kp[p.max_blocks + blk]);
+    for (int it = threadIdx.x; it < nvec * cpv; it += TREE_THREADS)
+    {
+        const int vec = it / cpv, d0 = 8 * (it % cpv);
+        uint4* const qdst = reinterpret_cast<uint4*>(p.q_ws + ((size_t) row * Hq + vec) * dp + d0);
+        if (d0 >= hs) // the padding of the workspace rows
+        {
+            if (vec < Hq)
+                *qdst = make_uint4(0, 0, 0, 0);
+            continue;
+        }
+        auto element = [&](int d) -> double // q / k / v element d of this head, bias added
+        {
+            const double x = T16<T>::to_float(src[vec * hs + d]);
+            return p.qkv_bias ? x + T16<T>::to_float(p.qkv_bias[vec * hs + d]) : x;
+        };
+        const uint4 r = *reinterpret_cast<const uint4*>(src + vec * hs + d0);
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+        double x[8], y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            x[e] = (e & 1) ? T16<T>::hi(w[e >> 1]) : T16<T>::lo(w[e >> 1]);
+        if (p.qkv_bias)
+        {
+            const uint4 rb = *reinterpret_cast<const uint4*>(p.qkv_bias + vec * hs + d0);
+            const uint32_t wb[4] = {rb.x, rb.y, rb.z, rb.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                x[e] += (e & 1) ? T16<T>::hi(wb[e >> 1]) : T16<T>::lo(wb[e >> 1]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            y[e] = x[e];
+        if (rope && vec < Hq + Hkv && d0 < p.rot_dim)
+        {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+            {
+                const int d = d0 + e;
+                if (d < p.rot_dim)
+                {
+                    // NeoX pairs (d, d + rot_dim / 2), GPT-J pairs (2 j, 2 j + 1)
+                    const bool first = p.pos_type == 2 ? d < half : !(e & 1);
+                    const int j = p.pos_type == 2 ? (first ? d : d - half) : d >> 1;
+                    const double other = p.pos_type == 2 ? element(first ? d + half : d - half) : x[e ^ 1];
+                    y[e] = first ? x[e] * cs_tab[j] - other * sn_tab[j] : x[e] * cs_tab[j] + other * sn_tab[j];
+                }
+            }
+        }
+        if (vec < Hq)
+        {
+            // q carries the score scale, the K dequantisation and log2(e): the matrix product then IS the exponent.  One
+            // rounding to T, as many bits as q had
+            uint32_t o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                o[e] = pack2<T>((float) (y[2 * e] * qscale), (float) (y[2 * e + 1] * qscale));
+            *qdst = make_uint4(o[0], o[1], o[2], o[3]);
+            continue;
+        }
+        const int kv = (vec - Hq) / Hkv, hk = (vec - Hq) % Hkv;
+        char* const base = kv ? vdst : kdst;
+        if (!base)
+            continue;
+        const size_t e0 = ((size_t) hk * tpb + tin) * hs + d0;
+        if constexpr (KVT == 0)
+        {
+            uint32_t o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                o[e] = pack2<T>((float) y[2 * e], (float) y[2 * e + 1]);
+            *reinterpret_cast<uint4*>(base + 2 * e0) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+        else
+        {
+            uint32_t o[2] = {0, 0};
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+            {
+                const double z = y[e] * kvq;
+                const uint32_t c = KVT == 1 ? float_to_int8_sat((float) rint(z)) : float_to_fp8((float) z);
+                o[e >> 2] |= c << (8 * (e & 3));
+            }
+            *reinterpret_cast<uint2*>(base + e0) = make_uint2(o[0], o[1]);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- 2. attention
+template <typename T>
+__device__ __forceinline__ cf32x4_t tree_mfma16(const uint2& a, const uint2& b, cf32x4_t c);
+template <>
+__device__ __forceinline__ cf32x4_t tree_mfma16<bf16_t>(const uint2& a, const uint2& b, cf32x4_t c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(
+        __builtin_bit_cast(cs16x4_t, a), __builtin_bit_cast(cs16x4_t, b), c, 0, 0, 0);
+}
+template <>
+__device__ __forceinline__ cf32x4_t tree_mfma16<f16_t>(const uint2& a, const uint2& b, cf32x4_t c)
+{
+    typedef __attribute__((ext_vector_type(4))) _Float16 f16x4_t;
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4_t, a), __builtin_bit_cast(f16x4_t, b), c, 0, 0, 0);
+}
+
+// 8 cache bytes -> 8 values of T (exact: int8 and e4m3 have at most 8 significant bits)
+template <typename T, int KVT>
+__device__ __forceinline__ uint4 tree_kv8_to_t(uint32_t w0, uint32_t w1)
+{
+    const uint32_t w[2] = {w0, w1};
+    uint32_t o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        o[i] = pack2<T>(kv8_to_float<KVT>(w[i >> 1], 2 * (i & 1)), kv8_to_float<KVT>(w[i >> 1], 2 * (i & 1) + 1));
+    return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+// does a dword of two T values hold an infinity or NaN
+template <typename T>
+__device__ __forceinline__ bool tree_nonfinite2(uint32_t w)
+{
+    constexpr uint32_t EXP = T16<T>::is_bf16 ? 0x7f80u : 0x7c00u;
+    return (w & EXP) == EXP || ((w >> 16) & EXP) == EXP;
+}
+
+// 64 bits of a mask row from bit `s0` on; bits below 0 (keys of the history) read as 1, past the row as 0
+__device__ __forceinline__ uint64_t tree_mask64(const uint32_t* row, int words, int n, int s0)
+{
+    uint64_t v = 0;
+    const int w0 = s0 >> 5, sh = s0 & 31; // arithmetic shift: floor
+    uint32_t w[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+    {
+        const int j = w0 + i;
+        w[i] = (j >= 0 && j < words) ? row[j] : 0u;
+    }
+    v = ((uint64_t) w[1] << 32 | w[0]) >> sh;
+    if (sh)
+        v |= (uint64_t) w[2] << (64 - sh);
+    if (s0 < 0)
+        v |= s0 <= -64 ? ~0ull : (1ull << -s0) - 1;
+    const int live = n - s0; // keys of the window that exist
+    return live >= 64 ? v : (live <= 0 ? 0ull : v & ((1ull << live) - 1));
+}
+
+// grid: 1-D, ((group / 8) * mtiles + m) * 8 + group % 8 with group = (sequence, kv head, split): workgroups are dealt to the
+// 8 XCDs round-robin, so the m-tiles that share a stretch of keys run on one XCD and read it from HBM once.
+// A workgroup = RW * QT * 16 query rows (row r = node r / G, head r % G of the kv head's G query heads) x chunk_tiles tiles of
+// 64 keys.  Its 4 waves are RW row groups x KW key groups: with few rows the waves share the keys of a tile instead of
+// idling, and merge their states at the end.
+// S^T = K . Q^T (16x16x32): a lane holds one query column's scores of 4 consecutive keys, and the same registers, rounded
+// to T, are the B operand of O^T += V^T . P^T.
+// Softmax in the log2 domain with the running maximum as the C operand of the first product: what comes out is already
+// s - m, and as long as no column grows past m + 8 (p <= 256: harmless in T and in the fp32 sums) nothing is rescaled.
+// Whether one does is an integer maximum over the raw bits (negative floats are negative integers).
+template <typename T, int KVT, int DP, int RW, int KW, int QT>
+__global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP > 128 ? 1 : 2))) void tree_attn_kernel(TreeArgs p)
+{
+    static_assert(RW * KW == 4, "4 waves");
+    constexpr int M = RW * QT * 16;
+    constexpr int KS = DP / 32, DT = DP / 16;
+    constexpr int ROWB = DP * 2, CH = ROWB / 16;
+    constexpr int TILE_BYTES = TREE_KT * ROWB, STAGE_BYTES = 2 * TILE_BYTES;
+    constexpr int XW = 4 / KW;                      // 16-key subtiles per wave
+    constexpr int RPD = 1024 / ROWB, DPW = TREE_KT / RPD / 4; // 16-bit caches: rows per DMA instruction, DMAs per wave
+    constexpr int CH8 = DP / 16, LPT = TREE_KT * CH8 / TREE_THREADS; // 8-bit caches: 16-byte loads per thread and tile
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE_BYTES];
+    __shared__ uint32_t nonfinite[2]; // keys of the tile whose V row has an infinity or NaN
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int rw = wave % RW, kw = wave / RW;
+    const int lr = lane & 15, lq = lane >> 4;
+    const int mt = (blockIdx.x >> 3) % p.mtiles;
+    const int grp = (blockIdx.x >> 3) / p.mtiles * 8 + (blockIdx.x & 7);
+    if (grp >= p.groups)
+        return;
+    const int split = grp % p.splits, hk = grp / p.splits % p.num_kv_heads, b = grp / p.splits / p.num_kv_heads;
+    const int n = p.seq_nodes[b], G = p.group;
+    if (mt * M >= n * G)
+        return;
+    const int off = p.draft_offsets[b], past = p.past_lengths[b], total = past + n;
+    const int ntiles = (total + TREE_KT - 1) / TREE_KT;
+    const int tile_lo = split * p.chunk_tiles, tile_hi = min(ntiles, tile_lo + p.chunk_tiles);
+    if (tile_lo >= ntiles)
+        return;
+    const bool alone = ntiles <= p.chunk_tiles; // the sequence was not split
+    const int hs = p.hs, tpb_mask = (1 << p.tpb_log2) - 1;
+    const int64_t* const kp = p.block_ptrs + (size_t) b * 2 * p.max_blocks;
+    const int64_t* const vp = kp + p.max_blocks;
+
+    auto ksw = [](int row) { return CH >= 16 ? (row & 15) : ((row >> 1) & 7); };
+    auto vsw = [](int row) { return (((row & 3) << 2) | ((row >> 2) & 3)) & (CH - 1); };
+
+    // ---- tile loads.  16-bit caches: LDS-DMA, instruction d of a tile fills LDS bytes [1024 d, +1024), the swizzle applied
+    // on the source address.  8-bit caches: through registers, converted to T on the way into the LDS.
+    const uint32_t lds_base = __builtin_amdgcn_readfirstlane((uint32_t) (uintptr_t) (ctx_lds_void_t*) lds);
+    const int last_chunk = hs * (KVT ? 1 : 2) / 16 - 1; // heads narrower than DP: the padding re-reads the last chunk (q is 0 there)
+    uint4 kreg[KVT ? LPT : 1], vreg[KVT ? LPT : 1];
+    auto load_tile = [&](int tile, int buf)
+    {
+        const int t0 = tile * TREE_KT;
+        if constexpr (KVT == 0)
+        {
+            const int drow = lane / CH, dch = lane % CH;
+#pragma unroll
+            for (int i = 0; i < DPW; ++i)
+            {
+                const int d = wave * DPW + i, row = d * RPD + drow;
+                const int t = min(t0 + row, total - 1); // rows past the sequence re-read its last one
+                const size_t at = ((size_t) hk << p.tpb_log2) + (t & tpb_mask);
+                const char* kb = reinterpret_cast<const char*>(kp[t >> p.tpb_log2]) + at * hs * 2;
+                const char* vb = reinterpret_cast<const char*>(vp[t >> p.tpb_log2]) + at * hs * 2;
+                const uint32_t dst = lds_base + buf * STAGE_BYTES + d * 1024;
+                ctx_dma16(kb + 16 * min(dch ^ ksw(row), last_chunk), dst);
+                ctx_dma16(vb + 16 * min(dch ^ vsw(row), last_chunk), dst + TILE_BYTES);
+            }
+        }
+        else
+        {
+#pragma unroll
+            for (int i = 0; i < LPT; ++i)
+            {
+                const int c = tid + i * TREE_THREADS, row = c / CH8, ch = min(c % CH8, last_chunk);
+                const int t = min(t0 + row, total - 1);
+                const size_t at = ((size_t) hk << p.tpb_log2) + (t & tpb_mask);
+                kreg[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(kp[t >> p.tpb_log2]) + at * hs + 16 * ch);
+                vreg[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(vp[t >> p.tpb_log2]) + at * hs + 16 * ch);
+            }
+        }
+    };
+    auto store_tile = [&](int buf) // 8-bit caches
+    {
+        if constexpr (KVT != 0)
+        {
+#pragma unroll
+            for (int i = 0; i < LPT; ++i)
+            {
+                const int c = tid + i * TREE_THREADS, row = c / CH8, ch = 2 * (c % CH8);
+                uint8_t* kt = lds + buf * STAGE_BYTES + ROWB * row;
+                uint8_t* vt = kt + TILE_BYTES;
+                *reinterpret_cast<uint4*>(kt + 16 * (ch ^ ksw(row))) = tree_kv8_to_t<T, KVT>(kreg[i].x, kreg[i].y);
+                *reinterpret_cast<uint4*>(kt + 16 * ((ch + 1) ^ ksw(row))) = tree_kv8_to_t<T, KVT>(kreg[i].z, kreg[i].w);
+                *reinterpret_cast<uint4*>(vt + 16 * (ch ^ vsw(row))) = tree_kv8_to_t<T, KVT>(vreg[i].x, vreg[i].y);
+                *reinterpret_cast<uint4*>(vt + 16 * ((ch + 1) ^ vsw(row))) = tree_kv8_to_t<T, KVT>(vreg[i].z, vreg[i].w);
+            }
+        }
+    };
+
+    load_tile(tile_lo, tile_lo & 1);
+    // ---- Q^T fragments (B operand): column = row q0 + 16 qt + lr, k = d = 32 ks + 8 lq + j
+    const int q0 = mt * M + rw * QT * 16;
+    uint4 qf[QT][KS];
+    int node[QT];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt)
+    {
+        const int r = min(q0 + 16 * qt + lr, n * G - 1); // rows past the last re-read it; never stored
+        node[qt] = r / G;
+        const uint16_t* q = p.q_ws + ((size_t) (off + node[qt]) * p.num_heads + hk * G + r % G) * DP;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+            qf[qt][ks] = *reinterpret_cast<const uint4*>(q + 32 * ks + 8 * lq);
+    }
+    // end the compiler's own bookkeeping of the q loads here, before the loop's (to it invisible) DMAs
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+            asm volatile("" : "+v"(qf[qt][ks].x), "+v"(qf[qt][ks].y), "+v"(qf[qt][ks].z), "+v"(qf[qt][ks].w));
+
+    float m_run[QT], l_run[QT];
+    cf32x4_t minus_m[QT]; // C operand of the scores: -m, 0 while the column has no maximum yet
+    cf32x4_t o[QT][DT];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt)
+    {
+        m_run[qt] = NEG_BIG;
+        l_run[qt] = 0.f;
+        minus_m[qt] = cf32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+            o[qt][dt] = cf32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+    const int rq = lr >> 2, rp = lr & 3;
+    const int kb0 = kw * 16 * XW; // this wave's first key of a tile
+
+    auto compute = [&](int buf, int t0, bool tail)
+    {
+        const uint8_t* kt = lds + buf * STAGE_BYTES;
+        const uint8_t* vt = kt + TILE_BYTES;
+        cf32x4_t s[XW][QT];
+#pragma unroll
+        for (int x = 0; x < XW; ++x)
+        {
+            const int row = kb0 + 16 * x + lr;
+            uint4 kf[KS];
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+                kf[ks] = *reinterpret_cast<const uint4*>(kt + ROWB * row + 16 * ((4 * ks + lq) ^ ksw(row)));
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt)
+            {
+                s[x][qt] = minus_m[qt];
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks)
+                    s[x][qt] = ctx_mfma<T>(kf[ks], qf[qt][ks], s[x][qt]);
+            }
+        }
+        if (tail)
+        {
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt)
+            {
+                const uint64_t seen
+                    = tree_mask64(p.tree_mask + (size_t) (off + node[qt]) * p.mask_words, p.mask_words, n, t0 - past) >> (kb0 + 4 * lq);
+#pragma unroll
+                for (int x = 0; x < XW; ++x)
+#pragma unroll
+                    for (int rr = 0; rr < 4; ++rr)
+                        s[x][qt][rr] = (seen >> (16 * x + rr)) & 1 ? s[x][qt][rr] : -__builtin_inff();
+            }
+        }
+        uint32_t pk[QT][XW][2];
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt)
+        {
+            int mx = 0; // the largest positive s - m, as raw bits
+#pragma unroll
+            for (int x = 0; x < XW; ++x)
+#pragma unroll
+                for (int rr = 0; rr < 4; ++rr)
+                    mx = max(mx, __builtin_bit_cast(int, (float) s[x][qt][rr]));
+            const bool fresh = m_run[qt] == NEG_BIG;
+            if (__any(fresh || mx > 0x41000000 /* 8.0f */)) // wave-uniform
+            {
+                // the column's maximum of this tile, over its 4 lanes (a NaN stays out of the comparison and in the scores)
+                float top = -__builtin_inff();
+#pragma unroll
+                for (int x = 0; x < XW; ++x)
+#pragma unroll
+                    for (int rr = 0; rr < 4; ++rr)
+                        top = fmaxf(top, s[x][qt][rr]);
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const float up = top == -__builtin_inff() ? 0.f : (fresh ? top : fmaxf(top, 0.f));
+                const float corr = fresh ? 0.f : __builtin_amdgcn_exp2f(-up); // (nothing was summed before the first maximum)
+                if (top != -__builtin_inff())
+                {
+                    m_run[qt] = fresh ? up : m_run[qt] + up;
+                    minus_m[qt] = cf32x4_t{-m_run[qt], -m_run[qt], -m_run[qt], -m_run[qt]};
+                    l_run[qt] *= corr;
+                }
+                const float oc = top != -__builtin_inff() ? corr : 1.f;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                    for (int rr = 0; rr < 4; ++rr)
+                        o[qt][dt][rr] *= oc;
+#pragma unroll
+                for (int x = 0; x < XW; ++x)
+#pragma unroll
+                    for (int rr = 0; rr < 4; ++rr)
+                        s[x][qt][rr] -= up;
+            }
+#pragma unroll
+            for (int x = 0; x < XW; ++x)
+            {
+                float e[4];
+#pragma unroll
+                for (int rr = 0; rr < 4; ++rr)
+                {
+                    e[rr] = __builtin_amdgcn_exp2f(s[x][qt][rr]);
+                    l_run[qt] += e[rr];
+                }
+                // P in T: its relative rounding error (half a step of T) averages out over the keys
+                pk[qt][x][0] = pack2<T>(e[0], e[1]);
+                pk[qt][x][1] = pack2<T>(e[2], e[3]);
+            }
+        }
+        // ---- O^T += V^T . P^T  (A operand rows d = 16 dt + lr by the transposing LDS read)
+        if constexpr (XW >= 2)
+        {
+#pragma unroll
+            for (int kh = 0; kh < XW / 2; ++kh)
+            {
+                const int ra = kb0 + 32 * kh + 4 * lq + rq, rb = ra + 16;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+                {
+                    const int ch = 2 * dt + (rp >> 1), sub = 8 * (rp & 1);
+                    const cs16x4_t va
+                        = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_cs16x4_t*) (vt + ROWB * ra + 16 * (ch ^ vsw(ra)) + sub));
+                    const cs16x4_t vb
+                        = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_cs16x4_t*) (vt + ROWB * rb + 16 * (ch ^ vsw(rb)) + sub));
+                    const uint2 a2 = __builtin_bit_cast(uint2, va), b2 = __builtin_bit_cast(uint2, vb);
+                    const uint4 vf = make_uint4(a2.x, a2.y, b2.x, b2.y);
+#pragma unroll
+                    for (int qt = 0; qt < QT; ++qt)
+                        o[qt][dt] = ctx_mfma<T>(vf,
+                            make_uint4(pk[qt][2 * kh][0], pk[qt][2 * kh][1], pk[qt][2 * kh + 1][0], pk[qt][2 * kh + 1][1]), o[qt][dt]);
+                }
+            }
+        }
+        else
+        {
+            const int ra = kb0 + 4 * lq + rq;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+            {
+                const int ch = 2 * dt + (rp >> 1), sub = 8 * (rp & 1);
+                const cs16x4_t va
+                    = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_cs16x4_t*) (vt + ROWB * ra + 16 * (ch ^ vsw(ra)) + sub));
+#pragma unroll
+                for (int qt = 0; qt < QT; ++qt)
+                    o[qt][dt] = tree_mfma16<T>(__builtin_bit_cast(uint2, va), make_uint2(pk[qt][0][0], pk[qt][0][1]), o[qt][dt]);
+            }
+        }
+        if constexpr (KVT == 0)
+        {
+            // V rows of nodes with an infinity or NaN were zeroed for the products above (0 * inf would reach the columns
+            // that do not see them); the columns that do get those elements here
+            const uint64_t bad = tail ? ((uint64_t) nonfinite[1] << 32 | nonfinite[0]) : 0ull;
+            for (uint64_t left = bad; left; left &= left - 1)
+            {
+                const int k = __builtin_ctzll(left), t = t0 + k;
+                if (k < kb0 || k >= kb0 + 16 * XW)
+                    continue;
+                const size_t at = ((size_t) hk << p.tpb_log2) + (t & tpb_mask);
+                const uint16_t* v = reinterpret_cast<const uint16_t*>(vp[t >> p.tpb_log2]) + at * hs;
+#pragma unroll
+                for (int qt = 0; qt < QT; ++qt)
+                {
+                    const uint32_t* mrow = p.tree_mask + (size_t) (off + node[qt]) * p.mask_words;
+                    const bool sees = t < past || (((t - past) >> 5) < p.mask_words && (mrow[(t - past) >> 5] >> ((t - past) & 31)) & 1);
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                        for (int rr = 0; rr < 4; ++rr)
+                        {
+                            const int d = 16 * dt + 4 * lq + rr;
+                            if (sees && d < hs)
+                            {
+                                const uint32_t w = v[d];
+                                if (tree_nonfinite2<T>(w))
+                                    o[qt][dt][rr] += T16<T>::to_float(w);
+                            }
+                        }
+                }
+            }
+        }
+    };
+    // V rows of a tile with nodes, in the LDS: rows past the sequence are zeroed (whatever lies there, 0 * NaN is NaN), nodes'
+    // elements that are not finite are noted and zeroed.  History rows are seen by every column and stay as they are.
+    auto clean_tail = [&](int buf, int t0)
+    {
+        if (tid < 2)
+            nonfinite[tid] = 0;
+        __syncthreads();
+        uint8_t* vt = lds + buf * STAGE_BYTES + TILE_BYTES;
+        for (int c = tid; c < TREE_KT * CH; c += TREE_THREADS)
+        {
+            const int row = c / CH, t = t0 + row;
+            uint4* at = reinterpret_cast<uint4*>(vt + 16 * c);
+            if (t >= total)
+                *at = make_uint4(0, 0, 0, 0);
+            else if (KVT == 0 && t >= past)
+            {
+                uint4 w = *at;
+                uint32_t* x = reinterpret_cast<uint32_t*>(&w);
+                if (tree_nonfinite2<T>(x[0]) || tree_nonfinite2<T>(x[1]) || tree_nonfinite2<T>(x[2]) || tree_nonfinite2<T>(x[3]))
+                {
+                    constexpr uint32_t EXP = T16<T>::is_bf16 ? 0x7f80u : 0x7c00u;
+                    for (int e = 0; e < 4; ++e)
+                    {
+                        if ((x[e] & EXP) == EXP)
+                            x[e] &= 0xffff0000u;
+                        if (((x[e] >> 16) & EXP) == EXP)
+                            x[e] &= 0xffffu;
+                    }
+                    *at = w;
+                    atomicOr(&nonfinite[row >> 5], 1u << (row & 31));
+                }
+            }
+        }
+        __syncthreads();
+    };
+
+    if constexpr (KVT != 0)
+        store_tile(tile_lo & 1);
+    for (int i = tile_lo; i < tile_hi; ++i)
+    {
+        if constexpr (KVT == 0)
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // my share of tile i has landed
+        __syncthreads();                                     // everyone's has, and everyone is done with tile i - 1
+        if (i + 1 < tile_hi)
+            load_tile(i + 1, (i + 1) & 1);
+        const int t0 = i * TREE_KT;
+        const bool tail = t0 + TREE_KT > past; // uniform
+        if (tail)
+            clean_tail(i & 1, t0);
+        compute(i & 1, t0, tail);
+        if constexpr (KVT != 0)
+        {
+            if (i + 1 < tile_hi)
+                store_tile((i + 1) & 1);
+        }
+    }
+
+    // ---- the sum over the 4 lanes of a column, then the key groups of a row group through the LDS
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt)
+    {
+        l_run[qt] += __shfl_xor(l_run[qt], 16);
+        l_run[qt] += __shfl_xor(l_run[qt], 32);
+    }
+    if constexpr (KW > 1)
+    {
+        constexpr int STATE = QT * (DT + 1) * 64 * 16; // bytes of one wave's state: float4 per register group and lane
+        static_assert((KW - 1) * RW * STATE <= 2 * STAGE_BYTES, "states do not fit the tile buffers");
+        __syncthreads(); // everyone is done with the tiles
+        if (kw > 0)
+        {
+            cf32x4_t* st = reinterpret_cast<cf32x4_t*>(lds + ((kw - 1) * RW + rw) * STATE) + lane;
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt)
+            {
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+                    st[(qt * (DT + 1) + dt) * 64] = o[qt][dt];
+                st[(qt * (DT + 1) + DT) * 64] = cf32x4_t{m_run[qt], l_run[qt], 0.f, 0.f};
+            }
+        }
+        __syncthreads();
+        if (kw > 0)
+            return;
+#pragma unroll
+        for (int k = 1; k < KW; ++k)
+        {
+            const cf32x4_t* st = reinterpret_cast<const cf32x4_t*>(lds + ((k - 1) * RW + rw) * STATE) + lane;
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt)
+            {
+                const cf32x4_t ml = st[(qt * (DT + 1) + DT) * 64];
+                const float mm = fmaxf(m_run[qt], ml[0]);
+                const float c0 = __builtin_amdgcn_exp2f(m_run[qt] - mm), c1 = __builtin_amdgcn_exp2f(ml[0] - mm);
+                m_run[qt] = mm;
+                l_run[qt] = l_run[qt] * c0 + ml[1] * c1;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+                {
+                    const cf32x4_t x = st[(qt * (DT + 1) + dt) * 64];
+#pragma unroll
+                    for (int rr = 0; rr < 4; ++rr)
+                        o[qt][dt][rr] = o[qt][dt][rr] * c0 + x[rr] * c1;
+                }
+            }
+        }
+    }
+    const float v_deq = KVT ? p.kv_scale_quant_orig[0] : 1.f;
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt)
+    {
+        const int r = q0 + 16 * qt + lr;
+        if (r >= n * G)
+            continue;
+        const size_t head = (size_t) (off + r / G) * p.num_heads + hk * G + r % G;
+        if (alone)
+        {
+            // no visible key: the sum is exactly 0, and so is the row (a NaN sum stays a NaN)
+            const float inv = l_run[qt] == 0.f ? 0.f : v_deq / l_run[qt];
+            uint16_t* out = p.out + head * hs;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+                if (16 * dt + 4 * lq < hs)
+                    *reinterpret_cast<uint2*>(out + 16 * dt + 4 * lq) = make_uint2(
+                        pack2<T>(o[qt][dt][0] * inv, o[qt][dt][1] * inv), pack2<T>(o[qt][dt][2] * inv, o[qt][dt][3] * inv));
+        }
+        else
+        {
+            const size_t rec = (size_t) split * p.num_tokens * p.num_heads + head;
+            float* acc = p.part_acc + rec * DP;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+                *reinterpret_cast<cf32x4_t*>(acc + 16 * dt + 4 * lq) = o[qt][dt];
+            if (lq == 0)
+                p.part_ml[rec] = make_float2(m_run[qt], l_run[qt]);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- 3. combine
+// grid (max_draft, batch): one token; a wave takes the heads one after another.  Splits are summed in their order.
+template <typename T, int DP>
+__global__ __launch_bounds__(TREE_THREADS) void tree_combine_kernel(TreeArgs p, bool quantised)
+{
+    const int b = blockIdx.y, i = blockIdx.x, lane = threadIdx.x & 63;
+    const int n = p.seq_nodes[b];
+    if (i >= n)
+        return;
+    const int ntiles = (p.past_lengths[b] + n + TREE_KT - 1) / TREE_KT;
+    const int S = (ntiles + p.chunk_tiles - 1) / p.chunk_tiles; // <= 64
+    if (S <= 1)
+        return;
+    const float v_deq = quantised ? p.kv_scale_quant_orig[0] : 1.f;
+    const size_t row = p.draft_offsets[b] + i, stride = (size_t) p.num_tokens * p.num_heads;
+    constexpr int E = DP / 64;
+    for (int h = threadIdx.x >> 6; h < p.num_heads; h += TREE_THREADS / 64)
+    {
+        const size_t head = row * p.num_heads + h;
+        const float2 ml = p.part_ml[min(lane, S - 1) * stride + head];
+        const float m = lane < S ? ml.x : NEG_BIG;
+        float mm = m;
+#pragma unroll
+        for (int x = 32; x >= 1; x >>= 1)
+            mm = fmaxf(mm, __shfl_xor(mm, x));
+        const float c = lane < S ? __builtin_amdgcn_exp2f(m - mm) : 0.f;
+        float l = lane < S ? ml.y * c : 0.f;
+#pragma unroll
+        for (int x = 32; x >= 1; x >>= 1)
+            l += __shfl_xor(l, x);
+        float acc[E] = {};
+        for (int s = 0; s < S; ++s)
+        {
+            const float cs = __shfl(c, s);
+            const float* src = p.part_acc + (s * stride + head) * DP + E * lane;
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                acc[e] += src[e] * cs;
+        }
+        const float inv = l == 0.f ? 0.f : v_deq / l;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (E * lane + e < p.hs)
+                p.out[head * p.hs + E * lane + e] = T16<T>::from_float(acc[e] * inv);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- host
+struct TreePlan
+{
+    int dp, rows, rows_per_wg; // padded head size; query rows of a kv head at most; rows per workgroup
+    int mtiles, max_tiles, chunk_tiles, splits;
+    size_t q_bytes, seq_bytes, acc_bytes, ml_bytes;
+    size_t total() const
+    {
+        return q_bytes + seq_bytes + acc_bytes + ml_bytes;
+    }
+};
+size_t round256(size_t x)
+{
+    return (x + 255) / 256 * 256;
+}
+
+void tree_check(const mi355q_tree_attention_params& q)
+{
+    MQ_CHECK(q.act_type == MI355Q_HALF || q.act_type == MI355Q_BF16, "act_type %d", q.act_type);
+    MQ_CHECK(q.kv_type == q.act_type || q.kv_type == MI355Q_INT8 || q.kv_type == MI355Q_FP8, "kv cache type %d", q.kv_type);
+    MQ_CHECK(q.batch >= 0 && q.batch <= 65535 && q.num_heads > 0 && q.num_kv_heads > 0 && q.num_heads % q.num_kv_heads == 0,
+        "batch %d, heads %d / %d", q.batch, q.num_heads, q.num_kv_heads);
+    MQ_CHECK(q.head_size >= 8 && q.head_size <= 256 && q.head_size % (q.kv_type == q.act_type ? 8 : 16) == 0,
+        "tree attention: head_size %d (multiples of 8, with an 8-bit cache of 16, up to 256)", q.head_size);
+    MQ_CHECK(q.num_tokens >= 0 && q.max_draft_length >= 0 && q.max_draft_length <= TREE_MAX_DRAFT,
+        "num_tokens %d, max_draft_length %d (at most %d)", q.num_tokens, q.max_draft_length, TREE_MAX_DRAFT);
+    MQ_CHECK((int64_t) q.num_heads * q.max_draft_length <= (1 << 24), "num_heads %d x max_draft_length %d", q.num_heads, q.max_draft_length);
+    MQ_CHECK(q.tokens_per_block > 0 && (q.tokens_per_block & (q.tokens_per_block - 1)) == 0 && q.tokens_per_block <= (1 << 20),
+        "tokens_per_block must be a power of 2, got %d", q.tokens_per_block);
+    MQ_CHECK(q.max_blocks_per_seq > 0, "max_blocks_per_seq %d", q.max_blocks_per_seq);
+    MQ_CHECK(q.max_past_length >= 0 && q.max_past_length <= (1 << 30), "max_past_length %d", q.max_past_length);
+    MQ_CHECK(q.multi_block_mode >= 0, "multi_block_mode %d", q.multi_block_mode);
+}
+
+TreePlan tree_plan(const mi355q_tree_attention_params& q)
+{
+    TreePlan t{};
+    t.dp = q.head_size <= 64 ? 64 : (q.head_size <= 128 ? 128 : 256);
+    const int group = q.num_heads / q.num_kv_heads;
+    t.rows = std::max(q.max_draft_length, 1) * group;
+    // few rows: the 4 waves of a workgroup share the keys of a tile instead of the rows
+    t.rows_per_wg = t.rows <= 16 ? 16 : (t.rows <= 32 ? 32 : (t.rows <= 64 ? 64 : 128));
+    t.mtiles = (t.rows + t.rows_per_wg - 1) / t.rows_per_wg;
+    t.max_tiles = (q.max_past_length + q.max_draft_length + TREE_KT - 1) / TREE_KT;
+    t.max_tiles = std::max(t.max_tiles, 1);
+    // two workgroups live on a CU (one with heads beyond 128): split the keys until 256 CUs have that many, in
+    // stretches of at least 4 tiles (a stretch costs its prologue and a partial state)
+    const int64_t base = (int64_t) q.batch * q.num_kv_heads * t.mtiles;
+    const int64_t want = t.dp > 128 ? 256 : 512;
+    int splits = (int) std::min<int64_t>((want + base - 1) / std::max<int64_t>(base, 1), t.max_tiles / 4);
+    if (q.multi_block_mode > 0)
+        splits = q.multi_block_mode;
+    splits = std::max(1, std::min(std::min(splits, t.max_tiles), TREE_MAX_SPLITS));
+    t.chunk_tiles = (t.max_tiles + splits - 1) / splits;
+    t.splits = (t.max_tiles + t.chunk_tiles - 1) / t.chunk_tiles;
+    const size_t heads = (size_t) q.num_tokens * q.num_heads;
+    t.q_bytes = round256(heads * t.dp * 2);
+    t.seq_bytes = round256((size_t) q.batch * sizeof(int32_t));
+    if (t.splits > 1)
+    {
+        t.acc_bytes = round256(t.splits * heads * t.dp * sizeof(float));
+        t.ml_bytes = round256(t.splits * heads * sizeof(float2));
+    }
+    return t;
+}
+
+template <typename T, int KVT, int DP>
+void tree_launch_attn(const TreeArgs& a, const TreePlan& t, hipStream_t stream)
+{
+    const int64_t grid = ((int64_t) a.groups + 7) / 8 * 8 * t.mtiles;
+    MQ_CHECK(grid < (1ll << 31), "tree attention grid %lld", (long long) grid);
+    const dim3 g((unsigned) grid), b(TREE_THREADS);
+    switch (t.rows_per_wg)
+    {
+    case 16: hipLaunchKernelGGL((tree_attn_kernel<T, KVT, DP, 1, 4, 1>), g, b, 0, stream, a); break;
+    case 32: hipLaunchKernelGGL((tree_attn_kernel<T, KVT, DP, 1, 4, 2>), g, b, 0, stream, a); break;
+    case 64: hipLaunchKernelGGL((tree_attn_kernel<T, KVT, DP, 2, 2, 2>), g, b, 0, stream, a); break;
+    default: hipLaunchKernelGGL((tree_attn_kernel<T, KVT, DP, 4, 1, 2>), g, b, 0, stream, a); break;
+    }
+    MQ_HIP(hipGetLastError());
+}
+
+template <typename T, int KVT>
+void tree_launch(const mi355q_tree_attention_params& q, const TreeArgs& a, const TreePlan& t, hipStream_t stream)
+{
+    hipLaunchKernelGGL((tree_prepare_kernel<T, KVT>), dim3(q.max_draft_length + 1, q.batch), dim3(TREE_THREADS), 0, stream, a, t.dp);
+    MQ_HIP(hipGetLastError());
+    if (t.dp == 64)
+        tree_launch_attn<T, KVT, 64>(a, t, stream);
+    else if (t.dp == 128)
+        tree_launch_attn<T, KVT, 128>(a, t, stream);
+    else
+        tree_launch_attn<T, KVT, 256>(a, t, stream);
+    if (t.splits > 1)
+    {
+        const dim3 g(q.max_draft_length, q.batch), b(TREE_THREADS);
+        if (t.dp == 64)
+            hipLaunchKernelGGL((tree_combine_kernel<T, 64>), g, b, 0, stream, a, KVT != 0);
+        else if (t.dp == 128)
+            hipLaunchKernelGGL((tree_combine_kernel<T, 128>), g, b, 0, stream, a, KVT != 0);
+        else
+            hipLaunchKernelGGL((tree_combine_kernel<T, 256>), g, b, 0, stream, a, KVT != 0);
+        MQ_HIP(hipGetLastError());
+    }
+}
+
+template <typename T>
+void tree_launch_kv(const mi355q_tree_attention_params& q, const TreeArgs& a, const TreePlan& t, hipStream_t stream)
+{
+    if (q.kv_type == q.act_type)
+        tree_launch<T, 0>(q, a, t, stream);
+    else if (q.kv_type == MI355Q_INT8)
+        tree_launch<T, 1>(q, a, t, stream);
+    else
+        tree_launch<T, 2>(q, a, t, stream);
+}
+
+bool aligned16(const void* p)
+{
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+}
+} // namespace
+
+size_t tree_attention_workspace_size(const mi355q_tree_attention_params& q)
+{
+    tree_check(q);
+    return tree_plan(q).total();
+}
+
+void tree_attention(const mi355q_tree_attention_params& q, hipStream_t stream)
+{
+    tree_check(q);
+    if (q.batch == 0 || q.num_tokens == 0 || q.max_draft_length == 0)
+        return;
+    const size_t hidden = (size_t) (q.num_heads + 2 * q.num_kv_heads) * q.head_size;
+    MQ_CHECK(q.qkv && q.out && q.past_lengths && q.draft_offsets && q.tree_mask && q.block_pointers, "null tensor");
+    MQ_CHECK(q.qkv_stride == 0 || ((size_t) q.qkv_stride >= hidden && q.qkv_stride % 8 == 0), "qkv_stride %lld (rows of %zu)",
+        (long long) q.qkv_stride, hidden);
+    MQ_CHECK(aligned16(q.qkv) && aligned16(q.qkv_bias) && aligned16(q.out) && aligned16(q.workspace), "tensors must be 16-byte aligned");
+    MQ_CHECK(q.mask_words >= (q.max_draft_length + 31) / 32, "tree_mask rows of %d words do not hold %d nodes", q.mask_words,
+        q.max_draft_length);
+    MQ_CHECK((int64_t) q.max_past_length <= (int64_t) q.max_blocks_per_seq * q.tokens_per_block,
+        "past length %d exceeds the block table (%d x %d)", q.max_past_length, q.max_blocks_per_seq, q.tokens_per_block);
+    if (q.kv_type != q.act_type)
+        MQ_CHECK(q.kv_scale_orig_quant && q.kv_scale_quant_orig, "8-bit kv cache needs kv_scale_orig_quant and kv_scale_quant_orig");
+    if (q.position_embedding_type == 1 || q.position_embedding_type == 2)
+    {
+        MQ_CHECK(q.rotary_embedding_dim > 0 && q.rotary_embedding_dim <= q.head_size && q.rotary_embedding_dim % 2 == 0,
+            "rotary_embedding_dim %d", q.rotary_embedding_dim);
+        MQ_CHECK(q.rotary_embedding_base > 0.f, "rotary_embedding_base %g", q.rotary_embedding_base);
+        MQ_CHECK(q.rotary_embedding_scale_type >= 0 && q.rotary_embedding_scale_type <= 2, "rotary_embedding_scale_type %d",
+            q.rotary_embedding_scale_type);
+        if (q.rotary_embedding_scale_type != 0)
+            MQ_CHECK(q.rotary_embedding_scale > 0.f, "rotary_embedding_scale %g", q.rotary_embedding_scale);
+        if (q.rotary_embedding_scale_type == 2)
+            MQ_CHECK(q.rotary_embedding_max_positions > 0 && q.rotary_embedding_dim > 2 && q.rotary_embedding_scale >= 1.f,
+                "dynamic rotary scaling: max_positions %d, dim %d, scale %g", q.rotary_embedding_max_positions, q.rotary_embedding_dim,
+                q.rotary_embedding_scale);
+    }
+    else if (q.position_embedding_type != 0)
+        MQ_UNSUPPORTED("tree attention: position_embedding_type %d is not built (0 - 2)", q.position_embedding_type);
+    const TreePlan t = tree_plan(q);
+    MQ_CHECK(q.workspace && q.workspace_bytes >= t.total(), "workspace too small: %zu < %zu", q.workspace_bytes, t.total());
+    TreeArgs a{};
+    a.qkv = static_cast<const uint16_t*>(q.qkv);
+    a.qkv_bias = static_cast<const uint16_t*>(q.qkv_bias);
+    a.out = static_cast<uint16_t*>(q.out);
+    a.past_lengths = q.past_lengths;
+    a.draft_offsets = q.draft_offsets;
+    a.position_offsets = q.position_offsets;
+    a.tree_mask = q.tree_mask;
+    a.block_ptrs = q.block_pointers;
+    a.kv_scale_orig_quant = q.kv_scale_orig_quant;
+    a.kv_scale_quant_orig = q.kv_scale_quant_orig;
+    char* ws = static_cast<char*>(q.workspace);
+    a.q_ws = reinterpret_cast<uint16_t*>(ws);
+    a.seq_nodes = reinterpret_cast<int32_t*>(ws + t.q_bytes);
+    a.part_acc = reinterpret_cast<float*>(ws + t.q_bytes + t.seq_bytes);
+    a.part_ml = reinterpret_cast<float2*>(ws + t.q_bytes + t.seq_bytes + t.acc_bytes);
+    a.qkv_stride = q.qkv_stride ? q.qkv_stride : (int64_t) hidden;
+    a.batch = q.batch;
+    a.num_heads = q.num_heads;
+    a.num_kv_heads = q.num_kv_heads;
+    a.group = q.num_heads / q.num_kv_heads;
+    a.hs = q.head_size;
+    a.num_tokens = q.num_tokens;
+    a.max_draft = q.max_draft_length;
+    a.max_past = q.max_past_length;
+    a.mask_words = q.mask_words;
+    a.max_blocks = q.max_blocks_per_seq;
+    while ((1 << a.tpb_log2) < q.tokens_per_block)
+        ++a.tpb_log2;
+    a.mtiles = t.mtiles;
+    a.chunk_tiles = t.chunk_tiles;
+    a.splits = t.splits;
+    const int64_t groups = (int64_t) q.batch * q.num_kv_heads * t.splits;
+    MQ_CHECK(groups < (1 << 28), "tree attention: %lld (sequence, kv head, split) groups", (long long) groups);
+    a.groups = (int) groups;
+    a.pos_type = q.position_embedding_type;
+    a.rot_dim = q.rotary_embedding_dim;
+    a.rot_scale_type = q.rotary_embedding_scale_type;
+    a.rot_max_pos = q.rotary_embedding_max_positions;
+    a.rot_log2_base = q.rotary_embedding_base > 0.f ? log2((double) q.rotary_embedding_base) : 0.0;
+    a.rot_scale = q.rotary_embedding_scale;
+    a.score_scale = 1.f / (sqrtf((float) q.head_size) * (q.q_scaling == 0.f ? 1.f : q.q_scaling));
+    if (q.act_type == MI355Q_BF16)
+        tree_launch_kv<bf16_t>(q, a, t, stream);
+    else
+        tree_launch_kv<f16_t>(q, a, t, stream);
+}
+
+} // namespace mi355q

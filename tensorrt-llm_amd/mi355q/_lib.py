@@ -133,6 +133,52 @@ class ContextAttentionParams(C.Structure):
     ]
 
 
+class TreeAttentionParams(C.Structure):
+    _fields_ = [
+        ("qkv", C.c_void_p), ("qkv_bias", C.c_void_p), ("out", C.c_void_p),
+        ("past_lengths", C.c_void_p), ("draft_offsets", C.c_void_p), ("position_offsets", C.c_void_p),
+        ("tree_mask", C.c_void_p), ("block_pointers", C.c_void_p),
+        ("kv_scale_orig_quant", C.c_void_p), ("kv_scale_quant_orig", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("qkv_stride", C.c_int64),
+        ("batch", C.c_int32), ("num_heads", C.c_int32), ("num_kv_heads", C.c_int32), ("head_size", C.c_int32),
+        ("num_tokens", C.c_int32), ("max_draft_length", C.c_int32), ("max_past_length", C.c_int32), ("mask_words", C.c_int32),
+        ("max_blocks_per_seq", C.c_int32), ("tokens_per_block", C.c_int32), ("act_type", C.c_int32), ("kv_type", C.c_int32),
+        ("position_embedding_type", C.c_int32), ("rotary_embedding_dim", C.c_int32),
+        ("rotary_embedding_base", C.c_float), ("rotary_embedding_scale_type", C.c_int32),
+        ("rotary_embedding_scale", C.c_float), ("rotary_embedding_max_positions", C.c_int32),
+        ("q_scaling", C.c_float), ("multi_block_mode", C.c_int32),
+    ]
+
+
+class KvBlockTablesParams(C.Structure):
+    _fields_ = [
+        ("past_lengths", C.c_void_p), ("new_lengths", C.c_void_p), ("block_table", C.c_void_p),
+        ("block_counts", C.c_void_p), ("block_counts_out", C.c_void_p), ("free_blocks", C.c_void_p),
+        ("free_state", C.c_void_p), ("free_state_out", C.c_void_p), ("pool_bases", C.c_void_p),
+        ("block_pointers", C.c_void_p), ("token_offsets", C.c_void_p), ("slot_map", C.c_void_p), ("status", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("block_bytes", C.c_int64),
+        ("batch", C.c_int32), ("max_blocks_per_seq", C.c_int32), ("num_blocks", C.c_int32), ("num_pools", C.c_int32),
+        ("num_tokens", C.c_int32), ("tokens_per_block", C.c_int32),
+    ]
+
+
+class DraftTreeAcceptParams(C.Structure):
+    _fields_ = [
+        ("draft_tokens", C.c_void_p), ("parents", C.c_void_p), ("target_tokens", C.c_void_p), ("draft_offsets", C.c_void_p),
+        ("accept_path", C.c_void_p), ("accept_counts", C.c_void_p), ("accepted_tokens", C.c_void_p),
+        ("batch", C.c_int32), ("num_tokens", C.c_int32), ("max_path", C.c_int32),
+    ]
+
+
+class KvCommitPathParams(C.Structure):
+    _fields_ = [
+        ("block_pointers", C.c_void_p), ("past_lengths", C.c_void_p), ("accept_path", C.c_void_p),
+        ("accept_counts", C.c_void_p), ("new_lengths", C.c_void_p),
+        ("batch", C.c_int32), ("num_pools", C.c_int32), ("max_blocks_per_seq", C.c_int32), ("tokens_per_block", C.c_int32),
+        ("num_kv_heads", C.c_int32), ("head_size", C.c_int32), ("max_path", C.c_int32), ("kv_type", C.c_int32),
+    ]
+
+
 MAX_RANKS_PER_NODE, IPC_HANDLE_BYTES, COMM_UNIQUE_ID_BYTES = 8, 64, 128
 AR_RING, AR_ONESHOT, AR_TWOSHOT, AR_AUTO = range(4)
 
@@ -219,6 +265,12 @@ SYMBOLS = {
     "mi355q_masked_multihead_attention_static": (_i32, [C.POINTER(DecodeAttentionParams), _vp]),
     "mi355q_context_attention_workspace_size": (_sz, [C.POINTER(ContextAttentionParams)]),
     "mi355q_context_attention": (_i32, [C.POINTER(ContextAttentionParams), _vp]),
+    "mi355q_tree_attention_workspace_size": (_sz, [C.POINTER(TreeAttentionParams)]),
+    "mi355q_tree_attention": (_i32, [C.POINTER(TreeAttentionParams), _vp]),
+    "mi355q_kv_block_tables_workspace_size": (_sz, [_i32]),
+    "mi355q_kv_block_tables": (_i32, [C.POINTER(KvBlockTablesParams), _vp]),
+    "mi355q_draft_tree_accept": (_i32, [C.POINTER(DraftTreeAcceptParams), _vp]),
+    "mi355q_kv_commit_path": (_i32, [C.POINTER(KvCommitPathParams), _vp]),
     "mi355q_allreduce_select_implementation": (_i32, [_sz, _i32, _sz]),
     "mi355q_allreduce_max_workspace_size": (_sz, [_i32]),
     "mi355q_allreduce_params_deserialize": (_i32, [C.POINTER(AllReduceParams), _PP, _sz, _sz, C.c_uint32]),

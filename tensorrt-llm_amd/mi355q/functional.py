@@ -413,3 +413,200 @@ def gpt_attention(plugin, *, qkv, sequence_length, host_past_key_value_lengths, 
     if qkv_bias is not None:
         inputs += [qkv_bias]
     return plugin(*inputs, device=qkv.device)
+
+
+# ----------------------------------------------------------------------------- speculative decoding (device state only)
+def _check_tensor(name, t, device, dtype=None, shape=None):
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"{name} is {t.dtype}, expected {dtype}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} is not contiguous")
+    return t.data_ptr()
+
+
+class _On:
+    """The tensors' device made current for one call (a call may come while another device is), and its current stream."""
+
+    def __init__(self, t):
+        if not t.is_cuda:
+            raise ValueError(f"tensors must be on the GPU, got {t.device}")
+        self.index = t.device.index
+        self.previous = None
+
+    def __enter__(self):
+        if torch.cuda.current_device() != self.index:
+            self.previous = torch.cuda.current_device()
+            torch.cuda.set_device(self.index)
+        return C.c_void_p(torch.cuda.current_stream(self.index).cuda_stream)
+
+    def __exit__(self, *exc):
+        if self.previous is not None:
+            torch.cuda.set_device(self.previous)
+
+
+class TreeAttention:
+    """Attention of a tree of drafted tokens over the paged cache (mi355q_tree_attention in mi355q.h, which defines it): one
+    object per layer configuration, called once per step.
+
+    qkv [num_tokens, (Hq + 2 Hkv) Dh] holds the drafted tokens (nodes) of all sequences back to back, rows
+    draft_offsets[b] .. draft_offsets[b + 1] (int32 [batch + 1]) of sequence b; past_lengths int32 [batch]; tree_mask int32
+    [num_tokens, words], bit j of a row = node j of the same sequence is seen; block_pointers int64 [batch, 2, max_blocks]
+    (one layer of what KVCacheManager / kv_block_tables make); position_offsets int32 [num_tokens], a node's depth (default:
+    its index).  max_draft_length and max_past_length bound the device-side lengths.  K / V of the nodes are stored in slots
+    past .. past + n - 1 of the cache.  Rows of qkv may be strided (the last dimension contiguous)."""
+
+    def __init__(self, *, num_heads, num_kv_heads, head_size, dtype, kv_dtype=None, tokens_per_block=64, q_scaling=1.0,
+                 position_embedding_type=PositionEmbeddingType.learned_absolute, rotary_embedding_dim=0,
+                 rotary_embedding_base=10000.0, rotary_embedding_scale_type=RotaryScalingType.none, rotary_embedding_scale=1.0,
+                 rotary_embedding_max_positions=1024, multi_block_mode=0):
+        kv_dtype = dtype if kv_dtype is None else kv_dtype
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"dtype must be float16 or bfloat16, got {dtype}")
+        if kv_dtype not in (dtype, torch.int8, torch.float8_e4m3fn):
+            raise ValueError(f"kv_dtype must be {dtype}, int8 or float8_e4m3fn, got {kv_dtype}")
+        self.dtype, self.kv_dtype = dtype, kv_dtype
+        self.hidden, self.out_hidden = (num_heads + 2 * num_kv_heads) * head_size, num_heads * head_size
+        self._fields = dict(
+            num_heads=num_heads, num_kv_heads=num_kv_heads, head_size=head_size, tokens_per_block=tokens_per_block,
+            act_type=torch_dtype_to_trt(dtype), kv_type=torch_dtype_to_trt(kv_dtype), q_scaling=q_scaling,
+            position_embedding_type=position_embedding_type, rotary_embedding_dim=rotary_embedding_dim,
+            rotary_embedding_base=rotary_embedding_base, rotary_embedding_scale_type=rotary_embedding_scale_type,
+            rotary_embedding_scale=rotary_embedding_scale, rotary_embedding_max_positions=rotary_embedding_max_positions,
+            multi_block_mode=multi_block_mode)
+        self._template = bytes(L.TreeAttentionParams(**self._fields))
+
+    def _params(self, batch, num_tokens, max_draft_length, max_past_length, max_blocks, mask_words):
+        p = L.TreeAttentionParams.from_buffer_copy(self._template)
+        p.batch, p.num_tokens, p.max_draft_length, p.max_past_length = batch, num_tokens, max_draft_length, max_past_length
+        p.max_blocks_per_seq, p.mask_words = max_blocks, mask_words
+        return p
+
+    def workspace_size(self, batch, num_tokens, max_draft_length, max_past_length, max_blocks):
+        """Bytes of workspace a call with these bounds uses."""
+        p = self._params(batch, num_tokens, max_draft_length, max_past_length, max_blocks, (max_draft_length + 31) // 32)
+        n = L.lib().mi355q_tree_attention_workspace_size(C.byref(p))
+        if n == 0 and batch:
+            L.check(-1)
+        return n
+
+    def __call__(self, qkv, past_lengths, draft_offsets, tree_mask, block_pointers, *, max_draft_length, max_past_length,
+                 position_offsets=None, qkv_bias=None, kv_scale_orig_quant=None, kv_scale_quant_orig=None, out=None,
+                 workspace=None):
+        dev, i32 = qkv.device, torch.int32
+        if qkv.dim() != 2 or qkv.dtype != self.dtype or qkv.shape[1] != self.hidden or (qkv.numel() and qkv.stride(1) != 1):
+            raise ValueError(f"qkv must be {self.dtype} [num_tokens, {self.hidden}] with contiguous rows, got {qkv.dtype} "
+                             f"{tuple(qkv.shape)} strides {qkv.stride()}")
+        tokens, batch = qkv.shape[0], past_lengths.shape[0]
+        if tree_mask.dim() != 2 or block_pointers.dim() != 3:
+            raise ValueError("tree_mask must be [num_tokens, words], block_pointers [batch, 2, max_blocks]")
+        p = self._params(batch, tokens, max_draft_length, max_past_length, block_pointers.shape[2], tree_mask.shape[1])
+        p.past_lengths = _check_tensor("past_lengths", past_lengths, dev, i32, (batch,))
+        p.draft_offsets = _check_tensor("draft_offsets", draft_offsets, dev, i32, (batch + 1,))
+        if tree_mask.dtype not in (torch.int32, torch.uint32):
+            raise ValueError(f"tree_mask is {tree_mask.dtype}, expected int32")
+        p.tree_mask = _check_tensor("tree_mask", tree_mask, dev, None, (tokens, tree_mask.shape[1]))
+        p.block_pointers = _check_tensor("block_pointers", block_pointers, dev, torch.int64, (batch, 2, block_pointers.shape[2]))
+        if position_offsets is not None:
+            p.position_offsets = _check_tensor("position_offsets", position_offsets, dev, i32, (tokens,))
+        if qkv_bias is not None:
+            p.qkv_bias = _check_tensor("qkv_bias", qkv_bias, dev, self.dtype, (self.hidden,))
+        if kv_scale_orig_quant is not None:
+            p.kv_scale_orig_quant = _check_tensor("kv_scale_orig_quant", kv_scale_orig_quant, dev, torch.float32, (1,))
+            p.kv_scale_quant_orig = _check_tensor("kv_scale_quant_orig", kv_scale_quant_orig, dev, torch.float32, (1,))
+        p.qkv, p.qkv_stride = qkv.data_ptr(), qkv.stride(0) if tokens > 1 else 0
+        with _On(qkv) as stream:
+            if out is None:
+                out = torch.empty(tokens, self.out_hidden, dtype=self.dtype, device=dev)
+            p.out = _check_tensor("out", out, dev, self.dtype, (tokens, self.out_hidden))
+            need = L.lib().mi355q_tree_attention_workspace_size(C.byref(p))
+            if workspace is None:  # from torch's allocator: ordered on this stream, kept by a graph that captures the call
+                workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+            p.workspace, p.workspace_bytes = _check_tensor("workspace", workspace, dev), workspace.numel() * workspace.element_size()
+            L.check(L.lib().mi355q_tree_attention(C.byref(p), stream))
+        return out
+
+
+def kv_block_tables(past_lengths, new_lengths, block_table, block_counts, free_blocks, free_state, pool_bases, *, block_bytes,
+                    tokens_per_block, num_tokens, block_counts_out=None, free_state_out=None):
+    """Block tables, block pointers and slot maps on the device (mi355q_kv_block_tables in mi355q.h, which defines it).
+    past_lengths, new_lengths, block_counts int32 [batch]; block_table int32 [batch, max_blocks]; free_blocks int32
+    [num_blocks], the ring; free_state int32 [2]; pool_bases int64 [pools].  block_table and free_blocks are updated in
+    place, block_counts and free_state too unless *_out is given.  num_tokens: rows of the slot map (at least the sum of the
+    positive new_lengths for all of them to be there).  Returns (block_pointers int64 [pools, batch, 2, max_blocks],
+    token_offsets int32 [batch + 1], slot_map int64 [num_tokens], status int32 [batch])."""
+    dev, i32 = past_lengths.device, torch.int32
+    if block_table.dim() != 2 or free_blocks.dim() != 1 or pool_bases.dim() != 1:
+        raise ValueError("block_table must be [batch, max_blocks], free_blocks [num_blocks], pool_bases [pools]")
+    batch, max_blocks, pools = past_lengths.shape[0], block_table.shape[1], pool_bases.shape[0]
+    block_counts_out = block_counts if block_counts_out is None else block_counts_out
+    free_state_out = free_state if free_state_out is None else free_state_out
+    p = L.KvBlockTablesParams()
+    p.past_lengths = _check_tensor("past_lengths", past_lengths, dev, i32, (batch,))
+    p.new_lengths = _check_tensor("new_lengths", new_lengths, dev, i32, (batch,))
+    p.block_table = _check_tensor("block_table", block_table, dev, i32, (batch, max_blocks))
+    p.block_counts = _check_tensor("block_counts", block_counts, dev, i32, (batch,))
+    p.block_counts_out = _check_tensor("block_counts_out", block_counts_out, dev, i32, (batch,))
+    p.free_blocks = _check_tensor("free_blocks", free_blocks, dev, i32)
+    p.free_state = _check_tensor("free_state", free_state, dev, i32, (2,))
+    p.free_state_out = _check_tensor("free_state_out", free_state_out, dev, i32, (2,))
+    p.pool_bases = _check_tensor("pool_bases", pool_bases, dev, torch.int64)
+    p.block_bytes, p.batch, p.max_blocks_per_seq, p.num_blocks = block_bytes, batch, max_blocks, free_blocks.shape[0]
+    p.num_pools, p.num_tokens, p.tokens_per_block = pools, num_tokens, tokens_per_block
+    with _On(past_lengths) as stream:
+        pointers = torch.empty(pools, batch, 2, max_blocks, dtype=torch.int64, device=dev)
+        offsets = torch.empty(batch + 1, dtype=i32, device=dev)
+        slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
+        status = torch.empty(batch, dtype=i32, device=dev)
+        p.workspace_bytes = L.lib().mi355q_kv_block_tables_workspace_size(batch)
+        workspace = torch.empty(max(p.workspace_bytes, 16), dtype=torch.uint8, device=dev)
+        p.block_pointers, p.token_offsets, p.slot_map, p.status = (t.data_ptr() for t in (pointers, offsets, slots, status))
+        p.workspace = workspace.data_ptr()
+        L.check(L.lib().mi355q_kv_block_tables(C.byref(p), stream))
+    return pointers, offsets, slots, status
+
+
+def draft_tree_accept(draft_tokens, parents, target_tokens, draft_offsets, max_path):
+    """The path along which the model agrees with a tree of drafted tokens (mi355q_draft_tree_accept in mi355q.h): int32
+    tensors, draft_tokens / parents / target_tokens [num_tokens], draft_offsets [batch + 1].  Returns (accept_path [batch,
+    max_path], accept_counts [batch], accepted_tokens [batch, max_path]), -1 behind the counts."""
+    dev, i32 = draft_tokens.device, torch.int32
+    tokens, batch = draft_tokens.shape[0], draft_offsets.shape[0] - 1
+    p = L.DraftTreeAcceptParams()
+    p.draft_tokens = _check_tensor("draft_tokens", draft_tokens, dev, i32, (tokens,))
+    p.parents = _check_tensor("parents", parents, dev, i32, (tokens,))
+    p.target_tokens = _check_tensor("target_tokens", target_tokens, dev, i32, (tokens,))
+    p.draft_offsets = _check_tensor("draft_offsets", draft_offsets, dev, i32, (batch + 1,))
+    p.batch, p.num_tokens, p.max_path = batch, tokens, max_path
+    with _On(draft_tokens) as stream:
+        path = torch.empty(batch, max_path, dtype=i32, device=dev)
+        counts = torch.empty(batch, dtype=i32, device=dev)
+        emitted = torch.empty(batch, max_path, dtype=i32, device=dev)
+        p.accept_path, p.accept_counts, p.accepted_tokens = path.data_ptr(), counts.data_ptr(), emitted.data_ptr()
+        L.check(L.lib().mi355q_draft_tree_accept(C.byref(p), stream))
+    return path, counts, emitted
+
+
+def kv_commit_path(block_pointers, past_lengths, accept_path, accept_counts, *, num_kv_heads, head_size, tokens_per_block,
+                   kv_dtype):
+    """Moves the keys and values of the accepted path to the end of every sequence's history, in every pool, in place
+    (mi355q_kv_commit_path in mi355q.h).  block_pointers int64 [pools, batch, 2, max_blocks].  Returns the new lengths."""
+    dev, i32 = block_pointers.device, torch.int32
+    if block_pointers.dim() != 4 or accept_path.dim() != 2:
+        raise ValueError("block_pointers must be [pools, batch, 2, max_blocks], accept_path [batch, max_path]")
+    pools, batch, _, max_blocks = block_pointers.shape
+    p = L.KvCommitPathParams()
+    p.block_pointers = _check_tensor("block_pointers", block_pointers, dev, torch.int64, (pools, batch, 2, max_blocks))
+    p.past_lengths = _check_tensor("past_lengths", past_lengths, dev, i32, (batch,))
+    p.accept_path = _check_tensor("accept_path", accept_path, dev, i32, (batch, accept_path.shape[1]))
+    p.accept_counts = _check_tensor("accept_counts", accept_counts, dev, i32, (batch,))
+    p.batch, p.num_pools, p.max_blocks_per_seq, p.tokens_per_block = batch, pools, max_blocks, tokens_per_block
+    p.num_kv_heads, p.head_size, p.max_path, p.kv_type = num_kv_heads, head_size, accept_path.shape[1], torch_dtype_to_trt(kv_dtype)
+    with _On(block_pointers) as stream:
+        lengths = torch.empty(batch, dtype=i32, device=dev)
+        p.new_lengths = lengths.data_ptr()
+        L.check(L.lib().mi355q_kv_commit_path(C.byref(p), stream))
+    return lengths

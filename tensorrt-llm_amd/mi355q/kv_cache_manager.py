@@ -272,3 +272,37 @@ class KVCacheManager:
     def get_block_pointers(self, beam_width):
         """[pools, batch, beam_width, 2, max_blocks_per_seq] int64."""
         return torch.stack([self.blocks_manager.get_pointer_array(p, beam_width) for p in range(self.num_pools)], dim=0)
+
+
+class DeviceBlocksManager:
+    """The block bookkeeping kept on the GPU: a batch of `batch_size` request rows whose tables, free ring and pointers are
+    updated by one call per step from the requests' lengths (functional.kv_block_tables), so that a step whose lengths are
+    only known there (speculative decoding) needs no copy to the host.  Same pools, hand-out order and pointers as
+    BlocksManager; beam width 1, no attention window."""
+
+    def __init__(self, memory_pools, blocks, tokens_per_block, max_blocks_per_seq, batch_size):
+        dev = memory_pools[0].device
+        sizes = {p.nelement() * p.element_size() // (2 * blocks) for p in memory_pools}
+        if len(sizes) != 1 or any(p.device != dev for p in memory_pools):
+            raise ValueError("the pools must have one block size and lie on one device")
+        self.memory_pools, self.blocks, self.tokens_per_block = memory_pools, blocks, tokens_per_block
+        self.block_bytes = sizes.pop()
+        t = lambda v, dt=torch.int32: torch.tensor(v, dtype=dt, device=dev)
+        self.pool_bases = t([p.data_ptr() for p in memory_pools], torch.int64)
+        self.block_table = torch.full((batch_size, max_blocks_per_seq), -1, dtype=torch.int32, device=dev)
+        self.block_counts = torch.zeros(batch_size, dtype=torch.int32, device=dev)
+        self.free_ring = torch.arange(blocks, dtype=torch.int32, device=dev)
+        self.free_state = t([0, blocks])
+
+    def step(self, past_lengths, new_lengths, num_tokens):
+        """Blocks for new_lengths[b] more tokens of every row (negative: the request ends and gives its blocks back; 0 leaves
+        a row as it is).  Returns (block_pointers [pools, batch, 2, max_blocks], token_offsets, slot_map [num_tokens],
+        status)."""
+        from . import functional
+        return functional.kv_block_tables(
+            past_lengths, new_lengths, self.block_table, self.block_counts, self.free_ring, self.free_state, self.pool_bases,
+            block_bytes=self.block_bytes, tokens_per_block=self.tokens_per_block, num_tokens=num_tokens)
+
+    def free_blocks(self):
+        """Number of free blocks (copies two words to the host)."""
+        return int(self.free_state[1])
