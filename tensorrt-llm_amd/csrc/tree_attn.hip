@@ -24,6 +24,28 @@ constexpr int TREE_MAX_SPLITS = 64; // lane = split in the combine kernel
 constexpr int TREE_MAX_DRAFT = 1024;
 constexpr float LOG2E = 1.4426950408889634f;
 
+// The type the products run in: the activation type; fp16 for an 8-bit cache, whose codes it holds exactly (int8 and e4m3 have
+// at most 8 significant bits) and in which q and P keep 3 bits more than in bf16.
+template <typename T, int KVT>
+struct TreeCompute
+{
+    typedef T type;
+};
+template <>
+struct TreeCompute<bf16_t, 1>
+{
+    typedef f16_t type;
+};
+template <>
+struct TreeCompute<bf16_t, 2>
+{
+    typedef f16_t type;
+};
+// q in two parts (its rounding to the compute type and what that left over): the rotated query would otherwise be the
+// largest error beside the result's own rounding.  A bf16 result over fp16 products does not need it.
+template <typename T, int KVT>
+constexpr bool TREE_Q2 = KVT == 0 || !T16<T>::is_bf16;
+
 struct TreeArgs
 {
     const uint16_t* qkv;
@@ -36,7 +58,7 @@ struct TreeArgs
     const int64_t* block_ptrs;
     const float* kv_scale_orig_quant;
     const float* kv_scale_quant_orig;
-    uint16_t* q_ws;      // [tokens][Hq][DP] T: rotated, times the score scale (and the K dequantisation) and log2(e)
+    uint16_t* q_ws;      // [tokens][Hq][1 or 2 parts][DP]: rotated, times the score scale (and the K dequantisation) and log2(e)
     int32_t* seq_nodes;  // [batch]: nodes of the sequence, 0 if it is skipped
     float* part_acc;     // [splits][tokens * Hq][DP]
     float2* part_ml;     // [splits][tokens * Hq] (running maximum in the log2 domain, sum)
@@ -70,6 +92,8 @@ __device__ __forceinline__ bool tree_seq(const TreeArgs& p, int b, int& off, int
 template <typename T, int KVT>
 __global__ __launch_bounds__(TREE_THREADS) void tree_prepare_kernel(TreeArgs p, int dp)
 {
+    typedef typename TreeCompute<T, KVT>::type C;
+    constexpr int PARTS = TREE_Q2<T, KVT> ? 2 : 1;
     const int b = blockIdx.y, i = blockIdx.x;
     int off, n, past;
     const bool ok = tree_seq(p, b, off, n, past);
@@ -125,11 +149,12 @@ __global__ __launch_bounds__(TREE_THREADS) void tree_prepare_kernel(TreeArgs p, 
     for (int it = threadIdx.x; it < nvec * cpv; it += TREE_THREADS)
     {
         const int vec = it / cpv, d0 = 8 * (it % cpv);
-        uint4* const qdst = reinterpret_cast<uint4*>(p.q_ws + ((size_t) row * Hq + vec) * dp + d0);
+        uint4* const qdst = reinterpret_cast<uint4*>(p.q_ws + ((size_t) row * Hq + vec) * PARTS * dp + d0);
         if (d0 >= hs) // the padding of the workspace rows
         {
             if (vec < Hq)
-                *qdst = make_uint4(0, 0, 0, 0);
+                for (int part = 0; part < PARTS; ++part)
+                    qdst[part * dp / 8] = make_uint4(0, 0, 0, 0);
             continue;
         }
         auto element = [&](int d) -> double // q / k / v element d of this head, bias added
@@ -172,13 +197,20 @@ __global__ __launch_bounds__(TREE_THREADS) void tree_prepare_kernel(TreeArgs p, 
         }
         if (vec < Hq)
         {
-            // q carries the score scale, the K dequantisation and log2(e): the matrix product then IS the exponent.  One
-            // rounding to T, as many bits as q had
-            uint32_t o[4];
+            // q carries the score scale, the K dequantisation and log2(e): the matrix product then IS the exponent
+            float hi[8], lo[8];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                o[e] = pack2<T>((float) (y[2 * e] * qscale), (float) (y[2 * e + 1] * qscale));
-            *qdst = make_uint4(o[0], o[1], o[2], o[3]);
+            for (int e = 0; e < 8; ++e)
+            {
+                double z = y[e] * qscale;
+                if constexpr (!T16<C>::is_bf16) // a finite query stays finite in fp16
+                    z = fabs(z) > 65504.0 && fabs(z) < HUGE_VAL ? copysign(65504.0, z) : z;
+                hi[e] = T16<C>::to_float(T16<C>::from_float((float) z));
+                lo[e] = fabsf(hi[e]) < HUGE_VALF ? (float) (z - hi[e]) : 0.f;
+            }
+            *qdst = make_uint4(pack2<C>(hi[0], hi[1]), pack2<C>(hi[2], hi[3]), pack2<C>(hi[4], hi[5]), pack2<C>(hi[6], hi[7]));
+            if constexpr (PARTS == 2)
+                qdst[dp / 8] = make_uint4(pack2<C>(lo[0], lo[1]), pack2<C>(lo[2], lo[3]), pack2<C>(lo[4], lo[5]), pack2<C>(lo[6], lo[7]));
             continue;
         }
         const int kv = (vec - Hq) / Hkv, hk = (vec - Hq) % Hkv;
@@ -225,16 +257,40 @@ __device__ __forceinline__ cf32x4_t tree_mfma16<f16_t>(const uint2& a, const uin
     return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4_t, a), __builtin_bit_cast(f16x4_t, b), c, 0, 0, 0);
 }
 
-// 8 cache bytes -> 8 values of T (exact: int8 and e4m3 have at most 8 significant bits)
-template <typename T, int KVT>
-__device__ __forceinline__ uint4 tree_kv8_to_t(uint32_t w0, uint32_t w1)
+// 8 cache bytes -> 8 fp16 values (exact)
+template <int KVT>
+__device__ __forceinline__ uint4 tree_kv8_to_f16(uint32_t w0, uint32_t w1)
 {
-    const uint32_t w[2] = {w0, w1};
-    uint32_t o[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        o[i] = pack2<T>(kv8_to_float<KVT>(w[i >> 1], 2 * (i & 1)), kv8_to_float<KVT>(w[i >> 1], 2 * (i & 1) + 1));
-    return make_uint4(o[0], o[1], o[2], o[3]);
+    uint4 r;
+    if constexpr (KVT == 2)
+    {
+        r.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, 1.f, false));
+        r.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, 1.f, true));
+        r.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, 1.f, false));
+        r.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, 1.f, true));
+    }
+    else
+    {
+        r.x = pack2<f16_t>(kv8_to_float<1>(w0, 0), kv8_to_float<1>(w0, 1));
+        r.y = pack2<f16_t>(kv8_to_float<1>(w0, 2), kv8_to_float<1>(w0, 3));
+        r.z = pack2<f16_t>(kv8_to_float<1>(w1, 0), kv8_to_float<1>(w1, 1));
+        r.w = pack2<f16_t>(kv8_to_float<1>(w1, 2), kv8_to_float<1>(w1, 3));
+    }
+    return r;
+}
+
+// 16 bytes from an address that was an integer in a table: a global load (a plain cast would make it a flat one)
+__device__ __forceinline__ uint4 tree_load16(int64_t address)
+{
+    typedef __attribute__((ext_vector_type(4))) uint32_t u32x4_t;
+    const u32x4_t v = *(const __attribute__((address_space(1))) u32x4_t*) address;
+    return make_uint4(v.x, v.y, v.z, v.w);
+}
+
+// the LDS-DMA of ctx_dma16 with a wave-uniform base and a 32-bit lane offset
+__device__ __forceinline__ void tree_dma16(int64_t base, uint32_t offset, uint32_t lds_off)
+{
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(lds_off) : "memory", "m0");
 }
 
 // does a dword of two T values hold an infinity or NaN
@@ -280,13 +336,16 @@ template <typename T, int KVT, int DP, int RW, int KW, int QT>
 __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP > 128 ? 1 : 2))) void tree_attn_kernel(TreeArgs p)
 {
     static_assert(RW * KW == 4, "4 waves");
+    typedef typename TreeCompute<T, KVT>::type C;
+    constexpr int PARTS = TREE_Q2<T, KVT> ? 2 : 1;
     constexpr int M = RW * QT * 16;
     constexpr int KS = DP / 32, DT = DP / 16;
     constexpr int ROWB = DP * 2, CH = ROWB / 16;
     constexpr int TILE_BYTES = TREE_KT * ROWB, STAGE_BYTES = 2 * TILE_BYTES;
     constexpr int XW = 4 / KW;                      // 16-key subtiles per wave
-    constexpr int RPD = 1024 / ROWB, DPW = TREE_KT / RPD / 4; // 16-bit caches: rows per DMA instruction, DMAs per wave
-    constexpr int CH8 = DP / 16, LPT = TREE_KT * CH8 / TREE_THREADS; // 8-bit caches: 16-byte loads per thread and tile
+    constexpr int WROWS = TREE_KT / 4;              // a wave loads 16 consecutive keys of a tile
+    constexpr int RPD = 1024 / ROWB, DPW = WROWS / RPD; // 16-bit caches: rows per DMA instruction, DMAs per wave
+    constexpr int CH8 = DP / 16, RPL = 64 / CH8, LPT = WROWS / RPL; // 8-bit caches: rows per 16-byte load, loads per thread
     __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE_BYTES];
     __shared__ uint32_t nonfinite[2]; // keys of the tile whose V row has an infinity or NaN
 
@@ -309,46 +368,79 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
         return;
     const bool alone = ntiles <= p.chunk_tiles; // the sequence was not split
     const int hs = p.hs, tpb_mask = (1 << p.tpb_log2) - 1;
+    const int row_bytes = hs * (KVT ? 1 : 2); // of a head in the cache
     const int64_t* const kp = p.block_ptrs + (size_t) b * 2 * p.max_blocks;
     const int64_t* const vp = kp + p.max_blocks;
 
-    auto ksw = [](int row) { return CH >= 16 ? (row & 15) : ((row >> 1) & 7); };
-    auto vsw = [](int row) { return (((row & 3) << 2) | ((row >> 2) & 3)) & (CH - 1); };
+    // swizzle of the 16-byte chunk index by the row, K and V alike: 16 consecutive rows x one chunk (a K fragment) and 4 rows
+    // x two chunks (a transposing V read) fall on different banks
+    auto sw = [](int row) { return CH >= 16 ? ((row & 3) << 2 | ((row >> 2) & 3)) : (((row >> 1) & 3) << 1 | ((row >> 3) & 1)); };
 
-    // ---- tile loads.  16-bit caches: LDS-DMA, instruction d of a tile fills LDS bytes [1024 d, +1024), the swizzle applied
-    // on the source address.  8-bit caches: through registers, converted to T on the way into the LDS.
+    // ---- tile loads.  A wave loads 16 consecutive keys, which lie in one block (of at least 16 tokens): the block's address is
+    // a scalar load, issued a tile ahead, and a lane adds a fixed 32-bit offset.  16-bit caches: LDS-DMA, instruction d of a
+    // tile fills LDS bytes [1024 d, +1024), the swizzle applied on the source address.  8-bit caches: through registers,
+    // converted on the way into the LDS.  Keys past the sequence are whatever its last block holds there.
     const uint32_t lds_base = __builtin_amdgcn_readfirstlane((uint32_t) (uintptr_t) (ctx_lds_void_t*) lds);
-    const int last_chunk = hs * (KVT ? 1 : 2) / 16 - 1; // heads narrower than DP: the padding re-reads the last chunk (q is 0 there)
+    const int last_chunk = row_bytes / 16 - 1; // heads narrower than DP: the padding re-reads the last chunk (q is 0 there)
+    constexpr int LOADS = KVT ? LPT : DPW;
+    uint32_t lane_off[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i)
+    {
+        const int r = i * (KVT ? RPL : RPD) + lane / (KVT ? CH8 : CH), row = wave * WROWS + r; // row of the wave's 16, of the tile
+        const int ch = lane % (KVT ? CH8 : CH);
+        lane_off[i] = r * row_bytes + 16 * min(KVT ? ch : ch ^ sw(row), last_chunk);
+    }
+    const bool one_block = p.tpb_log2 >= 4;
+    typedef const __attribute__((address_space(4))) int64_t* scalar_ptr;
+    int64_t kbase = 0, vbase = 0; // where the wave's 16 keys of the tile to be loaded next begin
+    auto find_tile = [&](int tile)
+    {
+        if (one_block)
+        {
+            const int t0 = tile * TREE_KT + wave * WROWS;
+            const int blk = __builtin_amdgcn_readfirstlane(min(t0, total - 1) >> p.tpb_log2);
+            const int64_t in_block = (((int64_t) hk << p.tpb_log2) + (t0 & tpb_mask)) * row_bytes;
+            kbase = ((scalar_ptr) kp)[blk] + in_block;
+            vbase = ((scalar_ptr) vp)[blk] + in_block;
+        }
+    };
     uint4 kreg[KVT ? LPT : 1], vreg[KVT ? LPT : 1];
     auto load_tile = [&](int tile, int buf)
     {
-        const int t0 = tile * TREE_KT;
-        if constexpr (KVT == 0)
-        {
-            const int drow = lane / CH, dch = lane % CH;
 #pragma unroll
-            for (int i = 0; i < DPW; ++i)
+        for (int i = 0; i < LOADS; ++i)
+        {
+            const uint32_t dst = lds_base + buf * STAGE_BYTES + (wave * DPW + i) * 1024;
+            if (one_block)
             {
-                const int d = wave * DPW + i, row = d * RPD + drow;
-                const int t = min(t0 + row, total - 1); // rows past the sequence re-read its last one
-                const size_t at = ((size_t) hk << p.tpb_log2) + (t & tpb_mask);
-                const char* kb = reinterpret_cast<const char*>(kp[t >> p.tpb_log2]) + at * hs * 2;
-                const char* vb = reinterpret_cast<const char*>(vp[t >> p.tpb_log2]) + at * hs * 2;
-                const uint32_t dst = lds_base + buf * STAGE_BYTES + d * 1024;
-                ctx_dma16(kb + 16 * min(dch ^ ksw(row), last_chunk), dst);
-                ctx_dma16(vb + 16 * min(dch ^ vsw(row), last_chunk), dst + TILE_BYTES);
+                if constexpr (KVT == 0)
+                {
+                    tree_dma16(kbase, lane_off[i], dst);
+                    tree_dma16(vbase, lane_off[i], dst + TILE_BYTES);
+                }
+                else
+                {
+                    kreg[i] = tree_load16(kbase + lane_off[i]);
+                    vreg[i] = tree_load16(vbase + lane_off[i]);
+                }
             }
-        }
-        else
-        {
-#pragma unroll
-            for (int i = 0; i < LPT; ++i)
+            else // blocks of 1 - 8 tokens: every lane looks its key's block up
             {
-                const int c = tid + i * TREE_THREADS, row = c / CH8, ch = min(c % CH8, last_chunk);
-                const int t = min(t0 + row, total - 1);
-                const size_t at = ((size_t) hk << p.tpb_log2) + (t & tpb_mask);
-                kreg[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(kp[t >> p.tpb_log2]) + at * hs + 16 * ch);
-                vreg[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(vp[t >> p.tpb_log2]) + at * hs + 16 * ch);
+                const int r = i * (KVT ? RPL : RPD) + lane / (KVT ? CH8 : CH);
+                const int t = min(tile * TREE_KT + wave * WROWS + r, total - 1);
+                const int64_t in_block = (((int64_t) hk << p.tpb_log2) + (t & tpb_mask) - r) * row_bytes;
+                const int64_t ka = kp[t >> p.tpb_log2] + in_block + lane_off[i], va = vp[t >> p.tpb_log2] + in_block + lane_off[i];
+                if constexpr (KVT == 0)
+                {
+                    ctx_dma16(reinterpret_cast<const void*>(ka), dst);
+                    ctx_dma16(reinterpret_cast<const void*>(va), dst + TILE_BYTES);
+                }
+                else
+                {
+                    kreg[i] = tree_load16(ka);
+                    vreg[i] = tree_load16(va);
+                }
             }
         }
     };
@@ -359,46 +451,53 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
 #pragma unroll
             for (int i = 0; i < LPT; ++i)
             {
-                const int c = tid + i * TREE_THREADS, row = c / CH8, ch = 2 * (c % CH8);
+                const int row = wave * WROWS + i * RPL + lane / CH8, ch = 2 * (lane % CH8);
                 uint8_t* kt = lds + buf * STAGE_BYTES + ROWB * row;
                 uint8_t* vt = kt + TILE_BYTES;
-                *reinterpret_cast<uint4*>(kt + 16 * (ch ^ ksw(row))) = tree_kv8_to_t<T, KVT>(kreg[i].x, kreg[i].y);
-                *reinterpret_cast<uint4*>(kt + 16 * ((ch + 1) ^ ksw(row))) = tree_kv8_to_t<T, KVT>(kreg[i].z, kreg[i].w);
-                *reinterpret_cast<uint4*>(vt + 16 * (ch ^ vsw(row))) = tree_kv8_to_t<T, KVT>(vreg[i].x, vreg[i].y);
-                *reinterpret_cast<uint4*>(vt + 16 * ((ch + 1) ^ vsw(row))) = tree_kv8_to_t<T, KVT>(vreg[i].z, vreg[i].w);
+                *reinterpret_cast<uint4*>(kt + 16 * (ch ^ sw(row))) = tree_kv8_to_f16<KVT>(kreg[i].x, kreg[i].y);
+                *reinterpret_cast<uint4*>(kt + 16 * ((ch + 1) ^ sw(row))) = tree_kv8_to_f16<KVT>(kreg[i].z, kreg[i].w);
+                *reinterpret_cast<uint4*>(vt + 16 * (ch ^ sw(row))) = tree_kv8_to_f16<KVT>(vreg[i].x, vreg[i].y);
+                *reinterpret_cast<uint4*>(vt + 16 * ((ch + 1) ^ sw(row))) = tree_kv8_to_f16<KVT>(vreg[i].z, vreg[i].w);
             }
         }
     };
 
+    find_tile(tile_lo);
     load_tile(tile_lo, tile_lo & 1);
+    find_tile(min(tile_lo + 1, tile_hi - 1));
     // ---- Q^T fragments (B operand): column = row q0 + 16 qt + lr, k = d = 32 ks + 8 lq + j
     const int q0 = mt * M + rw * QT * 16;
-    uint4 qf[QT][KS];
+    uint4 qf[PARTS][QT][KS];
     int node[QT];
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt)
     {
         const int r = min(q0 + 16 * qt + lr, n * G - 1); // rows past the last re-read it; never stored
         node[qt] = r / G;
-        const uint16_t* q = p.q_ws + ((size_t) (off + node[qt]) * p.num_heads + hk * G + r % G) * DP;
+        const uint16_t* q = p.q_ws + ((size_t) (off + node[qt]) * p.num_heads + hk * G + r % G) * PARTS * DP;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-            qf[qt][ks] = *reinterpret_cast<const uint4*>(q + 32 * ks + 8 * lq);
+        for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+                qf[part][qt][ks] = *reinterpret_cast<const uint4*>(q + part * DP + 32 * ks + 8 * lq);
     }
     // end the compiler's own bookkeeping of the q loads here, before the loop's (to it invisible) DMAs
 #pragma unroll
-    for (int qt = 0; qt < QT; ++qt)
+    for (int part = 0; part < PARTS; ++part)
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-            asm volatile("" : "+v"(qf[qt][ks].x), "+v"(qf[qt][ks].y), "+v"(qf[qt][ks].z), "+v"(qf[qt][ks].w));
+        for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+                asm volatile("" : "+v"(qf[part][qt][ks].x), "+v"(qf[part][qt][ks].y), "+v"(qf[part][qt][ks].z), "+v"(qf[part][qt][ks].w));
 
-    float m_run[QT], l_run[QT];
-    cf32x4_t minus_m[QT]; // C operand of the scores: -m, 0 while the column has no maximum yet
+    float l_run[QT];
+    cf32x4_t minus_m[QT]; // C operand of the scores: minus the running maximum
+    bool fresh[QT];       // the column has no maximum yet (minus_m is 0)
     cf32x4_t o[QT][DT];
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt)
     {
-        m_run[qt] = NEG_BIG;
+        fresh[qt] = true;
         l_run[qt] = 0.f;
         minus_m[qt] = cf32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -408,26 +507,30 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
     const int rq = lr >> 2, rp = lr & 3;
     const int kb0 = kw * 16 * XW; // this wave's first key of a tile
 
-    auto compute = [&](int buf, int t0, bool tail)
+    // 32 keys (16 with four key groups) from key kb of the tile on
+    constexpr int X2 = XW < 2 ? XW : 2;
+    auto compute = [&](int buf, int t0, int kb, bool tail)
     {
         const uint8_t* kt = lds + buf * STAGE_BYTES;
         const uint8_t* vt = kt + TILE_BYTES;
-        cf32x4_t s[XW][QT];
+        cf32x4_t s[X2][QT];
 #pragma unroll
-        for (int x = 0; x < XW; ++x)
+        for (int x = 0; x < X2; ++x)
         {
-            const int row = kb0 + 16 * x + lr;
+            const int row = kb + 16 * x + lr;
             uint4 kf[KS];
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
-                kf[ks] = *reinterpret_cast<const uint4*>(kt + ROWB * row + 16 * ((4 * ks + lq) ^ ksw(row)));
+                kf[ks] = *reinterpret_cast<const uint4*>(kt + ROWB * row + 16 * ((4 * ks + lq) ^ sw(row)));
 #pragma unroll
             for (int qt = 0; qt < QT; ++qt)
             {
                 s[x][qt] = minus_m[qt];
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks)
-                    s[x][qt] = ctx_mfma<T>(kf[ks], qf[qt][ks], s[x][qt]);
+                for (int part = PARTS - 1; part >= 0; --part)
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks)
+                        s[x][qt] = ctx_mfma<C>(kf[ks], qf[part][qt][ks], s[x][qt]);
             }
         }
         if (tail)
@@ -436,58 +539,57 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
             for (int qt = 0; qt < QT; ++qt)
             {
                 const uint64_t seen
-                    = tree_mask64(p.tree_mask + (size_t) (off + node[qt]) * p.mask_words, p.mask_words, n, t0 - past) >> (kb0 + 4 * lq);
+                    = tree_mask64(p.tree_mask + (size_t) (off + node[qt]) * p.mask_words, p.mask_words, n, t0 - past) >> (kb + 4 * lq);
 #pragma unroll
-                for (int x = 0; x < XW; ++x)
+                for (int x = 0; x < X2; ++x)
 #pragma unroll
                     for (int rr = 0; rr < 4; ++rr)
                         s[x][qt][rr] = (seen >> (16 * x + rr)) & 1 ? s[x][qt][rr] : -__builtin_inff();
             }
         }
-        uint32_t pk[QT][XW][2];
+        uint32_t pk[QT][X2][2];
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt)
         {
             int mx = 0; // the largest positive s - m, as raw bits
 #pragma unroll
-            for (int x = 0; x < XW; ++x)
+            for (int x = 0; x < X2; ++x)
 #pragma unroll
                 for (int rr = 0; rr < 4; ++rr)
                     mx = max(mx, __builtin_bit_cast(int, (float) s[x][qt][rr]));
-            const bool fresh = m_run[qt] == NEG_BIG;
-            if (__any(fresh || mx > 0x41000000 /* 8.0f */)) // wave-uniform
+            if (__any(fresh[qt] || mx > 0x41000000 /* 8.0f */)) // wave-uniform
             {
-                // the column's maximum of this tile, over its 4 lanes (a NaN stays out of the comparison and in the scores)
+                // the column's maximum of these keys, over its 4 lanes (a NaN stays out of the comparison and in the scores)
                 float top = -__builtin_inff();
 #pragma unroll
-                for (int x = 0; x < XW; ++x)
+                for (int x = 0; x < X2; ++x)
 #pragma unroll
                     for (int rr = 0; rr < 4; ++rr)
                         top = fmaxf(top, s[x][qt][rr]);
                 top = fmaxf(top, __shfl_xor(top, 16));
                 top = fmaxf(top, __shfl_xor(top, 32));
-                const float up = top == -__builtin_inff() ? 0.f : (fresh ? top : fmaxf(top, 0.f));
-                const float corr = fresh ? 0.f : __builtin_amdgcn_exp2f(-up); // (nothing was summed before the first maximum)
                 if (top != -__builtin_inff())
                 {
-                    m_run[qt] = fresh ? up : m_run[qt] + up;
-                    minus_m[qt] = cf32x4_t{-m_run[qt], -m_run[qt], -m_run[qt], -m_run[qt]};
+                    const float up = fresh[qt] ? top : fmaxf(top, 0.f);
+                    const float corr = fresh[qt] ? 0.f : __builtin_amdgcn_exp2f(-up); // (nothing was summed before the first maximum)
+                    const float mm = minus_m[qt][0] - up;
+                    minus_m[qt] = cf32x4_t{mm, mm, mm, mm};
+                    fresh[qt] = false;
                     l_run[qt] *= corr;
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                        for (int rr = 0; rr < 4; ++rr)
+                            o[qt][dt][rr] *= corr;
+#pragma unroll
+                    for (int x = 0; x < X2; ++x)
+#pragma unroll
+                        for (int rr = 0; rr < 4; ++rr)
+                            s[x][qt][rr] -= up;
                 }
-                const float oc = top != -__builtin_inff() ? corr : 1.f;
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                    for (int rr = 0; rr < 4; ++rr)
-                        o[qt][dt][rr] *= oc;
-#pragma unroll
-                for (int x = 0; x < XW; ++x)
-#pragma unroll
-                    for (int rr = 0; rr < 4; ++rr)
-                        s[x][qt][rr] -= up;
             }
 #pragma unroll
-            for (int x = 0; x < XW; ++x)
+            for (int x = 0; x < X2; ++x)
             {
                 float e[4];
 #pragma unroll
@@ -496,47 +598,35 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
                     e[rr] = __builtin_amdgcn_exp2f(s[x][qt][rr]);
                     l_run[qt] += e[rr];
                 }
-                // P in T: its relative rounding error (half a step of T) averages out over the keys
-                pk[qt][x][0] = pack2<T>(e[0], e[1]);
-                pk[qt][x][1] = pack2<T>(e[2], e[3]);
+                // P in the compute type: its rounding (half a step, relative) averages out over the keys
+                pk[qt][x][0] = pack2<C>(e[0], e[1]);
+                pk[qt][x][1] = pack2<C>(e[2], e[3]);
             }
         }
         // ---- O^T += V^T . P^T  (A operand rows d = 16 dt + lr by the transposing LDS read)
-        if constexpr (XW >= 2)
+        const int ra = kb + 4 * lq + rq, rb = ra + 16;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
         {
-#pragma unroll
-            for (int kh = 0; kh < XW / 2; ++kh)
+            const int ch = 2 * dt + (rp >> 1), sub = 8 * (rp & 1);
+            const cs16x4_t va
+                = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_cs16x4_t*) (vt + ROWB * ra + 16 * (ch ^ sw(ra)) + sub));
+            const uint2 a2 = __builtin_bit_cast(uint2, va);
+            if constexpr (X2 == 2)
             {
-                const int ra = kb0 + 32 * kh + 4 * lq + rq, rb = ra + 16;
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
-                {
-                    const int ch = 2 * dt + (rp >> 1), sub = 8 * (rp & 1);
-                    const cs16x4_t va
-                        = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_cs16x4_t*) (vt + ROWB * ra + 16 * (ch ^ vsw(ra)) + sub));
-                    const cs16x4_t vb
-                        = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_cs16x4_t*) (vt + ROWB * rb + 16 * (ch ^ vsw(rb)) + sub));
-                    const uint2 a2 = __builtin_bit_cast(uint2, va), b2 = __builtin_bit_cast(uint2, vb);
-                    const uint4 vf = make_uint4(a2.x, a2.y, b2.x, b2.y);
-#pragma unroll
-                    for (int qt = 0; qt < QT; ++qt)
-                        o[qt][dt] = ctx_mfma<T>(vf,
-                            make_uint4(pk[qt][2 * kh][0], pk[qt][2 * kh][1], pk[qt][2 * kh + 1][0], pk[qt][2 * kh + 1][1]), o[qt][dt]);
-                }
-            }
-        }
-        else
-        {
-            const int ra = kb0 + 4 * lq + rq;
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
-            {
-                const int ch = 2 * dt + (rp >> 1), sub = 8 * (rp & 1);
-                const cs16x4_t va
-                    = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_cs16x4_t*) (vt + ROWB * ra + 16 * (ch ^ vsw(ra)) + sub));
+                const cs16x4_t vb
+                    = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_cs16x4_t*) (vt + ROWB * rb + 16 * (ch ^ sw(rb)) + sub));
+                const uint2 b2 = __builtin_bit_cast(uint2, vb);
 #pragma unroll
                 for (int qt = 0; qt < QT; ++qt)
-                    o[qt][dt] = tree_mfma16<T>(__builtin_bit_cast(uint2, va), make_uint2(pk[qt][0][0], pk[qt][0][1]), o[qt][dt]);
+                    o[qt][dt] = ctx_mfma<C>(make_uint4(a2.x, a2.y, b2.x, b2.y),
+                        make_uint4(pk[qt][0][0], pk[qt][0][1], pk[qt][X2 - 1][0], pk[qt][X2 - 1][1]), o[qt][dt]);
+            }
+            else
+            {
+#pragma unroll
+                for (int qt = 0; qt < QT; ++qt)
+                    o[qt][dt] = tree_mfma16<C>(a2, make_uint2(pk[qt][0][0], pk[qt][0][1]), o[qt][dt]);
             }
         }
         if constexpr (KVT == 0)
@@ -547,7 +637,7 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
             for (uint64_t left = bad; left; left &= left - 1)
             {
                 const int k = __builtin_ctzll(left), t = t0 + k;
-                if (k < kb0 || k >= kb0 + 16 * XW)
+                if (k < kb || k >= kb + 16 * X2)
                     continue;
                 const size_t at = ((size_t) hk << p.tpb_log2) + (t & tpb_mask);
                 const uint16_t* v = reinterpret_cast<const uint16_t*>(vp[t >> p.tpb_log2]) + at * hs;
@@ -617,12 +707,17 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // my share of tile i has landed
         __syncthreads();                                     // everyone's has, and everyone is done with tile i - 1
         if (i + 1 < tile_hi)
+        {
             load_tile(i + 1, (i + 1) & 1);
+            find_tile(min(i + 2, tile_hi - 1));
+        }
         const int t0 = i * TREE_KT;
         const bool tail = t0 + TREE_KT > past; // uniform
         if (tail)
             clean_tail(i & 1, t0);
-        compute(i & 1, t0, tail);
+#pragma unroll 1
+        for (int x = 0; x < XW; x += X2)
+            compute(i & 1, t0, kb0 + 16 * x, tail);
         if constexpr (KVT != 0)
         {
             if (i + 1 < tile_hi)
@@ -630,6 +725,10 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
         }
     }
 
+    float m_run[QT];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt)
+        m_run[qt] = fresh[qt] ? NEG_BIG : -minus_m[qt][0];
     // ---- the sum over the 4 lanes of a column, then the key groups of a row group through the LDS
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt)
@@ -800,7 +899,7 @@ TreePlan tree_plan(const mi355q_tree_attention_params& q)
     const int group = q.num_heads / q.num_kv_heads;
     t.rows = std::max(q.max_draft_length, 1) * group;
     // few rows: the 4 waves of a workgroup share the keys of a tile instead of the rows
-    t.rows_per_wg = t.rows <= 16 ? 16 : (t.rows <= 32 ? 32 : (t.rows <= 64 ? 64 : 128));
+    t.rows_per_wg = t.rows <= 16 ? 16 : (t.rows <= 32 ? 32 : (t.rows <= 64 || t.dp > 128 ? 64 : 128));
     t.mtiles = (t.rows + t.rows_per_wg - 1) / t.rows_per_wg;
     t.max_tiles = (q.max_past_length + q.max_draft_length + TREE_KT - 1) / TREE_KT;
     t.max_tiles = std::max(t.max_tiles, 1);
@@ -815,7 +914,8 @@ TreePlan tree_plan(const mi355q_tree_attention_params& q)
     t.chunk_tiles = (t.max_tiles + splits - 1) / splits;
     t.splits = (t.max_tiles + t.chunk_tiles - 1) / t.chunk_tiles;
     const size_t heads = (size_t) q.num_tokens * q.num_heads;
-    t.q_bytes = round256(heads * t.dp * 2);
+    const bool two_parts = q.kv_type == q.act_type || q.act_type == MI355Q_HALF; // TREE_Q2
+    t.q_bytes = round256(heads * t.dp * 2 * (two_parts ? 2 : 1));
     t.seq_bytes = round256((size_t) q.batch * sizeof(int32_t));
     if (t.splits > 1)
     {
@@ -831,13 +931,16 @@ void tree_launch_attn(const TreeArgs& a, const TreePlan& t, hipStream_t stream)
     const int64_t grid = ((int64_t) a.groups + 7) / 8 * 8 * t.mtiles;
     MQ_CHECK(grid < (1ll << 31), "tree attention grid %lld", (long long) grid);
     const dim3 g((unsigned) grid), b(TREE_THREADS);
-    switch (t.rows_per_wg)
-    {
-    case 16: hipLaunchKernelGGL((tree_attn_kernel<T, KVT, DP, 1, 4, 1>), g, b, 0, stream, a); break;
-    case 32: hipLaunchKernelGGL((tree_attn_kernel<T, KVT, DP, 1, 4, 2>), g, b, 0, stream, a); break;
-    case 64: hipLaunchKernelGGL((tree_attn_kernel<T, KVT, DP, 2, 2, 2>), g, b, 0, stream, a); break;
-    default: hipLaunchKernelGGL((tree_attn_kernel<T, KVT, DP, 4, 1, 2>), g, b, 0, stream, a); break;
-    }
+    // 32 rows a wave; 16 with heads beyond 128, whose accumulators take twice the registers
+    constexpr int QT = DP > 128 ? 1 : 2;
+    if (t.rows_per_wg == 16)
+        hipLaunchKernelGGL((tree_attn_kernel<T, KVT, DP, 1, 4, 1>), g, b, 0, stream, a);
+    else if (t.rows_per_wg == 16 * QT)
+        hipLaunchKernelGGL((tree_attn_kernel<T, KVT, DP, 1, 4, QT>), g, b, 0, stream, a);
+    else if (t.rows_per_wg == 32 * QT)
+        hipLaunchKernelGGL((tree_attn_kernel<T, KVT, DP, 2, 2, QT>), g, b, 0, stream, a);
+    else
+        hipLaunchKernelGGL((tree_attn_kernel<T, KVT, DP, 4, 1, QT>), g, b, 0, stream, a);
     MQ_HIP(hipGetLastError());
 }
 
