@@ -37,96 +37,120 @@ struct TableArgs
 
 constexpr int PLAN_THREADS = 1024;
 
-// exclusive prefix sum over the workgroup; `sum` receives the total.  lds: [17] int64
-__device__ __forceinline__ int64_t exclusive_scan(int64_t v, int64_t* lds, int64_t& sum)
+// exclusive prefix sums of NV values over the workgroup; sum receives the totals
+template <int NV>
+__device__ __forceinline__ void exclusive_scan(const int64_t (&v)[NV], int64_t (&before)[NV], int64_t (&sum)[NV], int64_t (*lds)[PLAN_THREADS / 64])
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int64_t x = v;
+    int64_t x[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        x[i] = v[i];
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1)
-    {
-        const int64_t y = __shfl_up(x, o);
-        if (lane >= o)
-            x += y;
-    }
-    __syncthreads();
-    if (lane == 63)
-        lds[wave] = x;
-    __syncthreads();
-    int64_t base = 0, total = 0;
 #pragma unroll
-    for (int w = 0; w < PLAN_THREADS / 64; ++w)
+        for (int i = 0; i < NV; ++i)
+        {
+            const int64_t y = __shfl_up(x[i], o);
+            x[i] += lane >= o ? y : 0;
+        }
+    __syncthreads(); // the previous sums have been read
+    if (lane == 63)
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            lds[i][wave] = x[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
     {
-        if (w < wave)
-            base += lds[w];
-        total += lds[w];
+        before[i] = x[i] - v[i];
+        sum[i] = 0;
+        for (int w = 0; w < (int) blockDim.x / 64; ++w)
+        {
+            before[i] += w < wave ? lds[i][w] : 0;
+            sum[i] += lds[i][w];
+        }
     }
-    sum = total;
-    return base + x - v;
 }
 
+// x mod N for 0 <= x < 3 N (a 64-bit remainder is over a hundred instructions)
+__device__ __forceinline__ int wrap(int64_t x, int64_t N)
+{
+    x = x >= N ? x - N : x;
+    return (int) (x >= N ? x - N : x);
+}
+
+// one workgroup of up to 1024 threads
 __global__ __launch_bounds__(PLAN_THREADS) void table_plan_kernel(TableArgs p)
 {
-    __shared__ int64_t lds[PLAN_THREADS / 64];
+    __shared__ int64_t lds[3][PLAN_THREADS / 64];
     const int64_t N = p.num_blocks;
-    const int64_t head = ((p.free_state[0] % N) + N) % N;
+    const int head = p.free_state[0] >= 0 && p.free_state[0] < N ? p.free_state[0] : 0;
     const int64_t avail = min((int64_t) max(p.free_state[1], 0), N);
     int64_t demand = 0, granted = 0, returned = 0, tokens = 0;
-    for (int b0 = 0; b0 < p.batch; b0 += PLAN_THREADS)
+    for (int b0 = 0; b0 < p.batch; b0 += blockDim.x)
     {
         const int b = b0 + threadIdx.x;
         int count = 0, status = 0;
-        int64_t need = 0, back = 0, fresh = 0;
+        int64_t v[3] = {0, 0, 0}; // blocks asked for, blocks returned, tokens
         bool release = false;
         if (b < p.batch)
         {
             const int64_t past = p.past_lengths[b], add = p.new_lengths[b];
             count = p.block_counts[b];
             release = add < 0;
-            fresh = max(add, (int64_t) 0);
-            if (past < 0 || count < 0 || count > p.max_blocks)
+            v[2] = max(add, (int64_t) 0);
+            if (past < 0 || count < 0 || count > p.max_blocks || count > N)
                 status = 3;
             else if (release)
-                back = count;
+                v[1] = count;
             else
             {
                 const int64_t total = (past + add + p.tpb - 1) >> p.tpb_log2;
                 if (total > p.max_blocks)
                     status = 2;
                 else
-                    need = max(total - count, (int64_t) 0);
+                    v[0] = max(total - count, (int64_t) 0);
             }
         }
-        int64_t s_need, s_back, s_fresh, s_grant;
-        const int64_t need_from = demand + exclusive_scan(need, lds, s_need);
-        const int64_t back_from = returned + exclusive_scan(back, lds, s_back);
-        const int64_t tok_from = tokens + exclusive_scan(fresh, lds, s_fresh);
-        // first come, first served: a request that the blocks do not reach for gets none, nor does any behind it that asks
-        if (need > 0 && need_from + need > avail)
+        int64_t before[3], sum[3];
+        exclusive_scan(v, before, sum, lds);
+        // first come, first served: a request that the blocks do not reach for gets none, nor does any behind it that asks.
+        // So what is granted is the demand up to the first one refused
+        const int64_t from_need = demand + before[0];
+        int64_t need = v[0];
+        if (need > 0 && from_need + need > avail)
         {
             status = 1;
             need = 0;
         }
-        exclusive_scan(need, lds, s_grant);
+        const int64_t mine[1] = {need};
+        int64_t unused[1], grant[1];
+        if (demand + sum[0] > avail) // uniform
+            exclusive_scan(mine, unused, grant, lds);
+        else
+            grant[0] = sum[0];
         if (b < p.batch)
         {
             const bool gives = release && status == 0;
-            const int64_t from = gives ? head + avail + back_from : head + need_from;
-            p.rows[b] = make_int4(count, gives ? -1 : (int) need, (int) (from % N), status);
-            p.token_offsets[b] = (int) min(tok_from, (int64_t) INT32_MAX);
+            // ring positions of granted blocks end before the free ones do, those of returned blocks (more than N in all only
+            // with a corrupt state) behind them
+            const int64_t from = gives ? avail + min(returned + before[1], N) : min(from_need, N);
+            p.rows[b] = make_int4(count, gives ? -1 : (int) need, wrap(head + from, N), status);
+            p.token_offsets[b] = (int) min(tokens + before[2], (int64_t) INT32_MAX);
             p.status[b] = status;
             p.block_counts_out[b] = gives ? 0 : count + (int) need;
         }
-        demand += s_need;
-        returned += s_back;
-        tokens += s_fresh;
-        granted += s_grant;
+        demand += sum[0];
+        returned += sum[1];
+        tokens += sum[2];
+        granted += grant[0];
     }
-    __syncthreads();
+    __syncthreads(); // free_state has been read by everyone
     if (threadIdx.x == 0)
     {
         p.token_offsets[p.batch] = (int) min(tokens, (int64_t) INT32_MAX);
-        p.free_state_out[0] = (int) ((head + granted) % N);
+        p.free_state_out[0] = wrap(head + granted, N);
         p.free_state_out[1] = (int) min(avail - granted + returned, N);
     }
 }
@@ -137,7 +161,7 @@ __device__ __forceinline__ int block_index(const TableArgs& p, int b, const int4
     int idx = -1;
     if (row.y >= 0 && row.x >= 0 && row.x <= p.max_blocks && j < row.x + row.y)
         idx = j < row.x ? p.block_table[(size_t) b * p.max_blocks + j]
-                        : p.free_blocks[(int) (((int64_t) row.z + j - row.x) % p.num_blocks)];
+                        : p.free_blocks[wrap((int64_t) row.z + j - row.x, p.num_blocks)];
     return idx >= 0 && idx < p.num_blocks ? idx : -1;
 }
 
@@ -156,9 +180,9 @@ __global__ __launch_bounds__(256) void table_fill_kernel(TableArgs p)
         {
             int32_t* entry = p.block_table + (size_t) b * p.max_blocks + k;
             if (row.y < 0 && k < row.x) // released
-                p.free_blocks[(int) (((int64_t) row.z + k) % p.num_blocks)] = *entry;
+                p.free_blocks[wrap((int64_t) row.z + k, p.num_blocks)] = *entry;
             else if (row.y > 0 && k >= row.x && k < row.x + row.y) // granted
-                *entry = p.free_blocks[(int) (((int64_t) row.z + k - row.x) % p.num_blocks)];
+                *entry = p.free_blocks[wrap((int64_t) row.z + k - row.x, p.num_blocks)];
         }
         return;
     }
@@ -427,7 +451,7 @@ void kv_block_tables(const mi355q_kv_block_tables_params& q, hipStream_t stream)
     a.num_pools = q.num_pools;
     a.num_tokens = q.num_tokens;
     a.tpb = q.tokens_per_block;
-    hipLaunchKernelGGL(table_plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, stream, a);
+    hipLaunchKernelGGL(table_plan_kernel, dim3(1), dim3(std::min(PLAN_THREADS, (q.batch + 63) / 64 * 64)), 0, stream, a);
     MQ_HIP(hipGetLastError());
     // the pools are dealt over enough workgroups to fill the chip (a table entry is read once per group)
     const int per_pool = (q.max_blocks_per_seq + 511) / 512 * q.batch;

@@ -85,7 +85,7 @@ __device__ __forceinline__ bool tree_seq(const TreeArgs& p, int b, int& off, int
 }
 
 // ---------------------------------------------------------------------------------------------- 1. prepare
-// grid (max_draft + 1, batch).  Rotation and quantisation of K / V run in 64 bits: the angle of a far position has no
+// grid (max_draft + 1, batch, parts of the heads).  Rotation and quantisation of K / V run in 64 bits: the angle of a far position has no
 // correct digits left in fp32 (position 2^17, fp32 angle: error 2^-8 rad), and a value next to a rounding border of the
 // cache's type lands on the side the definition says.  It costs nothing that shows: 2 Hkv Dh values per token against the
 // whole history that the attention reads.
@@ -101,6 +101,8 @@ __global__ __launch_bounds__(TREE_THREADS) void tree_prepare_kernel(TreeArgs p, 
     const int64_t* kp = p.block_ptrs + (size_t) b * 2 * p.max_blocks;
     if (i == p.max_draft)
     {
+        if (blockIdx.z > 0)
+            return;
         // every block the sequence's keys live in has to be there (0 = not allocated)
         bool bad = !ok;
         if (ok)
@@ -146,7 +148,7 @@ __global__ __launch_bounds__(TREE_THREADS) void tree_prepare_kernel(TreeArgs p, 
     const int slot = past + i, blk = slot >> p.tpb_log2, tin = slot & (tpb - 1);
     char* const kdst = reinterpret_cast<char*>(kp[blk]);
     char* const vdst = reinterpret_cast<char*>(kp[p.max_blocks + blk]);
-    for (int it = threadIdx.x; it < nvec * cpv; it += TREE_THREADS)
+    for (int it = blockIdx.z * TREE_THREADS + threadIdx.x; it < nvec * cpv; it += gridDim.z * TREE_THREADS)
     {
         const int vec = it / cpv, d0 = 8 * (it % cpv);
         uint4* const qdst = reinterpret_cast<uint4*>(p.q_ws + ((size_t) row * Hq + vec) * PARTS * dp + d0);
@@ -157,41 +159,68 @@ __global__ __launch_bounds__(TREE_THREADS) void tree_prepare_kernel(TreeArgs p, 
                     qdst[part * dp / 8] = make_uint4(0, 0, 0, 0);
             continue;
         }
-        auto element = [&](int d) -> double // q / k / v element d of this head, bias added
+        // the 8 elements from d on of this head, bias added: exact in 64 bits
+        auto elements = [&](int d, double (&x)[8])
         {
-            const double x = T16<T>::to_float(src[vec * hs + d]);
-            return p.qkv_bias ? x + T16<T>::to_float(p.qkv_bias[vec * hs + d]) : x;
-        };
-        const uint4 r = *reinterpret_cast<const uint4*>(src + vec * hs + d0);
-        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-        double x[8], y[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            x[e] = (e & 1) ? T16<T>::hi(w[e >> 1]) : T16<T>::lo(w[e >> 1]);
-        if (p.qkv_bias)
-        {
-            const uint4 rb = *reinterpret_cast<const uint4*>(p.qkv_bias + vec * hs + d0);
-            const uint32_t wb[4] = {rb.x, rb.y, rb.z, rb.w};
+            const uint4 r = *reinterpret_cast<const uint4*>(src + vec * hs + d);
+            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                x[e] += (e & 1) ? T16<T>::hi(wb[e >> 1]) : T16<T>::lo(wb[e >> 1]);
-        }
+                x[e] = (e & 1) ? T16<T>::hi(w[e >> 1]) : T16<T>::lo(w[e >> 1]);
+            if (p.qkv_bias)
+            {
+                const uint4 rb = *reinterpret_cast<const uint4*>(p.qkv_bias + vec * hs + d);
+                const uint32_t wb[4] = {rb.x, rb.y, rb.z, rb.w};
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    x[e] += (e & 1) ? T16<T>::hi(wb[e >> 1]) : T16<T>::lo(wb[e >> 1]);
+            }
+        };
+        double x[8], y[8];
+        elements(d0, x);
 #pragma unroll
         for (int e = 0; e < 8; ++e)
             y[e] = x[e];
         if (rope && vec < Hq + Hkv && d0 < p.rot_dim)
         {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
+            if (p.pos_type == 1) // GPT-J pairs (2 j, 2 j + 1)
             {
-                const int d = d0 + e;
-                if (d < p.rot_dim)
+#pragma unroll
+                for (int e = 0; e < 8; e += 2)
+                    if (d0 + e < p.rot_dim)
+                    {
+                        const int j = (d0 + e) >> 1;
+                        y[e] = x[e] * cs_tab[j] - x[e + 1] * sn_tab[j];
+                        y[e + 1] = x[e + 1] * cs_tab[j] + x[e] * sn_tab[j];
+                    }
+            }
+            else if (half % 8 == 0) // NeoX pairs (j, j + rot_dim / 2): the partners are a chunk of their own
+            {
+                const bool first = d0 < half;
+                double other[8];
+                elements(first ? d0 + half : d0 - half, other);
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
                 {
-                    // NeoX pairs (d, d + rot_dim / 2), GPT-J pairs (2 j, 2 j + 1)
-                    const bool first = p.pos_type == 2 ? d < half : !(e & 1);
-                    const int j = p.pos_type == 2 ? (first ? d : d - half) : d >> 1;
-                    const double other = p.pos_type == 2 ? element(first ? d + half : d - half) : x[e ^ 1];
-                    y[e] = first ? x[e] * cs_tab[j] - other * sn_tab[j] : x[e] * cs_tab[j] + other * sn_tab[j];
+                    const int j = d0 + e - (first ? 0 : half);
+                    y[e] = x[e] * cs_tab[j] + (first ? -other[e] : other[e]) * sn_tab[j];
+                }
+            }
+            else
+            {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                {
+                    const int d = d0 + e;
+                    if (d < p.rot_dim)
+                    {
+                        const bool first = d < half;
+                        const int j = first ? d : d - half, at = vec * hs + (first ? d + half : d - half);
+                        double other = T16<T>::to_float(src[at]);
+                        if (p.qkv_bias)
+                            other += T16<T>::to_float(p.qkv_bias[at]);
+                        y[e] = x[e] * cs_tab[j] + (first ? -other : other) * sn_tab[j];
+                    }
                 }
             }
         }
@@ -516,22 +545,26 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
         cf32x4_t s[X2][QT];
 #pragma unroll
         for (int x = 0; x < X2; ++x)
-        {
-            const int row = kb + 16 * x + lr;
-            uint4 kf[KS];
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
-                kf[ks] = *reinterpret_cast<const uint4*>(kt + ROWB * row + 16 * ((4 * ks + lq) ^ sw(row)));
 #pragma unroll
             for (int qt = 0; qt < QT; ++qt)
-            {
                 s[x][qt] = minus_m[qt];
 #pragma unroll
-                for (int part = PARTS - 1; part >= 0; --part)
+        for (int ks = 0; ks < KS; ++ks) // consecutive products go to different accumulators
+        {
+            uint4 kf[X2];
 #pragma unroll
-                    for (int ks = 0; ks < KS; ++ks)
-                        s[x][qt] = ctx_mfma<C>(kf[ks], qf[part][qt][ks], s[x][qt]);
+            for (int x = 0; x < X2; ++x)
+            {
+                const int row = kb + 16 * x + lr;
+                kf[x] = *reinterpret_cast<const uint4*>(kt + ROWB * row + 16 * ((4 * ks + lq) ^ sw(row)));
             }
+#pragma unroll
+            for (int part = PARTS - 1; part >= 0; --part)
+#pragma unroll
+                for (int x = 0; x < X2; ++x)
+#pragma unroll
+                    for (int qt = 0; qt < QT; ++qt)
+                        s[x][qt] = ctx_mfma<C>(kf[x], qf[part][qt][ks], s[x][qt]);
         }
         if (tail)
         {
@@ -812,50 +845,57 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
 }
 
 // ---------------------------------------------------------------------------------------------- 3. combine
-// grid (max_draft, batch): one token; a wave takes the heads one after another.  Splits are summed in their order.
+// grid (max_draft, batch, ceil(heads / 4)): a wave joins one (token, head).  Splits are summed in their order, 8 loads in
+// flight.
 template <typename T, int DP>
 __global__ __launch_bounds__(TREE_THREADS) void tree_combine_kernel(TreeArgs p, bool quantised)
 {
     const int b = blockIdx.y, i = blockIdx.x, lane = threadIdx.x & 63;
+    const int h = blockIdx.z * (TREE_THREADS / 64) + (threadIdx.x >> 6);
     const int n = p.seq_nodes[b];
-    if (i >= n)
+    if (i >= n || h >= p.num_heads)
         return;
     const int ntiles = (p.past_lengths[b] + n + TREE_KT - 1) / TREE_KT;
     const int S = (ntiles + p.chunk_tiles - 1) / p.chunk_tiles; // <= 64
     if (S <= 1)
         return;
-    const float v_deq = quantised ? p.kv_scale_quant_orig[0] : 1.f;
-    const size_t row = p.draft_offsets[b] + i, stride = (size_t) p.num_tokens * p.num_heads;
-    constexpr int E = DP / 64;
-    for (int h = threadIdx.x >> 6; h < p.num_heads; h += TREE_THREADS / 64)
+    const size_t head = (size_t) (p.draft_offsets[b] + i) * p.num_heads + h, stride = (size_t) p.num_tokens * p.num_heads;
+    constexpr int E = DP / 64, U = 8;
+    const float2 ml = p.part_ml[min(lane, S - 1) * stride + head];
+    const float m = lane < S ? ml.x : NEG_BIG;
+    float mm = m;
+#pragma unroll
+    for (int x = 32; x >= 1; x >>= 1)
+        mm = fmaxf(mm, __shfl_xor(mm, x));
+    const float c = lane < S ? __builtin_amdgcn_exp2f(m - mm) : 0.f;
+    float l = lane < S ? ml.y * c : 0.f;
+#pragma unroll
+    for (int x = 32; x >= 1; x >>= 1)
+        l += __shfl_xor(l, x);
+    float acc[E] = {};
+    const float* src = p.part_acc + head * DP + E * lane;
+    for (int s0 = 0; s0 < S; s0 += U)
     {
-        const size_t head = row * p.num_heads + h;
-        const float2 ml = p.part_ml[min(lane, S - 1) * stride + head];
-        const float m = lane < S ? ml.x : NEG_BIG;
-        float mm = m;
+        float v[U][E];
 #pragma unroll
-        for (int x = 32; x >= 1; x >>= 1)
-            mm = fmaxf(mm, __shfl_xor(mm, x));
-        const float c = lane < S ? __builtin_amdgcn_exp2f(m - mm) : 0.f;
-        float l = lane < S ? ml.y * c : 0.f;
-#pragma unroll
-        for (int x = 32; x >= 1; x >>= 1)
-            l += __shfl_xor(l, x);
-        float acc[E] = {};
-        for (int s = 0; s < S; ++s)
-        {
-            const float cs = __shfl(c, s);
-            const float* src = p.part_acc + (s * stride + head) * DP + E * lane;
+        for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int e = 0; e < E; ++e)
-                acc[e] += src[e] * cs;
-        }
-        const float inv = l == 0.f ? 0.f : v_deq / l;
+                v[u][e] = src[min(s0 + u, S - 1) * stride * DP + e];
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (E * lane + e < p.hs)
-                p.out[head * p.hs + E * lane + e] = T16<T>::from_float(acc[e] * inv);
+        for (int u = 0; u < U; ++u)
+        {
+            const float cs = s0 + u < S ? __shfl(c, min(s0 + u, 63)) : 0.f;
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                acc[e] = s0 + u < S ? acc[e] + v[u][e] * cs : acc[e];
+        }
     }
+    const float inv = l == 0.f ? 0.f : (quantised ? p.kv_scale_quant_orig[0] : 1.f) / l;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        if (E * lane + e < p.hs)
+            p.out[head * p.hs + E * lane + e] = T16<T>::from_float(acc[e] * inv);
 }
 
 // ---------------------------------------------------------------------------------------------- host
@@ -947,7 +987,10 @@ void tree_launch_attn(const TreeArgs& a, const TreePlan& t, hipStream_t stream)
 template <typename T, int KVT>
 void tree_launch(const mi355q_tree_attention_params& q, const TreeArgs& a, const TreePlan& t, hipStream_t stream)
 {
-    hipLaunchKernelGGL((tree_prepare_kernel<T, KVT>), dim3(q.max_draft_length + 1, q.batch), dim3(TREE_THREADS), 0, stream, a, t.dp);
+    // a token's heads over several workgroups, one 8-element chunk a thread, while the tokens alone do not fill the chip
+    const int passes = ((q.num_heads + 2 * q.num_kv_heads) * t.dp / 8 + TREE_THREADS - 1) / TREE_THREADS;
+    const int parts = std::max(1, (int) std::min<int64_t>(passes, 2048 / ((int64_t) q.batch * q.max_draft_length)));
+    hipLaunchKernelGGL((tree_prepare_kernel<T, KVT>), dim3(q.max_draft_length + 1, q.batch, parts), dim3(TREE_THREADS), 0, stream, a, t.dp);
     MQ_HIP(hipGetLastError());
     if (t.dp == 64)
         tree_launch_attn<T, KVT, 64>(a, t, stream);
@@ -957,7 +1000,7 @@ void tree_launch(const mi355q_tree_attention_params& q, const TreeArgs& a, const
         tree_launch_attn<T, KVT, 256>(a, t, stream);
     if (t.splits > 1)
     {
-        const dim3 g(q.max_draft_length, q.batch), b(TREE_THREADS);
+        const dim3 g(q.max_draft_length, q.batch, (q.num_heads + 3) / 4), b(TREE_THREADS);
         if (t.dp == 64)
             hipLaunchKernelGGL((tree_combine_kernel<T, 64>), g, b, 0, stream, a, KVT != 0);
         else if (t.dp == 128)
