@@ -531,7 +531,8 @@ extern "C"
         int32_t max_draft_length;   /* host bound of a sequence's nodes, <= 1024 */
         int32_t max_past_length;    /* host bound of past_lengths */
         int32_t mask_words;         /* >= ceil(max_draft_length / 32) */
-        int32_t max_blocks_per_seq, tokens_per_block;
+        int32_t max_blocks_per_seq;
+        int32_t tokens_per_block;   /* a power of 2, 16 or more */
         int32_t act_type;           /* MI355Q_HALF / MI355Q_BF16 */
         int32_t kv_type;            /* act_type, MI355Q_INT8 or MI355Q_FP8 */
         int32_t position_embedding_type; /* 0 none applied here, 1 RoPE GPT-J, 2 RoPE GPT-NeoX */

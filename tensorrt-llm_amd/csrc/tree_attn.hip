@@ -12,6 +12,7 @@
 //   3. tree_combine_kernel, where the keys of a sequence were split over workgroups: joins the partial states.
 #include "attn_mfma.h"
 #include "decode_common.h"
+#include <type_traits>
 
 namespace mi355q
 {
@@ -20,7 +21,7 @@ namespace
 
 constexpr int TREE_KT = 64;         // keys per tile
 constexpr int TREE_THREADS = 256;   // 4 waves
-constexpr int TREE_MAX_SPLITS = 64; // lane = split in the combine kernel
+constexpr int TREE_MAX_SPLITS = 128; // teams that share a (sequence, kv head): what the combine kernel reads
 constexpr int TREE_MAX_DRAFT = 1024;
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -60,13 +61,15 @@ struct TreeArgs
     const float* kv_scale_quant_orig;
     uint16_t* q_ws;      // [tokens][Hq][1 or 2 parts][DP]: rotated, times the score scale (and the K dequantisation) and log2(e)
     int32_t* seq_nodes;  // [batch]: nodes of the sequence, 0 if it is skipped
-    float* part_acc;     // [splits][tokens * Hq][DP]
-    float2* part_ml;     // [splits][tokens * Hq] (running maximum in the log2 domain, sum)
+    int32_t* tile_start; // [batch + 1]: key tiles of the sequences before this one
+    float* part_acc;     // partial states: [team][first | last stretch][m-tile][row][DP]
+    float2* part_ml;     // their (running maximum in the log2 domain, sum)
     int64_t qkv_stride;
     int batch, num_heads, num_kv_heads, group, hs;
     int num_tokens, max_draft, max_past, mask_words;
     int max_blocks, tpb_log2;
-    int mtiles, chunk_tiles, splits, groups; // groups = batch * kv heads * splits
+    int mtiles, rows_per_wg, teams, min_chunk;
+    int whole; // a team takes one (sequence, kv head) from end to end: nothing is joined
     int pos_type, rot_dim, rot_scale_type, rot_max_pos;
     double rot_log2_base, rot_scale;
     float score_scale;
@@ -84,8 +87,50 @@ __device__ __forceinline__ bool tree_seq(const TreeArgs& p, int b, int& off, int
         && keys <= ((int64_t) p.max_blocks << p.tpb_log2);
 }
 
+// the key tiles before every sequence, by one workgroup
+__device__ __forceinline__ void tree_count_tiles(const TreeArgs& p)
+{
+    __shared__ int wave_sum[TREE_THREADS / 64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int carry = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += TREE_THREADS)
+    {
+        const int b = b0 + threadIdx.x;
+        int off, n, past, x = 0;
+        if (b < p.batch && tree_seq(p, b, off, n, past))
+            x = (past + n + TREE_KT - 1) / TREE_KT;
+        const int mine = x;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1)
+        {
+            const int y = __shfl_up(x, o);
+            x += lane >= o ? y : 0;
+        }
+        if (lane == 63)
+            wave_sum[wave] = x;
+        __syncthreads();
+        int before = carry;
+        for (int w = 0; w < TREE_THREADS / 64; ++w)
+        {
+            before += w < wave ? wave_sum[w] : 0;
+            carry += wave_sum[w];
+        }
+        if (b < p.batch)
+            p.tile_start[b] = before + x - mine;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0)
+        p.tile_start[p.batch] = carry;
+}
+
+// tiles of a team's stretch: all (sequence, kv head, tile) units in equal parts
+__device__ __forceinline__ int tree_chunk(const TreeArgs& p, int units)
+{
+    return max((units + p.teams - 1) / p.teams, p.min_chunk);
+}
+
 // ---------------------------------------------------------------------------------------------- 1. prepare
-// grid (max_draft + 1, batch, parts of the heads).  Rotation and quantisation of K / V run in 64 bits: the angle of a far position has no
+// grid (max_draft + 2, batch, parts of the heads).  Rotation and quantisation of K / V run in 64 bits: the angle of a far position has no
 // correct digits left in fp32 (position 2^17, fp32 angle: error 2^-8 rad), and a value next to a rounding border of the
 // cache's type lands on the side the definition says.  It costs nothing that shows: 2 Hkv Dh values per token against the
 // whole history that the attention reads.
@@ -96,6 +141,12 @@ __global__ __launch_bounds__(TREE_THREADS) void tree_prepare_kernel(TreeArgs p, 
     constexpr int PARTS = TREE_Q2<T, KVT> ? 2 : 1;
     const int b = blockIdx.y, i = blockIdx.x;
     int off, n, past;
+    if (i == p.max_draft + 1)
+    {
+        if (b == 0 && blockIdx.z == 0)
+            tree_count_tiles(p);
+        return;
+    }
     const bool ok = tree_seq(p, b, off, n, past);
     const int tpb = 1 << p.tpb_log2;
     const int64_t* kp = p.block_ptrs + (size_t) b * 2 * p.max_blocks;
@@ -308,6 +359,14 @@ __device__ __forceinline__ uint4 tree_kv8_to_f16(uint32_t w0, uint32_t w1)
     return r;
 }
 
+// 16 bytes of the LDS from a byte address
+__device__ __forceinline__ uint4 tree_lds16(uint32_t address)
+{
+    typedef __attribute__((ext_vector_type(4))) uint32_t u32x4_t;
+    const u32x4_t v = *(const __attribute__((address_space(3))) u32x4_t*) (uintptr_t) address;
+    return make_uint4(v.x, v.y, v.z, v.w);
+}
+
 // 16 bytes from an address that was an integer in a table: a global load (a plain cast would make it a flat one)
 __device__ __forceinline__ uint4 tree_load16(int64_t address)
 {
@@ -351,18 +410,22 @@ __device__ __forceinline__ uint64_t tree_mask64(const uint32_t* row, int words, 
     return live >= 64 ? v : (live <= 0 ? 0ull : v & ((1ull << live) - 1));
 }
 
-// grid: 1-D, ((group / 8) * mtiles + m) * 8 + group % 8 with group = (sequence, kv head, split): workgroups are dealt to the
-// 8 XCDs round-robin, so the m-tiles that share a stretch of keys run on one XCD and read it from HBM once.
-// A workgroup = RW * QT * 16 query rows (row r = node r / G, head r % G of the kv head's G query heads) x chunk_tiles tiles of
-// 64 keys.  Its 4 waves are RW row groups x KW key groups: with few rows the waves share the keys of a tile instead of
-// idling, and merge their states at the end.
+// grid: 1-D, ((team / 8) * mtiles + m) * 8 + team % 8: workgroups are dealt to the 8 XCDs round-robin, so a team -- the m-tiles
+// that walk the same keys -- runs on one XCD and reads them from HBM once.
+// The keys of all sequences and kv heads, as one line of 64-key tiles, are cut into equal stretches, one per team: ragged
+// batches and single long sequences load the chip alike.  A stretch that covers a (sequence, kv head) entirely writes
+// its output; a part of one leaves its state for the combine kernel (a team has at most two such parts: its first and
+// its last).
+// A workgroup = RW * QT * 16 query rows (row r = node r / G, head r % G of the kv head's G query heads).  Its 4 waves are RW row
+// groups x KW key groups: with few rows the waves share the keys of a tile instead of idling, and merge their states at
+// the end.
 // S^T = K . Q^T (16x16x32): a lane holds one query column's scores of 4 consecutive keys, and the same registers, rounded
-// to T, are the B operand of O^T += V^T . P^T.
+// to the compute type, are the B operand of O^T += V^T . P^T.
 // Softmax in the log2 domain with the running maximum as the C operand of the first product: what comes out is already
-// s - m, and as long as no column grows past m + 8 (p <= 256: harmless in T and in the fp32 sums) nothing is rescaled.
+// s - m, and as long as no column grows past m + 8 (p <= 256: harmless in fp16 / bf16 and in the fp32 sums) nothing is rescaled.
 // Whether one does is an integer maximum over the raw bits (negative floats are negative integers).
-template <typename T, int KVT, int DP, int RW, int KW, int QT>
-__global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP > 128 ? 1 : 2))) void tree_attn_kernel(TreeArgs p)
+template <typename T, int KVT, int DP, int RW, int KW, int QT, int NS>
+__global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP > 128 || NS > 2 ? 1 : 2))) void tree_attn_kernel(TreeArgs p)
 {
     static_assert(RW * KW == 4, "4 waves");
     typedef typename TreeCompute<T, KVT>::type C;
@@ -372,43 +435,64 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
     constexpr int ROWB = DP * 2, CH = ROWB / 16;
     constexpr int TILE_BYTES = TREE_KT * ROWB, STAGE_BYTES = 2 * TILE_BYTES;
     constexpr int XW = 4 / KW;                      // 16-key subtiles per wave
+    constexpr int X2 = XW < 2 ? XW : 2;             // subtiles per compute step: 32 keys, or 16 with four key groups
     constexpr int WROWS = TREE_KT / 4;              // a wave loads 16 consecutive keys of a tile
     constexpr int RPD = 1024 / ROWB, DPW = WROWS / RPD; // 16-bit caches: rows per DMA instruction, DMAs per wave
     constexpr int CH8 = DP / 16, RPL = 64 / CH8, LPT = WROWS / RPL; // 8-bit caches: rows per 16-byte load, loads per thread
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE_BYTES];
-    __shared__ uint32_t nonfinite[2]; // keys of the tile whose V row has an infinity or NaN
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[NS * STAGE_BYTES];
+    __shared__ uint32_t nonfinite[TREE_MAX_DRAFT / 32]; // nodes of the stretch whose V row has an infinity or NaN
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int rw = wave % RW, kw = wave / RW;
     const int lr = lane & 15, lq = lane >> 4;
     const int mt = (blockIdx.x >> 3) % p.mtiles;
-    const int grp = (blockIdx.x >> 3) / p.mtiles * 8 + (blockIdx.x & 7);
-    if (grp >= p.groups)
+    const int team = (blockIdx.x >> 3) / p.mtiles * 8 + (blockIdx.x & 7);
+    if (team >= p.teams)
         return;
-    const int split = grp % p.splits, hk = grp / p.splits % p.num_kv_heads, b = grp / p.splits / p.num_kv_heads;
-    const int n = p.seq_nodes[b], G = p.group;
-    if (mt * M >= n * G)
-        return;
-    const int off = p.draft_offsets[b], past = p.past_lengths[b], total = past + n;
-    const int ntiles = (total + TREE_KT - 1) / TREE_KT;
-    const int tile_lo = split * p.chunk_tiles, tile_hi = min(ntiles, tile_lo + p.chunk_tiles);
-    if (tile_lo >= ntiles)
-        return;
-    const bool alone = ntiles <= p.chunk_tiles; // the sequence was not split
-    const int hs = p.hs, tpb_mask = (1 << p.tpb_log2) - 1;
+    const int G = p.group, hs = p.hs, tpb_mask = (1 << p.tpb_log2) - 1;
     const int row_bytes = hs * (KVT ? 1 : 2); // of a head in the cache
-    const int64_t* const kp = p.block_ptrs + (size_t) b * 2 * p.max_blocks;
-    const int64_t* const vp = kp + p.max_blocks;
 
-    // swizzle of the 16-byte chunk index by the row, K and V alike: 16 consecutive rows x one chunk (a K fragment) and 4 rows
-    // x two chunks (a transposing V read) fall on different banks
-    auto sw = [](int row) { return CH >= 16 ? ((row & 3) << 2 | ((row >> 2) & 3)) : (((row >> 1) & 3) << 1 | ((row >> 3) & 1)); };
+    // swizzle of the 16-byte chunk index by the row, K and V alike.  The banks see a 16-byte read of 64 lanes in groups of rows
+    // 0-3, 12-15 at one chunk with rows 4-11 at its neighbour (K fragments: row = lane & 15), and a transposing read in groups of
+    // 4 rows x 2 chunks (V): both fall on all banks once.  It depends on the row modulo 16 only.
+    auto sw = [](int row)
+    {
+        const int x = (row >> 2) & 3;
+        return CH >= 16 ? (row & 3) << 2 | ((x ^ x >> 1) & 1) << 1 | x >> 1 : ((row >> 1) & 3) << 1;
+    };
 
-    // ---- tile loads.  A wave loads 16 consecutive keys, which lie in one block (of at least 16 tokens): the block's address is
-    // a scalar load, issued a tile ahead, and a lane adds a fixed 32-bit offset.  16-bit caches: LDS-DMA, instruction d of a
-    // tile fills LDS bytes [1024 d, +1024), the swizzle applied on the source address.  8-bit caches: through registers,
-    // converted on the way into the LDS.  Keys past the sequence are whatever its last block holds there.
+    // ---- the team's stretch of units (sequence, kv head, tile)
+    int b = 0, hk = 0, tile = 0, left; // left: tiles of the stretch still to do
+    if (p.whole)
+    {
+        b = team / p.num_kv_heads;
+        hk = team % p.num_kv_heads;
+        left = p.tile_start[b + 1] - p.tile_start[b];
+    }
+    else
+    {
+        const int units = p.tile_start[p.batch] * p.num_kv_heads;
+        const int chunk = tree_chunk(p, units);
+        const int64_t u0 = (int64_t) team * chunk;
+        left = (int) min((int64_t) chunk, units - u0);
+        if (left <= 0)
+            return;
+        const int at = (int) u0 / p.num_kv_heads; // the sequences that end at or before this tile
+        for (int b0 = 0; b0 < p.batch; b0 += 64)
+        {
+            const uint64_t done = __ballot(b0 + lane < p.batch && p.tile_start[min(b0 + lane + 1, p.batch)] <= at);
+            b += __builtin_popcountll(done);
+            if (done != ~0ull)
+                break;
+        }
+        b = __builtin_amdgcn_readfirstlane(b);
+        const int nt = p.tile_start[b + 1] - p.tile_start[b], in_seq = (int) u0 - p.tile_start[b] * p.num_kv_heads;
+        hk = in_seq / nt;
+        tile = in_seq % nt;
+    }
+
+    // ---- what does not change from stretch to stretch
     const uint32_t lds_base = __builtin_amdgcn_readfirstlane((uint32_t) (uintptr_t) (ctx_lds_void_t*) lds);
     const int last_chunk = row_bytes / 16 - 1; // heads narrower than DP: the padding re-reads the last chunk (q is 0 there)
     constexpr int LOADS = KVT ? LPT : DPW;
@@ -416,482 +500,516 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
 #pragma unroll
     for (int i = 0; i < LOADS; ++i)
     {
-        const int r = i * (KVT ? RPL : RPD) + lane / (KVT ? CH8 : CH), row = wave * WROWS + r; // row of the wave's 16, of the tile
+        const int r = i * (KVT ? RPL : RPD) + lane / (KVT ? CH8 : CH); // row of the wave's 16
         const int ch = lane % (KVT ? CH8 : CH);
-        lane_off[i] = r * row_bytes + 16 * min(KVT ? ch : ch ^ sw(row), last_chunk);
-    }
-    const bool one_block = p.tpb_log2 >= 4;
-    typedef const __attribute__((address_space(4))) int64_t* scalar_ptr;
-    int64_t kbase = 0, vbase = 0; // where the wave's 16 keys of the tile to be loaded next begin
-    auto find_tile = [&](int tile)
-    {
-        if (one_block)
-        {
-            const int t0 = tile * TREE_KT + wave * WROWS;
-            const int blk = __builtin_amdgcn_readfirstlane(min(t0, total - 1) >> p.tpb_log2);
-            const int64_t in_block = (((int64_t) hk << p.tpb_log2) + (t0 & tpb_mask)) * row_bytes;
-            kbase = ((scalar_ptr) kp)[blk] + in_block;
-            vbase = ((scalar_ptr) vp)[blk] + in_block;
-        }
-    };
-    uint4 kreg[KVT ? LPT : 1], vreg[KVT ? LPT : 1];
-    auto load_tile = [&](int tile, int buf)
-    {
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i)
-        {
-            const uint32_t dst = lds_base + buf * STAGE_BYTES + (wave * DPW + i) * 1024;
-            if (one_block)
-            {
-                if constexpr (KVT == 0)
-                {
-                    tree_dma16(kbase, lane_off[i], dst);
-                    tree_dma16(vbase, lane_off[i], dst + TILE_BYTES);
-                }
-                else
-                {
-                    kreg[i] = tree_load16(kbase + lane_off[i]);
-                    vreg[i] = tree_load16(vbase + lane_off[i]);
-                }
-            }
-            else // blocks of 1 - 8 tokens: every lane looks its key's block up
-            {
-                const int r = i * (KVT ? RPL : RPD) + lane / (KVT ? CH8 : CH);
-                const int t = min(tile * TREE_KT + wave * WROWS + r, total - 1);
-                const int64_t in_block = (((int64_t) hk << p.tpb_log2) + (t & tpb_mask) - r) * row_bytes;
-                const int64_t ka = kp[t >> p.tpb_log2] + in_block + lane_off[i], va = vp[t >> p.tpb_log2] + in_block + lane_off[i];
-                if constexpr (KVT == 0)
-                {
-                    ctx_dma16(reinterpret_cast<const void*>(ka), dst);
-                    ctx_dma16(reinterpret_cast<const void*>(va), dst + TILE_BYTES);
-                }
-                else
-                {
-                    kreg[i] = tree_load16(ka);
-                    vreg[i] = tree_load16(va);
-                }
-            }
-        }
-    };
-    auto store_tile = [&](int buf) // 8-bit caches
-    {
-        if constexpr (KVT != 0)
-        {
-#pragma unroll
-            for (int i = 0; i < LPT; ++i)
-            {
-                const int row = wave * WROWS + i * RPL + lane / CH8, ch = 2 * (lane % CH8);
-                uint8_t* kt = lds + buf * STAGE_BYTES + ROWB * row;
-                uint8_t* vt = kt + TILE_BYTES;
-                *reinterpret_cast<uint4*>(kt + 16 * (ch ^ sw(row))) = tree_kv8_to_f16<KVT>(kreg[i].x, kreg[i].y);
-                *reinterpret_cast<uint4*>(kt + 16 * ((ch + 1) ^ sw(row))) = tree_kv8_to_f16<KVT>(kreg[i].z, kreg[i].w);
-                *reinterpret_cast<uint4*>(vt + 16 * (ch ^ sw(row))) = tree_kv8_to_f16<KVT>(vreg[i].x, vreg[i].y);
-                *reinterpret_cast<uint4*>(vt + 16 * ((ch + 1) ^ sw(row))) = tree_kv8_to_f16<KVT>(vreg[i].z, vreg[i].w);
-            }
-        }
-    };
-
-    find_tile(tile_lo);
-    load_tile(tile_lo, tile_lo & 1);
-    find_tile(min(tile_lo + 1, tile_hi - 1));
-    // ---- Q^T fragments (B operand): column = row q0 + 16 qt + lr, k = d = 32 ks + 8 lq + j
-    const int q0 = mt * M + rw * QT * 16;
-    uint4 qf[PARTS][QT][KS];
-    int node[QT];
-#pragma unroll
-    for (int qt = 0; qt < QT; ++qt)
-    {
-        const int r = min(q0 + 16 * qt + lr, n * G - 1); // rows past the last re-read it; never stored
-        node[qt] = r / G;
-        const uint16_t* q = p.q_ws + ((size_t) (off + node[qt]) * p.num_heads + hk * G + r % G) * PARTS * DP;
-#pragma unroll
-        for (int part = 0; part < PARTS; ++part)
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
-                qf[part][qt][ks] = *reinterpret_cast<const uint4*>(q + part * DP + 32 * ks + 8 * lq);
-    }
-    // end the compiler's own bookkeeping of the q loads here, before the loop's (to it invisible) DMAs
-#pragma unroll
-    for (int part = 0; part < PARTS; ++part)
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt)
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
-                asm volatile("" : "+v"(qf[part][qt][ks].x), "+v"(qf[part][qt][ks].y), "+v"(qf[part][qt][ks].z), "+v"(qf[part][qt][ks].w));
-
-    float l_run[QT];
-    cf32x4_t minus_m[QT]; // C operand of the scores: minus the running maximum
-    bool fresh[QT];       // the column has no maximum yet (minus_m is 0)
-    cf32x4_t o[QT][DT];
-#pragma unroll
-    for (int qt = 0; qt < QT; ++qt)
-    {
-        fresh[qt] = true;
-        l_run[qt] = 0.f;
-        minus_m[qt] = cf32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-            o[qt][dt] = cf32x4_t{0.f, 0.f, 0.f, 0.f};
+        lane_off[i] = r * row_bytes + 16 * min(KVT ? ch : ch ^ sw(r), last_chunk);
     }
     const int rq = lr >> 2, rp = lr & 3;
     const int kb0 = kw * 16 * XW; // this wave's first key of a tile
+    // LDS addresses of a lane's fragments in stage 0: K row lr, chunk lq (+ 4 ks by XOR); V row 4 lq + rq, column 4 rp (+ 16 dt by XOR)
+    const uint32_t k_addr = lds_base + ROWB * (kb0 + lr) + 16 * (lq ^ sw(lr));
+    const uint32_t v_addr = lds_base + TILE_BYTES + ROWB * (kb0 + 4 * lq + rq) + 16 * ((rp >> 1) ^ sw(4 * lq + rq)) + 8 * (rp & 1);
+    typedef const __attribute__((address_space(4))) int64_t* scalar_ptr;
 
-    // 32 keys (16 with four key groups) from key kb of the tile on
-    constexpr int X2 = XW < 2 ? XW : 2;
-    auto compute = [&](int buf, int t0, int kb, bool tail)
+    while (left > 0)
     {
-        const uint8_t* kt = lds + buf * STAGE_BYTES;
-        const uint8_t* vt = kt + TILE_BYTES;
-        cf32x4_t s[X2][QT];
-#pragma unroll
-        for (int x = 0; x < X2; ++x)
-#pragma unroll
-            for (int qt = 0; qt < QT; ++qt)
-                s[x][qt] = minus_m[qt];
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) // consecutive products go to different accumulators
+        const int nt = p.tile_start[b + 1] - p.tile_start[b];
+        const int tile_lo = tile, tile_hi = min(nt, tile + left);
+        const int seq = b, head_kv = hk;
+        left -= tile_hi - tile_lo;
+        tile = 0;
+        if (++hk == p.num_kv_heads)
         {
-            uint4 kf[X2];
-#pragma unroll
-            for (int x = 0; x < X2; ++x)
-            {
-                const int row = kb + 16 * x + lr;
-                kf[x] = *reinterpret_cast<const uint4*>(kt + ROWB * row + 16 * ((4 * ks + lq) ^ sw(row)));
-            }
-#pragma unroll
-            for (int part = PARTS - 1; part >= 0; --part)
-#pragma unroll
-                for (int x = 0; x < X2; ++x)
-#pragma unroll
-                    for (int qt = 0; qt < QT; ++qt)
-                        s[x][qt] = ctx_mfma<C>(kf[x], qf[part][qt][ks], s[x][qt]);
+            hk = 0;
+            ++b;
         }
-        if (tail)
+        const int n = tile_hi > tile_lo ? p.seq_nodes[seq] : 0;
+        if (mt * M >= n * G) // an empty sequence, one that is skipped, or no rows for this m-tile
+            continue;
+        const int off = p.draft_offsets[seq], past = p.past_lengths[seq], total = past + n;
+        const int64_t* const kp = p.block_ptrs + (size_t) seq * 2 * p.max_blocks;
+        const int64_t* const vp = kp + p.max_blocks;
+
+        // ---- tile loads.  A wave loads 16 consecutive keys, which lie in one block (tokens_per_block >= 16): the block's address
+        // is a scalar load, issued a tile ahead, and a lane adds a fixed 32-bit offset.  16-bit caches: LDS-DMA, instruction d of
+        // a tile fills LDS bytes [1024 d, +1024), the swizzle applied on the source address.  8-bit caches: through registers,
+        // converted on the way into the LDS.  Keys past the sequence are whatever its last block holds there.
+        int64_t kbase = 0, vbase = 0; // where the wave's 16 keys of the tile to be loaded next begin
+        auto find_tile = [&](int i)
+        {
+            const int t0 = i * TREE_KT + wave * WROWS;
+            const int blk = __builtin_amdgcn_readfirstlane(min(t0, total - 1) >> p.tpb_log2);
+            const int64_t in_block = (((int64_t) head_kv << p.tpb_log2) + (t0 & tpb_mask)) * row_bytes;
+            kbase = ((scalar_ptr) kp)[blk] + in_block;
+            vbase = ((scalar_ptr) vp)[blk] + in_block;
+        };
+        uint4 kreg[KVT ? LPT : 1], vreg[KVT ? LPT : 1];
+        auto load_tile = [&](uint32_t stage)
         {
 #pragma unroll
-            for (int qt = 0; qt < QT; ++qt)
+            for (int d = 0; d < LOADS; ++d)
             {
-                const uint64_t seen
-                    = tree_mask64(p.tree_mask + (size_t) (off + node[qt]) * p.mask_words, p.mask_words, n, t0 - past) >> (kb + 4 * lq);
-#pragma unroll
-                for (int x = 0; x < X2; ++x)
-#pragma unroll
-                    for (int rr = 0; rr < 4; ++rr)
-                        s[x][qt][rr] = (seen >> (16 * x + rr)) & 1 ? s[x][qt][rr] : -__builtin_inff();
+                if constexpr (KVT == 0)
+                {
+                    const uint32_t dst = lds_base + stage + (wave * DPW + d) * 1024;
+                    tree_dma16(kbase, lane_off[d], dst);
+                    tree_dma16(vbase, lane_off[d], dst + TILE_BYTES);
+                }
+                else
+                {
+                    kreg[d] = tree_load16(kbase + lane_off[d]);
+                    vreg[d] = tree_load16(vbase + lane_off[d]);
+                }
             }
+        };
+        auto store_tile = [&](uint32_t stage) // 8-bit caches
+        {
+            if constexpr (KVT != 0)
+            {
+#pragma unroll
+                for (int d = 0; d < LPT; ++d)
+                {
+                    const int r = d * RPL + lane / CH8, ch = 2 * (lane % CH8);
+                    uint8_t* kt = lds + stage + ROWB * (wave * WROWS + r);
+                    uint8_t* vt = kt + TILE_BYTES;
+                    *reinterpret_cast<uint4*>(kt + 16 * (ch ^ sw(r))) = tree_kv8_to_f16<KVT>(kreg[d].x, kreg[d].y);
+                    *reinterpret_cast<uint4*>(kt + 16 * ((ch + 1) ^ sw(r))) = tree_kv8_to_f16<KVT>(kreg[d].z, kreg[d].w);
+                    *reinterpret_cast<uint4*>(vt + 16 * (ch ^ sw(r))) = tree_kv8_to_f16<KVT>(vreg[d].x, vreg[d].y);
+                    *reinterpret_cast<uint4*>(vt + 16 * ((ch + 1) ^ sw(r))) = tree_kv8_to_f16<KVT>(vreg[d].z, vreg[d].w);
+                }
+            }
+        };
+
+        __syncthreads(); // everyone is done with the LDS of the stretch before
+        if (KVT == 0 && tid < TREE_MAX_DRAFT / 32)
+            nonfinite[tid] = 0; // (the barrier of the first tile comes before the first use)
+        constexpr int AHEAD = KVT ? 1 : NS - 1; // tiles in flight
+        find_tile(tile_lo);
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+        {
+            if (tile_lo + i < tile_hi)
+                load_tile(i * STAGE_BYTES);
+            find_tile(min(tile_lo + i + 1, tile_hi - 1));
         }
-        uint32_t pk[QT][X2][2];
+        // ---- Q^T fragments (B operand): column = row q0 + 16 qt + lr, k = d = 32 ks + 8 lq + j
+        const int q0 = mt * M + rw * QT * 16;
+        uint4 qf[PARTS][QT][KS];
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt)
         {
-            int mx = 0; // the largest positive s - m, as raw bits
+            const int r = min(q0 + 16 * qt + lr, n * G - 1); // rows past the last re-read it; never stored
+            const uint16_t* q = p.q_ws + ((size_t) (off + r / G) * p.num_heads + head_kv * G + r % G) * PARTS * DP;
+#pragma unroll
+            for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks)
+                    qf[part][qt][ks] = *reinterpret_cast<const uint4*>(q + part * DP + 32 * ks + 8 * lq);
+        }
+        // end the compiler's own bookkeeping of the q loads here, before the loop's (to it invisible) DMAs
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks)
+                    asm volatile("" : "+v"(qf[part][qt][ks].x), "+v"(qf[part][qt][ks].y), "+v"(qf[part][qt][ks].z), "+v"(qf[part][qt][ks].w));
+
+        float l_run[QT];
+        cf32x4_t minus_m[QT]; // C operand of the scores: minus the running maximum
+        bool fresh[QT];       // the column has no maximum yet (minus_m is 0)
+        cf32x4_t o[QT][DT];
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt)
+        {
+            fresh[qt] = true;
+            l_run[qt] = 0.f;
+            minus_m[qt] = cf32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+                o[qt][dt] = cf32x4_t{0.f, 0.f, 0.f, 0.f};
+        }
+
+        // One compute step: X2 subtiles from key `kb` of the tile in `stage` on.  GENERAL: columns may still be fresh, keys hidden.
+        auto step = [&](auto general, uint32_t stage, int kb, int t0)
+        {
+            constexpr bool GENERAL = decltype(general)::value;
+            const uint32_t ka = k_addr + stage + kb * ROWB, va = v_addr + stage + kb * ROWB;
+            cf32x4_t s[X2][QT];
 #pragma unroll
             for (int x = 0; x < X2; ++x)
 #pragma unroll
-                for (int rr = 0; rr < 4; ++rr)
-                    mx = max(mx, __builtin_bit_cast(int, (float) s[x][qt][rr]));
-            if (__any(fresh[qt] || mx > 0x41000000 /* 8.0f */)) // wave-uniform
+                for (int qt = 0; qt < QT; ++qt)
+                    s[x][qt] = minus_m[qt];
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) // consecutive products go to different accumulators
             {
-                // the column's maximum of these keys, over its 4 lanes (a NaN stays out of the comparison and in the scores)
-                float top = -__builtin_inff();
+                uint4 kf[X2];
 #pragma unroll
                 for (int x = 0; x < X2; ++x)
+                    kf[x] = tree_lds16((ka ^ (64 * ks)) + 16 * x * ROWB);
 #pragma unroll
-                    for (int rr = 0; rr < 4; ++rr)
-                        top = fmaxf(top, s[x][qt][rr]);
-                top = fmaxf(top, __shfl_xor(top, 16));
-                top = fmaxf(top, __shfl_xor(top, 32));
-                if (top != -__builtin_inff())
+                for (int part = PARTS - 1; part >= 0; --part)
+#pragma unroll
+                    for (int x = 0; x < X2; ++x)
+#pragma unroll
+                        for (int qt = 0; qt < QT; ++qt)
+                            s[x][qt] = ctx_mfma<C>(kf[x], qf[part][qt][ks], s[x][qt]);
+            }
+            if (GENERAL && t0 + TREE_KT > past)
+            {
+#pragma unroll
+                for (int qt = 0; qt < QT; ++qt)
                 {
-                    const float up = fresh[qt] ? top : fmaxf(top, 0.f);
-                    const float corr = fresh[qt] ? 0.f : __builtin_amdgcn_exp2f(-up); // (nothing was summed before the first maximum)
-                    const float mm = minus_m[qt][0] - up;
-                    minus_m[qt] = cf32x4_t{mm, mm, mm, mm};
-                    fresh[qt] = false;
-                    l_run[qt] *= corr;
-#pragma unroll
-                    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                        for (int rr = 0; rr < 4; ++rr)
-                            o[qt][dt][rr] *= corr;
+                    const int node = min(q0 + 16 * qt + lr, n * G - 1) / G;
+                    const uint64_t seen = tree_mask64(p.tree_mask + (size_t) (off + node) * p.mask_words, p.mask_words, n, t0 - past)
+                        >> (kb0 + kb + 4 * lq);
 #pragma unroll
                     for (int x = 0; x < X2; ++x)
 #pragma unroll
                         for (int rr = 0; rr < 4; ++rr)
-                            s[x][qt][rr] -= up;
+                            s[x][qt][rr] = (seen >> (16 * x + rr)) & 1 ? s[x][qt][rr] : -__builtin_inff();
                 }
             }
+            uint32_t pk[QT][X2][2];
 #pragma unroll
-            for (int x = 0; x < X2; ++x)
+            for (int qt = 0; qt < QT; ++qt)
             {
-                float e[4];
+                int mx = 0; // the largest positive s - m, as raw bits
 #pragma unroll
-                for (int rr = 0; rr < 4; ++rr)
+                for (int x = 0; x < X2; ++x)
+#pragma unroll
+                    for (int rr = 0; rr < 4; ++rr)
+                        mx = max(mx, __builtin_bit_cast(int, (float) s[x][qt][rr]));
+                const bool first = GENERAL && fresh[qt];
+                if (__any(first || mx > 0x41000000 /* 8.0f */)) // wave-uniform
                 {
-                    e[rr] = __builtin_amdgcn_exp2f(s[x][qt][rr]);
-                    l_run[qt] += e[rr];
+                    // the column's maximum of these keys, over its 4 lanes (a NaN stays out of the comparison and in the scores)
+                    float top = -__builtin_inff();
+#pragma unroll
+                    for (int x = 0; x < X2; ++x)
+#pragma unroll
+                        for (int rr = 0; rr < 4; ++rr)
+                            top = fmaxf(top, s[x][qt][rr]);
+                    top = fmaxf(top, __shfl_xor(top, 16));
+                    top = fmaxf(top, __shfl_xor(top, 32));
+                    if (top != -__builtin_inff())
+                    {
+                        const float up = first ? top : fmaxf(top, 0.f);
+                        const float corr = first ? 0.f : __builtin_amdgcn_exp2f(-up); // (nothing was summed before the first maximum)
+                        const float mm = minus_m[qt][0] - up;
+                        minus_m[qt] = cf32x4_t{mm, mm, mm, mm};
+                        if constexpr (GENERAL)
+                            fresh[qt] = false;
+                        l_run[qt] *= corr;
+#pragma unroll
+                        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                            for (int rr = 0; rr < 4; ++rr)
+                                o[qt][dt][rr] *= corr;
+#pragma unroll
+                        for (int x = 0; x < X2; ++x)
+#pragma unroll
+                            for (int rr = 0; rr < 4; ++rr)
+                                s[x][qt][rr] -= up;
+                    }
                 }
-                // P in the compute type: its rounding (half a step, relative) averages out over the keys
-                pk[qt][x][0] = pack2<C>(e[0], e[1]);
-                pk[qt][x][1] = pack2<C>(e[2], e[3]);
+#pragma unroll
+                for (int x = 0; x < X2; ++x)
+                {
+                    float e[4];
+#pragma unroll
+                    for (int rr = 0; rr < 4; ++rr)
+                    {
+                        e[rr] = __builtin_amdgcn_exp2f(s[x][qt][rr]);
+                        l_run[qt] += e[rr];
+                    }
+                    // P in the compute type: its rounding (half a step, relative) averages out over the keys
+                    pk[qt][x][0] = pack2<C>(e[0], e[1]);
+                    pk[qt][x][1] = pack2<C>(e[2], e[3]);
+                }
+            }
+            // ---- O^T += V^T . P^T  (A operand rows d = 16 dt + lr by the transposing LDS read)
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+            {
+                const uint2 a2 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_cs16x4_t*) (uintptr_t) (va ^ (32 * dt))));
+                if constexpr (X2 == 2)
+                {
+                    const uint2 b2 = __builtin_bit_cast(uint2,
+                        __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_cs16x4_t*) (uintptr_t) ((va ^ (32 * dt)) + 16 * ROWB)));
+#pragma unroll
+                    for (int qt = 0; qt < QT; ++qt)
+                        o[qt][dt] = ctx_mfma<C>(make_uint4(a2.x, a2.y, b2.x, b2.y),
+                            make_uint4(pk[qt][0][0], pk[qt][0][1], pk[qt][X2 - 1][0], pk[qt][X2 - 1][1]), o[qt][dt]);
+                }
+                else
+                {
+#pragma unroll
+                    for (int qt = 0; qt < QT; ++qt)
+                        o[qt][dt] = tree_mfma16<C>(a2, make_uint2(pk[qt][0][0], pk[qt][0][1]), o[qt][dt]);
+                }
+            }
+        };
+        // V rows of a tile with nodes, in the LDS: rows past the sequence are zeroed (whatever lies there, 0 * NaN is NaN), and so
+        // are nodes' elements that are not finite, which must not reach the columns that do not see them; the others get them
+        // at the end.  History rows are seen by every column and stay as they are.
+        auto clean_tail = [&](uint32_t stage, int t0)
+        {
+            for (int c = tid; c < TREE_KT * CH; c += TREE_THREADS)
+            {
+                const int row = c / CH, t = t0 + row;
+                uint4* at = reinterpret_cast<uint4*>(lds + stage + TILE_BYTES + 16 * c);
+                if (t >= total)
+                    *at = make_uint4(0, 0, 0, 0);
+                else if (KVT == 0 && t >= past)
+                {
+                    uint4 w = *at;
+                    uint32_t* x = reinterpret_cast<uint32_t*>(&w);
+                    if (tree_nonfinite2<T>(x[0]) || tree_nonfinite2<T>(x[1]) || tree_nonfinite2<T>(x[2]) || tree_nonfinite2<T>(x[3]))
+                    {
+                        constexpr uint32_t EXP = T16<T>::is_bf16 ? 0x7f80u : 0x7c00u;
+                        for (int e = 0; e < 4; ++e)
+                        {
+                            if ((x[e] & EXP) == EXP)
+                                x[e] &= 0xffff0000u;
+                            if (((x[e] >> 16) & EXP) == EXP)
+                                x[e] &= 0xffffu;
+                        }
+                        *at = w;
+                        atomicOr(&nonfinite[(t - past) >> 5], 1u << ((t - past) & 31));
+                    }
+                }
+            }
+            __syncthreads();
+        };
+
+        if constexpr (KVT != 0)
+            store_tile(0);
+        uint32_t stage = 0; // of the tile that is computed
+        int i = tile_lo;
+        auto enter_tile = [&]()
+        {
+            if constexpr (KVT == 0)
+            {
+                // my share of tile i has landed; up to NS - 2 later tiles stay in flight
+                if (NS > 2 && tile_hi - i > NS - 2)
+                    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 2) * 2 * DPW) : "memory");
+                else
+                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            }
+            __syncthreads(); // everyone's has, and everyone is done with tile i - 1
+            if (i + AHEAD < tile_hi)
+            {
+                load_tile(stage == 0 ? (NS - 1) * STAGE_BYTES : stage - STAGE_BYTES);
+                find_tile(min(i + AHEAD + 1, tile_hi - 1));
+            }
+        };
+        auto leave_tile = [&]()
+        {
+            stage = stage + STAGE_BYTES == NS * STAGE_BYTES ? 0 : stage + STAGE_BYTES;
+            ++i;
+            if constexpr (KVT != 0)
+            {
+                if (i < tile_hi)
+                    store_tile(stage);
+            }
+        };
+        // the first tile and the tiles with nodes go through the general step, the history's others through the short one
+        const int plain_end = min(tile_hi, past / TREE_KT);
+        while (i < tile_hi)
+        {
+            enter_tile();
+            const int t0 = i * TREE_KT;
+            if (t0 + TREE_KT > past)
+                clean_tail(stage, t0);
+#pragma unroll 1
+            for (int kb = 0; kb < 16 * XW; kb += 16 * X2)
+                step(std::true_type{}, stage, kb, t0);
+            leave_tile();
+            while (i < plain_end)
+            {
+                enter_tile();
+#pragma unroll 1
+                for (int kb = 0; kb < 16 * XW; kb += 16 * X2)
+                    step(std::false_type{}, stage, kb, 0);
+                leave_tile();
             }
         }
-        // ---- O^T += V^T . P^T  (A operand rows d = 16 dt + lr by the transposing LDS read)
-        const int ra = kb + 4 * lq + rq, rb = ra + 16;
+
+        float m_run[QT];
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
+        for (int qt = 0; qt < QT; ++qt)
+            m_run[qt] = fresh[qt] ? NEG_BIG : -minus_m[qt][0];
+        // ---- the sum over the 4 lanes of a column, then the key groups of a row group through the LDS
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt)
         {
-            const int ch = 2 * dt + (rp >> 1), sub = 8 * (rp & 1);
-            const cs16x4_t va
-                = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_cs16x4_t*) (vt + ROWB * ra + 16 * (ch ^ sw(ra)) + sub));
-            const uint2 a2 = __builtin_bit_cast(uint2, va);
-            if constexpr (X2 == 2)
+            l_run[qt] += __shfl_xor(l_run[qt], 16);
+            l_run[qt] += __shfl_xor(l_run[qt], 32);
+        }
+        if constexpr (KW > 1)
+        {
+            constexpr int STATE = QT * (DT + 1) * 64 * 16; // bytes of one wave's state: float4 per register group and lane
+            static_assert((KW - 1) * RW * STATE <= NS * STAGE_BYTES, "states do not fit the tile buffers");
+            __syncthreads(); // everyone is done with the tiles
+            if (kw > 0)
             {
-                const cs16x4_t vb
-                    = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_cs16x4_t*) (vt + ROWB * rb + 16 * (ch ^ sw(rb)) + sub));
-                const uint2 b2 = __builtin_bit_cast(uint2, vb);
+                cf32x4_t* st = reinterpret_cast<cf32x4_t*>(lds + ((kw - 1) * RW + rw) * STATE) + lane;
 #pragma unroll
                 for (int qt = 0; qt < QT; ++qt)
-                    o[qt][dt] = ctx_mfma<C>(make_uint4(a2.x, a2.y, b2.x, b2.y),
-                        make_uint4(pk[qt][0][0], pk[qt][0][1], pk[qt][X2 - 1][0], pk[qt][X2 - 1][1]), o[qt][dt]);
+                {
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt)
+                        st[(qt * (DT + 1) + dt) * 64] = o[qt][dt];
+                    st[(qt * (DT + 1) + DT) * 64] = cf32x4_t{m_run[qt], l_run[qt], 0.f, 0.f};
+                }
+            }
+            __syncthreads();
+            if (kw > 0)
+                continue;
+#pragma unroll
+            for (int k = 1; k < KW; ++k)
+            {
+                const cf32x4_t* st = reinterpret_cast<const cf32x4_t*>(lds + ((k - 1) * RW + rw) * STATE) + lane;
+#pragma unroll
+                for (int qt = 0; qt < QT; ++qt)
+                {
+                    const cf32x4_t ml = st[(qt * (DT + 1) + DT) * 64];
+                    const float mm = fmaxf(m_run[qt], ml[0]);
+                    const float c0 = __builtin_amdgcn_exp2f(m_run[qt] - mm), c1 = __builtin_amdgcn_exp2f(ml[0] - mm);
+                    m_run[qt] = mm;
+                    l_run[qt] = l_run[qt] * c0 + ml[1] * c1;
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt)
+                    {
+                        const cf32x4_t x = st[(qt * (DT + 1) + dt) * 64];
+#pragma unroll
+                        for (int rr = 0; rr < 4; ++rr)
+                            o[qt][dt][rr] = o[qt][dt][rr] * c0 + x[rr] * c1;
+                    }
+                }
+            }
+        }
+        if constexpr (KVT == 0)
+        {
+            const int words = (n + 31) >> 5;
+            bool any = false;
+            for (int w = 0; w < words; ++w)
+                any |= nonfinite[w] != 0;
+            if (any) // uniform, and rare
+            {
+                for (int j = 0; j < n; ++j)
+                {
+                    if (!((nonfinite[j >> 5] >> (j & 31)) & 1))
+                        continue;
+                    const int t = past + j;
+                    const size_t at = ((size_t) head_kv << p.tpb_log2) + (t & tpb_mask);
+                    const uint16_t* v = reinterpret_cast<const uint16_t*>(vp[t >> p.tpb_log2]) + at * hs;
+#pragma unroll
+                    for (int qt = 0; qt < QT; ++qt)
+                    {
+                        const int node = min(q0 + 16 * qt + lr, n * G - 1) / G;
+                        const bool sees = (p.tree_mask[(size_t) (off + node) * p.mask_words + (j >> 5)] >> (j & 31)) & 1;
+#pragma unroll
+                        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                            for (int rr = 0; rr < 4; ++rr)
+                            {
+                                const int d = 16 * dt + 4 * lq + rr;
+                                const uint32_t w = v[min(d, hs - 1)];
+                                o[qt][dt][rr] += sees && d < hs && tree_nonfinite2<T>(w) ? T16<T>::to_float(w) : 0.f;
+                            }
+                    }
+                }
+            }
+        }
+        const bool alone = tile_lo == 0 && tile_hi == nt; // nothing of this (sequence, kv head) is elsewhere
+        const float v_deq = KVT ? p.kv_scale_quant_orig[0] : 1.f;
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt)
+        {
+            const int in_tile = rw * QT * 16 + 16 * qt + lr, r = mt * M + in_tile;
+            if (r >= n * G)
+                continue;
+            if (alone)
+            {
+                // no visible key: the sum is exactly 0, and so is the row (a NaN sum stays a NaN)
+                const float inv = l_run[qt] == 0.f ? 0.f : v_deq / l_run[qt];
+                uint16_t* out = p.out + ((size_t) (off + r / G) * p.num_heads + head_kv * G + r % G) * hs;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+                    if (16 * dt + 4 * lq < hs)
+                        *reinterpret_cast<uint2*>(out + 16 * dt + 4 * lq) = make_uint2(
+                            pack2<T>(o[qt][dt][0] * inv, o[qt][dt][1] * inv), pack2<T>(o[qt][dt][2] * inv, o[qt][dt][3] * inv));
             }
             else
             {
-#pragma unroll
-                for (int qt = 0; qt < QT; ++qt)
-                    o[qt][dt] = tree_mfma16<C>(a2, make_uint2(pk[qt][0][0], pk[qt][0][1]), o[qt][dt]);
-            }
-        }
-        if constexpr (KVT == 0)
-        {
-            // V rows of nodes with an infinity or NaN were zeroed for the products above (0 * inf would reach the columns
-            // that do not see them); the columns that do get those elements here
-            const uint64_t bad = tail ? ((uint64_t) nonfinite[1] << 32 | nonfinite[0]) : 0ull;
-            for (uint64_t left = bad; left; left &= left - 1)
-            {
-                const int k = __builtin_ctzll(left), t = t0 + k;
-                if (k < kb || k >= kb + 16 * X2)
-                    continue;
-                const size_t at = ((size_t) hk << p.tpb_log2) + (t & tpb_mask);
-                const uint16_t* v = reinterpret_cast<const uint16_t*>(vp[t >> p.tpb_log2]) + at * hs;
-#pragma unroll
-                for (int qt = 0; qt < QT; ++qt)
-                {
-                    const uint32_t* mrow = p.tree_mask + (size_t) (off + node[qt]) * p.mask_words;
-                    const bool sees = t < past || (((t - past) >> 5) < p.mask_words && (mrow[(t - past) >> 5] >> ((t - past) & 31)) & 1);
-#pragma unroll
-                    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                        for (int rr = 0; rr < 4; ++rr)
-                        {
-                            const int d = 16 * dt + 4 * lq + rr;
-                            if (sees && d < hs)
-                            {
-                                const uint32_t w = v[d];
-                                if (tree_nonfinite2<T>(w))
-                                    o[qt][dt][rr] += T16<T>::to_float(w);
-                            }
-                        }
-                }
-            }
-        }
-    };
-    // V rows of a tile with nodes, in the LDS: rows past the sequence are zeroed (whatever lies there, 0 * NaN is NaN), nodes'
-    // elements that are not finite are noted and zeroed.  History rows are seen by every column and stay as they are.
-    auto clean_tail = [&](int buf, int t0)
-    {
-        if (tid < 2)
-            nonfinite[tid] = 0;
-        __syncthreads();
-        uint8_t* vt = lds + buf * STAGE_BYTES + TILE_BYTES;
-        for (int c = tid; c < TREE_KT * CH; c += TREE_THREADS)
-        {
-            const int row = c / CH, t = t0 + row;
-            uint4* at = reinterpret_cast<uint4*>(vt + 16 * c);
-            if (t >= total)
-                *at = make_uint4(0, 0, 0, 0);
-            else if (KVT == 0 && t >= past)
-            {
-                uint4 w = *at;
-                uint32_t* x = reinterpret_cast<uint32_t*>(&w);
-                if (tree_nonfinite2<T>(x[0]) || tree_nonfinite2<T>(x[1]) || tree_nonfinite2<T>(x[2]) || tree_nonfinite2<T>(x[3]))
-                {
-                    constexpr uint32_t EXP = T16<T>::is_bf16 ? 0x7f80u : 0x7c00u;
-                    for (int e = 0; e < 4; ++e)
-                    {
-                        if ((x[e] & EXP) == EXP)
-                            x[e] &= 0xffff0000u;
-                        if (((x[e] >> 16) & EXP) == EXP)
-                            x[e] &= 0xffffu;
-                    }
-                    *at = w;
-                    atomicOr(&nonfinite[row >> 5], 1u << (row & 31));
-                }
-            }
-        }
-        __syncthreads();
-    };
-
-    if constexpr (KVT != 0)
-        store_tile(tile_lo & 1);
-    for (int i = tile_lo; i < tile_hi; ++i)
-    {
-        if constexpr (KVT == 0)
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // my share of tile i has landed
-        __syncthreads();                                     // everyone's has, and everyone is done with tile i - 1
-        if (i + 1 < tile_hi)
-        {
-            load_tile(i + 1, (i + 1) & 1);
-            find_tile(min(i + 2, tile_hi - 1));
-        }
-        const int t0 = i * TREE_KT;
-        const bool tail = t0 + TREE_KT > past; // uniform
-        if (tail)
-            clean_tail(i & 1, t0);
-#pragma unroll 1
-        for (int x = 0; x < XW; x += X2)
-            compute(i & 1, t0, kb0 + 16 * x, tail);
-        if constexpr (KVT != 0)
-        {
-            if (i + 1 < tile_hi)
-                store_tile((i + 1) & 1);
-        }
-    }
-
-    float m_run[QT];
-#pragma unroll
-    for (int qt = 0; qt < QT; ++qt)
-        m_run[qt] = fresh[qt] ? NEG_BIG : -minus_m[qt][0];
-    // ---- the sum over the 4 lanes of a column, then the key groups of a row group through the LDS
-#pragma unroll
-    for (int qt = 0; qt < QT; ++qt)
-    {
-        l_run[qt] += __shfl_xor(l_run[qt], 16);
-        l_run[qt] += __shfl_xor(l_run[qt], 32);
-    }
-    if constexpr (KW > 1)
-    {
-        constexpr int STATE = QT * (DT + 1) * 64 * 16; // bytes of one wave's state: float4 per register group and lane
-        static_assert((KW - 1) * RW * STATE <= 2 * STAGE_BYTES, "states do not fit the tile buffers");
-        __syncthreads(); // everyone is done with the tiles
-        if (kw > 0)
-        {
-            cf32x4_t* st = reinterpret_cast<cf32x4_t*>(lds + ((kw - 1) * RW + rw) * STATE) + lane;
-#pragma unroll
-            for (int qt = 0; qt < QT; ++qt)
-            {
+                const size_t rec = ((size_t) (2 * team + (tile_lo == 0)) * p.mtiles + mt) * M + in_tile;
+                float* acc = p.part_acc + rec * DP;
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt)
-                    st[(qt * (DT + 1) + dt) * 64] = o[qt][dt];
-                st[(qt * (DT + 1) + DT) * 64] = cf32x4_t{m_run[qt], l_run[qt], 0.f, 0.f};
+                    *reinterpret_cast<cf32x4_t*>(acc + 16 * dt + 4 * lq) = o[qt][dt];
+                if (lq == 0)
+                    p.part_ml[rec] = make_float2(m_run[qt], l_run[qt]);
             }
-        }
-        __syncthreads();
-        if (kw > 0)
-            return;
-#pragma unroll
-        for (int k = 1; k < KW; ++k)
-        {
-            const cf32x4_t* st = reinterpret_cast<const cf32x4_t*>(lds + ((k - 1) * RW + rw) * STATE) + lane;
-#pragma unroll
-            for (int qt = 0; qt < QT; ++qt)
-            {
-                const cf32x4_t ml = st[(qt * (DT + 1) + DT) * 64];
-                const float mm = fmaxf(m_run[qt], ml[0]);
-                const float c0 = __builtin_amdgcn_exp2f(m_run[qt] - mm), c1 = __builtin_amdgcn_exp2f(ml[0] - mm);
-                m_run[qt] = mm;
-                l_run[qt] = l_run[qt] * c0 + ml[1] * c1;
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
-                {
-                    const cf32x4_t x = st[(qt * (DT + 1) + dt) * 64];
-#pragma unroll
-                    for (int rr = 0; rr < 4; ++rr)
-                        o[qt][dt][rr] = o[qt][dt][rr] * c0 + x[rr] * c1;
-                }
-            }
-        }
-    }
-    const float v_deq = KVT ? p.kv_scale_quant_orig[0] : 1.f;
-#pragma unroll
-    for (int qt = 0; qt < QT; ++qt)
-    {
-        const int r = q0 + 16 * qt + lr;
-        if (r >= n * G)
-            continue;
-        const size_t head = (size_t) (off + r / G) * p.num_heads + hk * G + r % G;
-        if (alone)
-        {
-            // no visible key: the sum is exactly 0, and so is the row (a NaN sum stays a NaN)
-            const float inv = l_run[qt] == 0.f ? 0.f : v_deq / l_run[qt];
-            uint16_t* out = p.out + head * hs;
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
-                if (16 * dt + 4 * lq < hs)
-                    *reinterpret_cast<uint2*>(out + 16 * dt + 4 * lq) = make_uint2(
-                        pack2<T>(o[qt][dt][0] * inv, o[qt][dt][1] * inv), pack2<T>(o[qt][dt][2] * inv, o[qt][dt][3] * inv));
-        }
-        else
-        {
-            const size_t rec = (size_t) split * p.num_tokens * p.num_heads + head;
-            float* acc = p.part_acc + rec * DP;
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
-                *reinterpret_cast<cf32x4_t*>(acc + 16 * dt + 4 * lq) = o[qt][dt];
-            if (lq == 0)
-                p.part_ml[rec] = make_float2(m_run[qt], l_run[qt]);
         }
     }
 }
 
 // ---------------------------------------------------------------------------------------------- 3. combine
-// grid (max_draft, batch, ceil(heads / 4)): a wave joins one (token, head).  Splits are summed in their order, 8 loads in
-// flight.
+// grid (max_draft, batch, ceil(heads / 4)): a wave joins one (token, head), if its keys lay in more than one stretch.  The
+// parts are summed in the keys' order, 8 loads in flight.
 template <typename T, int DP>
 __global__ __launch_bounds__(TREE_THREADS) void tree_combine_kernel(TreeArgs p, bool quantised)
 {
     const int b = blockIdx.y, i = blockIdx.x, lane = threadIdx.x & 63;
     const int h = blockIdx.z * (TREE_THREADS / 64) + (threadIdx.x >> 6);
-    const int n = p.seq_nodes[b];
-    if (i >= n || h >= p.num_heads)
+    if (i >= p.seq_nodes[b] || h >= p.num_heads)
         return;
-    const int ntiles = (p.past_lengths[b] + n + TREE_KT - 1) / TREE_KT;
-    const int S = (ntiles + p.chunk_tiles - 1) / p.chunk_tiles; // <= 64
+    const int chunk = tree_chunk(p, p.tile_start[p.batch] * p.num_kv_heads);
+    const int nt = p.tile_start[b + 1] - p.tile_start[b];
+    const int u0 = p.tile_start[b] * p.num_kv_heads + h / p.group * nt;
+    const int team0 = u0 / chunk, S = (u0 + nt - 1) / chunk - team0 + 1;
     if (S <= 1)
         return;
-    const size_t head = (size_t) (p.draft_offsets[b] + i) * p.num_heads + h, stride = (size_t) p.num_tokens * p.num_heads;
+    const int M = p.rows_per_wg, r = i * p.group + h % p.group;
+    // record of part s: the last stretch of the first team, the first stretch of the others
+    auto record = [&](int s) { return ((size_t) (2 * (team0 + s) + (s == 0)) * p.mtiles + r / M) * M + r % M; };
     constexpr int E = DP / 64, U = 8;
-    const float2 ml = p.part_ml[min(lane, S - 1) * stride + head];
-    const float m = lane < S ? ml.x : NEG_BIG;
-    float mm = m;
+    float mm = NEG_BIG, l = 0.f;
+    for (int s = lane; s < S; s += 64)
+        mm = fmaxf(mm, p.part_ml[record(s)].x);
 #pragma unroll
     for (int x = 32; x >= 1; x >>= 1)
         mm = fmaxf(mm, __shfl_xor(mm, x));
-    const float c = lane < S ? __builtin_amdgcn_exp2f(m - mm) : 0.f;
-    float l = lane < S ? ml.y * c : 0.f;
-#pragma unroll
-    for (int x = 32; x >= 1; x >>= 1)
-        l += __shfl_xor(l, x);
     float acc[E] = {};
-    const float* src = p.part_acc + head * DP + E * lane;
     for (int s0 = 0; s0 < S; s0 += U)
     {
         float v[U][E];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-                v[u][e] = src[min(s0 + u, S - 1) * stride * DP + e];
+        float2 ml[U];
 #pragma unroll
         for (int u = 0; u < U; ++u)
         {
-            const float cs = s0 + u < S ? __shfl(c, min(s0 + u, 63)) : 0.f;
+            const size_t rec = record(min(s0 + u, S - 1));
+            ml[u] = p.part_ml[rec];
 #pragma unroll
             for (int e = 0; e < E; ++e)
-                acc[e] = s0 + u < S ? acc[e] + v[u][e] * cs : acc[e];
+                v[u][e] = p.part_acc[rec * DP + E * lane + e];
         }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (s0 + u < S)
+            {
+                const float c = __builtin_amdgcn_exp2f(ml[u].x - mm);
+                l += ml[u].y * c;
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    acc[e] += v[u][e] * c;
+            }
     }
     const float inv = l == 0.f ? 0.f : (quantised ? p.kv_scale_quant_orig[0] : 1.f) / l;
+    const size_t head = (size_t) (p.draft_offsets[b] + i) * p.num_heads + h;
 #pragma unroll
     for (int e = 0; e < E; ++e)
         if (E * lane + e < p.hs)
@@ -901,12 +1019,12 @@ __global__ __launch_bounds__(TREE_THREADS) void tree_combine_kernel(TreeArgs p, 
 // ---------------------------------------------------------------------------------------------- host
 struct TreePlan
 {
-    int dp, rows, rows_per_wg; // padded head size; query rows of a kv head at most; rows per workgroup
-    int mtiles, max_tiles, chunk_tiles, splits;
-    size_t q_bytes, seq_bytes, acc_bytes, ml_bytes;
+    int dp, rows_per_wg, mtiles, stages; // padded head size; query rows per workgroup; m-tiles of a (sequence, kv head); LDS ring
+    int teams, min_chunk, whole;
+    size_t q_bytes, seq_bytes, tile_bytes, acc_bytes, ml_bytes;
     size_t total() const
     {
-        return q_bytes + seq_bytes + acc_bytes + ml_bytes;
+        return q_bytes + seq_bytes + tile_bytes + acc_bytes + ml_bytes;
     }
 };
 size_t round256(size_t x)
@@ -927,6 +1045,8 @@ void tree_check(const mi355q_tree_attention_params& q)
     MQ_CHECK((int64_t) q.num_heads * q.max_draft_length <= (1 << 24), "num_heads %d x max_draft_length %d", q.num_heads, q.max_draft_length);
     MQ_CHECK(q.tokens_per_block > 0 && (q.tokens_per_block & (q.tokens_per_block - 1)) == 0 && q.tokens_per_block <= (1 << 20),
         "tokens_per_block must be a power of 2, got %d", q.tokens_per_block);
+    if (q.tokens_per_block < 16) // a wave's 16 keys of a tile come from one block
+        MQ_UNSUPPORTED("tree attention: tokens_per_block %d is not built (16 or more)", q.tokens_per_block);
     MQ_CHECK(q.max_blocks_per_seq > 0, "max_blocks_per_seq %d", q.max_blocks_per_seq);
     MQ_CHECK(q.max_past_length >= 0 && q.max_past_length <= (1 << 30), "max_past_length %d", q.max_past_length);
     MQ_CHECK(q.multi_block_mode >= 0, "multi_block_mode %d", q.multi_block_mode);
@@ -936,31 +1056,38 @@ TreePlan tree_plan(const mi355q_tree_attention_params& q)
 {
     TreePlan t{};
     t.dp = q.head_size <= 64 ? 64 : (q.head_size <= 128 ? 128 : 256);
-    const int group = q.num_heads / q.num_kv_heads;
-    t.rows = std::max(q.max_draft_length, 1) * group;
+    const int rows = std::max(q.max_draft_length, 1) * (q.num_heads / q.num_kv_heads);
     // few rows: the 4 waves of a workgroup share the keys of a tile instead of the rows
-    t.rows_per_wg = t.rows <= 16 ? 16 : (t.rows <= 32 ? 32 : (t.rows <= 64 || t.dp > 128 ? 64 : 128));
-    t.mtiles = (t.rows + t.rows_per_wg - 1) / t.rows_per_wg;
-    t.max_tiles = (q.max_past_length + q.max_draft_length + TREE_KT - 1) / TREE_KT;
-    t.max_tiles = std::max(t.max_tiles, 1);
-    // two workgroups live on a CU (one with heads beyond 128): split the keys until 256 CUs have that many, in
-    // stretches of at least 4 tiles (a stretch costs its prologue and a partial state)
-    const int64_t base = (int64_t) q.batch * q.num_kv_heads * t.mtiles;
-    const int64_t want = t.dp > 128 ? 256 : 512;
-    int splits = (int) std::min<int64_t>((want + base - 1) / std::max<int64_t>(base, 1), t.max_tiles / 4);
+    t.rows_per_wg = rows <= 16 ? 16 : (rows <= 32 ? 32 : (rows <= 64 || t.dp > 128 ? 64 : 128));
+    t.mtiles = (rows + t.rows_per_wg - 1) / t.rows_per_wg;
+    t.stages = 2;
+    const int max_tiles = std::max((q.max_past_length + q.max_draft_length + TREE_KT - 1) / TREE_KT, 1);
+    const int64_t groups = (int64_t) q.batch * q.num_kv_heads;
+    // two workgroups live on a CU (one with heads beyond 128): as many teams as fill 256 CUs, of at least 2 tiles each (a
+    // stretch costs its prologue and a partial state), and no (sequence, kv head) over more teams than the combine reads
+    const int64_t slots = t.dp > 128 ? 256 : 512;
+    int64_t teams = std::max<int64_t>(slots / t.mtiles, 1);
+    t.min_chunk = std::max(2, (max_tiles + TREE_MAX_SPLITS - 2) / (TREE_MAX_SPLITS - 1));
     if (q.multi_block_mode > 0)
-        splits = q.multi_block_mode;
-    splits = std::max(1, std::min(std::min(splits, t.max_tiles), TREE_MAX_SPLITS));
-    t.chunk_tiles = (t.max_tiles + splits - 1) / splits;
-    t.splits = (t.max_tiles + t.chunk_tiles - 1) / t.chunk_tiles;
-    const size_t heads = (size_t) q.num_tokens * q.num_heads;
-    const bool two_parts = q.kv_type == q.act_type || q.act_type == MI355Q_HALF; // TREE_Q2
-    t.q_bytes = round256(heads * t.dp * 2 * (two_parts ? 2 : 1));
-    t.seq_bytes = round256((size_t) q.batch * sizeof(int32_t));
-    if (t.splits > 1)
     {
-        t.acc_bytes = round256(t.splits * heads * t.dp * sizeof(float));
-        t.ml_bytes = round256(t.splits * heads * sizeof(float2));
+        // that many stretches to the longest history
+        t.min_chunk = std::max(1, (max_tiles + q.multi_block_mode - 1) / q.multi_block_mode);
+        t.min_chunk = std::max(t.min_chunk, (max_tiles + TREE_MAX_SPLITS - 2) / (TREE_MAX_SPLITS - 1));
+        teams = groups * ((max_tiles + t.min_chunk - 1) / t.min_chunk);
+    }
+    // short histories: one team per (sequence, kv head), nothing to join
+    t.whole = q.multi_block_mode == 1 || (q.multi_block_mode == 0 && max_tiles <= 4);
+    t.teams = (int) std::min<int64_t>(t.whole ? groups : std::min(teams, (groups * max_tiles + t.min_chunk - 1) / t.min_chunk), INT32_MAX / 16);
+    t.teams = std::max(t.teams, 1);
+    const bool two_parts = q.kv_type == q.act_type || q.act_type == MI355Q_HALF; // TREE_Q2
+    t.q_bytes = round256((size_t) q.num_tokens * q.num_heads * t.dp * 2 * (two_parts ? 2 : 1));
+    t.seq_bytes = round256((size_t) q.batch * sizeof(int32_t));
+    t.tile_bytes = round256((size_t) (q.batch + 1) * sizeof(int32_t));
+    if (!t.whole)
+    {
+        const size_t records = (size_t) 2 * t.teams * t.mtiles * t.rows_per_wg;
+        t.acc_bytes = round256(records * t.dp * sizeof(float));
+        t.ml_bytes = round256(records * sizeof(float2));
     }
     return t;
 }
@@ -968,19 +1095,19 @@ TreePlan tree_plan(const mi355q_tree_attention_params& q)
 template <typename T, int KVT, int DP>
 void tree_launch_attn(const TreeArgs& a, const TreePlan& t, hipStream_t stream)
 {
-    const int64_t grid = ((int64_t) a.groups + 7) / 8 * 8 * t.mtiles;
+    const int64_t grid = ((int64_t) t.teams + 7) / 8 * 8 * t.mtiles;
     MQ_CHECK(grid < (1ll << 31), "tree attention grid %lld", (long long) grid);
     const dim3 g((unsigned) grid), b(TREE_THREADS);
     // 32 rows a wave; 16 with heads beyond 128, whose accumulators take twice the registers
     constexpr int QT = DP > 128 ? 1 : 2;
     if (t.rows_per_wg == 16)
-        hipLaunchKernelGGL((tree_attn_kernel<T, KVT, DP, 1, 4, 1>), g, b, 0, stream, a);
+        hipLaunchKernelGGL((tree_attn_kernel<T, KVT, DP, 1, 4, 1, 2>), g, b, 0, stream, a);
     else if (t.rows_per_wg == 16 * QT)
-        hipLaunchKernelGGL((tree_attn_kernel<T, KVT, DP, 1, 4, QT>), g, b, 0, stream, a);
+        hipLaunchKernelGGL((tree_attn_kernel<T, KVT, DP, 1, 4, QT, 2>), g, b, 0, stream, a);
     else if (t.rows_per_wg == 32 * QT)
-        hipLaunchKernelGGL((tree_attn_kernel<T, KVT, DP, 2, 2, QT>), g, b, 0, stream, a);
+        hipLaunchKernelGGL((tree_attn_kernel<T, KVT, DP, 2, 2, QT, 2>), g, b, 0, stream, a);
     else
-        hipLaunchKernelGGL((tree_attn_kernel<T, KVT, DP, 4, 1, QT>), g, b, 0, stream, a);
+        hipLaunchKernelGGL((tree_attn_kernel<T, KVT, DP, 4, 1, QT, 2>), g, b, 0, stream, a);
     MQ_HIP(hipGetLastError());
 }
 
@@ -990,7 +1117,7 @@ void tree_launch(const mi355q_tree_attention_params& q, const TreeArgs& a, const
     // a token's heads over several workgroups, one 8-element chunk a thread, while the tokens alone do not fill the chip
     const int passes = ((q.num_heads + 2 * q.num_kv_heads) * t.dp / 8 + TREE_THREADS - 1) / TREE_THREADS;
     const int parts = std::max(1, (int) std::min<int64_t>(passes, 2048 / ((int64_t) q.batch * q.max_draft_length)));
-    hipLaunchKernelGGL((tree_prepare_kernel<T, KVT>), dim3(q.max_draft_length + 1, q.batch, parts), dim3(TREE_THREADS), 0, stream, a, t.dp);
+    hipLaunchKernelGGL((tree_prepare_kernel<T, KVT>), dim3(q.max_draft_length + 2, q.batch, parts), dim3(TREE_THREADS), 0, stream, a, t.dp);
     MQ_HIP(hipGetLastError());
     if (t.dp == 64)
         tree_launch_attn<T, KVT, 64>(a, t, stream);
@@ -998,7 +1125,7 @@ void tree_launch(const mi355q_tree_attention_params& q, const TreeArgs& a, const
         tree_launch_attn<T, KVT, 128>(a, t, stream);
     else
         tree_launch_attn<T, KVT, 256>(a, t, stream);
-    if (t.splits > 1)
+    if (!t.whole)
     {
         const dim3 g(q.max_draft_length, q.batch, (q.num_heads + 3) / 4), b(TREE_THREADS);
         if (t.dp == 64)
@@ -1082,8 +1209,9 @@ void tree_attention(const mi355q_tree_attention_params& q, hipStream_t stream)
     char* ws = static_cast<char*>(q.workspace);
     a.q_ws = reinterpret_cast<uint16_t*>(ws);
     a.seq_nodes = reinterpret_cast<int32_t*>(ws + t.q_bytes);
-    a.part_acc = reinterpret_cast<float*>(ws + t.q_bytes + t.seq_bytes);
-    a.part_ml = reinterpret_cast<float2*>(ws + t.q_bytes + t.seq_bytes + t.acc_bytes);
+    a.tile_start = reinterpret_cast<int32_t*>(ws + t.q_bytes + t.seq_bytes);
+    a.part_acc = reinterpret_cast<float*>(ws + t.q_bytes + t.seq_bytes + t.tile_bytes);
+    a.part_ml = reinterpret_cast<float2*>(ws + t.q_bytes + t.seq_bytes + t.tile_bytes + t.acc_bytes);
     a.qkv_stride = q.qkv_stride ? q.qkv_stride : (int64_t) hidden;
     a.batch = q.batch;
     a.num_heads = q.num_heads;
@@ -1098,11 +1226,12 @@ void tree_attention(const mi355q_tree_attention_params& q, hipStream_t stream)
     while ((1 << a.tpb_log2) < q.tokens_per_block)
         ++a.tpb_log2;
     a.mtiles = t.mtiles;
-    a.chunk_tiles = t.chunk_tiles;
-    a.splits = t.splits;
-    const int64_t groups = (int64_t) q.batch * q.num_kv_heads * t.splits;
-    MQ_CHECK(groups < (1 << 28), "tree attention: %lld (sequence, kv head, split) groups", (long long) groups);
-    a.groups = (int) groups;
+    a.rows_per_wg = t.rows_per_wg;
+    a.teams = t.teams;
+    a.min_chunk = t.min_chunk;
+    a.whole = t.whole;
+    MQ_CHECK((int64_t) q.batch * q.num_kv_heads * ((q.max_past_length + q.max_draft_length + TREE_KT - 1) / TREE_KT) < (1 << 30),
+        "tree attention: %d sequences x %d kv heads x %d keys", q.batch, q.num_kv_heads, q.max_past_length);
     a.pos_type = q.position_embedding_type;
     a.rot_dim = q.rotary_embedding_dim;
     a.rot_scale_type = q.rotary_embedding_scale_type;

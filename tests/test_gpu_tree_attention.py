@@ -83,7 +83,7 @@ def test_lengths(cuda, past, n, kv):
     check(TreeCase([past, 17], trees([n, 3], n), 2, 2, 64, BF, kv, tpb=32, rope=1, seed=past + n), cuda)
 
 
-@pytest.mark.parametrize("tpb", [1, 4, 16, 64, 128, 1024])
+@pytest.mark.parametrize("tpb", [16, 32, 64, 128, 1024])
 @pytest.mark.parametrize("kv", [HF, I8])
 def test_block_sizes(cuda, tpb, kv):
     check(TreeCase([150, 3], trees([20, 5]), 4, 2, 64, HF, kv, tpb=tpb, kv_scale=1 / 32 if kv == I8 else 1.0), cuda)
