@@ -60,8 +60,8 @@ struct TreeArgs
     const float* kv_scale_orig_quant;
     const float* kv_scale_quant_orig;
     uint16_t* q_ws;      // [tokens][Hq][1 or 2 parts][DP]: rotated, times the score scale (and the K dequantisation) and log2(e)
-    int32_t* seq_nodes;  // [batch]: nodes of the sequence, 0 if it is skipped
-    int32_t* tile_start; // [batch + 1]: key tiles of the sequences before this one
+    int4* seq;           // [batch + 1]: key tiles of the sequences before this one, nodes, first row, history; [batch].x: all tiles
+    int32_t* seq_ok;     // [batch]: the sequence's blocks are all there
     float* part_acc;     // partial states: [team][first | last stretch][m-tile][row][DP]
     float2* part_ml;     // their (running maximum in the log2 domain, sum)
     int64_t qkv_stride;
@@ -116,11 +116,11 @@ __device__ __forceinline__ void tree_count_tiles(const TreeArgs& p)
             carry += wave_sum[w];
         }
         if (b < p.batch)
-            p.tile_start[b] = before + x - mine;
+            p.seq[b] = make_int4(before + x - mine, mine ? n : 0, off, past);
         __syncthreads();
     }
     if (threadIdx.x == 0)
-        p.tile_start[p.batch] = carry;
+        p.seq[p.batch] = make_int4(carry, 0, 0, 0);
 }
 
 // tiles of a team's stretch: all (sequence, kv head, tile) units in equal parts
@@ -161,7 +161,7 @@ __global__ __launch_bounds__(TREE_THREADS) void tree_prepare_kernel(TreeArgs p, 
                 bad |= kp[j] == 0 || kp[p.max_blocks + j] == 0;
         bad = __syncthreads_or(bad);
         if (threadIdx.x == 0)
-            p.seq_nodes[b] = bad ? 0 : n;
+            p.seq_ok[b] = !bad;
         return;
     }
     if (!ok || i >= n)
@@ -462,32 +462,46 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
         return CH >= 16 ? (row & 3) << 2 | ((x ^ x >> 1) & 1) << 1 | x >> 1 : ((row >> 1) & 3) << 1;
     };
 
-    // ---- the team's stretch of units (sequence, kv head, tile)
-    int b = 0, hk = 0, tile = 0, left; // left: tiles of the stretch still to do
+    // ---- the team's stretch of units (sequence, kv head, tile).  A lane holds the record of one of 64 sequences; the one at work
+    // is a lane read away
+    int b = 0, hk = 0, tile = 0, left, b0; // left: tiles of the stretch still to do; b0: the first sequence in the lanes
+    int4 info;
+    int info_next, info_ok;
+    auto fetch_info = [&](int first)
+    {
+        b0 = first;
+        info = p.seq[min(first + lane, p.batch)];
+        info_next = p.seq[min(first + lane + 1, p.batch)].x;
+        info_ok = p.seq_ok[min(first + lane, p.batch - 1)];
+    };
     if (p.whole)
     {
         b = team / p.num_kv_heads;
         hk = team % p.num_kv_heads;
-        left = p.tile_start[b + 1] - p.tile_start[b];
+        fetch_info(b & ~63);
+        left = INT32_MAX;
     }
     else
     {
-        const int units = p.tile_start[p.batch] * p.num_kv_heads;
+        fetch_info(0);
+        const int units = p.seq[p.batch].x * p.num_kv_heads;
         const int chunk = tree_chunk(p, units);
         const int64_t u0 = (int64_t) team * chunk;
         left = (int) min((int64_t) chunk, units - u0);
         if (left <= 0)
             return;
         const int at = (int) u0 / p.num_kv_heads; // the sequences that end at or before this tile
-        for (int b0 = 0; b0 < p.batch; b0 += 64)
+        for (;;)
         {
-            const uint64_t done = __ballot(b0 + lane < p.batch && p.tile_start[min(b0 + lane + 1, p.batch)] <= at);
-            b += __builtin_popcountll(done);
+            const uint64_t done = __ballot(b0 + lane < p.batch && info_next <= at);
+            b = b0 + __builtin_popcountll(done);
             if (done != ~0ull)
                 break;
+            fetch_info(b0 + 64);
         }
         b = __builtin_amdgcn_readfirstlane(b);
-        const int nt = p.tile_start[b + 1] - p.tile_start[b], in_seq = (int) u0 - p.tile_start[b] * p.num_kv_heads;
+        const int start = __builtin_amdgcn_readlane(info.x, b - b0), nt = __builtin_amdgcn_readlane(info_next, b - b0) - start;
+        const int in_seq = (int) u0 - start * p.num_kv_heads;
         hk = in_seq / nt;
         tile = in_seq % nt;
     }
@@ -513,20 +527,24 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
 
     while (left > 0)
     {
-        const int nt = p.tile_start[b + 1] - p.tile_start[b];
-        const int tile_lo = tile, tile_hi = min(nt, tile + left);
-        const int seq = b, head_kv = hk;
+        if (b >= b0 + 64)
+            fetch_info(b);
+        const int at = b - b0, seq = b, head_kv = hk;
+        const int nt = __builtin_amdgcn_readlane(info_next, at) - __builtin_amdgcn_readlane(info.x, at);
+        const int tile_lo = tile, tile_hi = min(nt, left < INT32_MAX - nt ? tile + left : nt);
         left -= tile_hi - tile_lo;
         tile = 0;
-        if (++hk == p.num_kv_heads)
+        if (p.whole)
+            left = 0;
+        else if (++hk == p.num_kv_heads)
         {
             hk = 0;
             ++b;
         }
-        const int n = tile_hi > tile_lo ? p.seq_nodes[seq] : 0;
-        if (mt * M >= n * G) // an empty sequence, one that is skipped, or no rows for this m-tile
+        const int n = __builtin_amdgcn_readlane(info_ok, at) ? __builtin_amdgcn_readlane(info.y, at) : 0;
+        if (tile_hi <= tile_lo || mt * M >= n * G) // an empty sequence, one that is skipped, or no rows for this m-tile
             continue;
-        const int off = p.draft_offsets[seq], past = p.past_lengths[seq], total = past + n;
+        const int off = __builtin_amdgcn_readlane(info.z, at), past = __builtin_amdgcn_readlane(info.w, at), total = past + n;
         const int64_t* const kp = p.block_ptrs + (size_t) seq * 2 * p.max_blocks;
         const int64_t* const vp = kp + p.max_blocks;
 
@@ -595,10 +613,16 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
         // ---- Q^T fragments (B operand): column = row q0 + 16 qt + lr, k = d = 32 ks + 8 lq + j
         const int q0 = mt * M + rw * QT * 16;
         uint4 qf[PARTS][QT][KS];
+        uint64_t mask_row[QT]; // the first 64 nodes' bits
+        const bool long_tree = n > 64;
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt)
         {
             const int r = min(q0 + 16 * qt + lr, n * G - 1); // rows past the last re-read it; never stored
+            const uint32_t* mrow = p.tree_mask + (size_t) (off + r / G) * p.mask_words;
+            mask_row[qt] = (uint64_t) mrow[p.mask_words > 1 ? 1 : 0] << 32 | mrow[0];
+            if (n < 64)
+                mask_row[qt] &= (1ull << n) - 1;
             const uint16_t* q = p.q_ws + ((size_t) (off + r / G) * p.num_heads + head_kv * G + r % G) * PARTS * DP;
 #pragma unroll
             for (int part = 0; part < PARTS; ++part)
@@ -606,7 +630,10 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
                 for (int ks = 0; ks < KS; ++ks)
                     qf[part][qt][ks] = *reinterpret_cast<const uint4*>(q + part * DP + 32 * ks + 8 * lq);
         }
-        // end the compiler's own bookkeeping of the q loads here, before the loop's (to it invisible) DMAs
+        // end the compiler's own bookkeeping of these loads here, before the loop's (to it invisible) DMAs
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt)
+            asm volatile("" : "+v"(mask_row[qt]));
 #pragma unroll
         for (int part = 0; part < PARTS; ++part)
 #pragma unroll
@@ -661,9 +688,16 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
 #pragma unroll
                 for (int qt = 0; qt < QT; ++qt)
                 {
-                    const int node = min(q0 + 16 * qt + lr, n * G - 1) / G;
-                    const uint64_t seen = tree_mask64(p.tree_mask + (size_t) (off + node) * p.mask_words, p.mask_words, n, t0 - past)
-                        >> (kb0 + kb + 4 * lq);
+                    const int s0 = t0 - past; // > -64
+                    uint64_t seen;
+                    if (long_tree) // uniform
+                    {
+                        const int node = min(q0 + 16 * qt + lr, n * G - 1) / G;
+                        seen = tree_mask64(p.tree_mask + (size_t) (off + node) * p.mask_words, p.mask_words, n, s0);
+                    }
+                    else // the history's keys are seen
+                        seen = s0 < 0 ? mask_row[qt] << -s0 | ((1ull << -s0) - 1) : (s0 < 64 ? mask_row[qt] >> s0 : 0);
+                    seen >>= kb0 + kb + 4 * lq;
 #pragma unroll
                     for (int x = 0; x < X2; ++x)
 #pragma unroll
@@ -756,7 +790,7 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
         // at the end.  History rows are seen by every column and stay as they are.
         auto clean_tail = [&](uint32_t stage, int t0)
         {
-            for (int c = tid; c < TREE_KT * CH; c += TREE_THREADS)
+            for (int c = max(past - t0, 0) * CH + tid; c < TREE_KT * CH; c += TREE_THREADS)
             {
                 const int row = c / CH, t = t0 + row;
                 uint4* at = reinterpret_cast<uint4*>(lds + stage + TILE_BYTES + 16 * c);
@@ -965,11 +999,12 @@ __global__ __launch_bounds__(TREE_THREADS) void tree_combine_kernel(TreeArgs p, 
 {
     const int b = blockIdx.y, i = blockIdx.x, lane = threadIdx.x & 63;
     const int h = blockIdx.z * (TREE_THREADS / 64) + (threadIdx.x >> 6);
-    if (i >= p.seq_nodes[b] || h >= p.num_heads)
+    const int4 info = p.seq[b];
+    if (i >= info.y || h >= p.num_heads || !p.seq_ok[b])
         return;
-    const int chunk = tree_chunk(p, p.tile_start[p.batch] * p.num_kv_heads);
-    const int nt = p.tile_start[b + 1] - p.tile_start[b];
-    const int u0 = p.tile_start[b] * p.num_kv_heads + h / p.group * nt;
+    const int chunk = tree_chunk(p, p.seq[p.batch].x * p.num_kv_heads);
+    const int nt = p.seq[b + 1].x - info.x;
+    const int u0 = info.x * p.num_kv_heads + h / p.group * nt;
     const int team0 = u0 / chunk, S = (u0 + nt - 1) / chunk - team0 + 1;
     if (S <= 1)
         return;
@@ -1009,7 +1044,7 @@ __global__ __launch_bounds__(TREE_THREADS) void tree_combine_kernel(TreeArgs p, 
             }
     }
     const float inv = l == 0.f ? 0.f : (quantised ? p.kv_scale_quant_orig[0] : 1.f) / l;
-    const size_t head = (size_t) (p.draft_offsets[b] + i) * p.num_heads + h;
+    const size_t head = (size_t) (info.z + i) * p.num_heads + h;
 #pragma unroll
     for (int e = 0; e < E; ++e)
         if (E * lane + e < p.hs)
@@ -1021,10 +1056,10 @@ struct TreePlan
 {
     int dp, rows_per_wg, mtiles, stages; // padded head size; query rows per workgroup; m-tiles of a (sequence, kv head); LDS ring
     int teams, min_chunk, whole;
-    size_t q_bytes, seq_bytes, tile_bytes, acc_bytes, ml_bytes;
+    size_t q_bytes, seq_bytes, ok_bytes, acc_bytes, ml_bytes;
     size_t total() const
     {
-        return q_bytes + seq_bytes + tile_bytes + acc_bytes + ml_bytes;
+        return q_bytes + seq_bytes + ok_bytes + acc_bytes + ml_bytes;
     }
 };
 size_t round256(size_t x)
@@ -1081,8 +1116,8 @@ TreePlan tree_plan(const mi355q_tree_attention_params& q)
     t.teams = std::max(t.teams, 1);
     const bool two_parts = q.kv_type == q.act_type || q.act_type == MI355Q_HALF; // TREE_Q2
     t.q_bytes = round256((size_t) q.num_tokens * q.num_heads * t.dp * 2 * (two_parts ? 2 : 1));
-    t.seq_bytes = round256((size_t) q.batch * sizeof(int32_t));
-    t.tile_bytes = round256((size_t) (q.batch + 1) * sizeof(int32_t));
+    t.seq_bytes = round256((size_t) (q.batch + 1) * sizeof(int4));
+    t.ok_bytes = round256((size_t) q.batch * sizeof(int32_t));
     if (!t.whole)
     {
         const size_t records = (size_t) 2 * t.teams * t.mtiles * t.rows_per_wg;
@@ -1208,10 +1243,10 @@ void tree_attention(const mi355q_tree_attention_params& q, hipStream_t stream)
     a.kv_scale_quant_orig = q.kv_scale_quant_orig;
     char* ws = static_cast<char*>(q.workspace);
     a.q_ws = reinterpret_cast<uint16_t*>(ws);
-    a.seq_nodes = reinterpret_cast<int32_t*>(ws + t.q_bytes);
-    a.tile_start = reinterpret_cast<int32_t*>(ws + t.q_bytes + t.seq_bytes);
-    a.part_acc = reinterpret_cast<float*>(ws + t.q_bytes + t.seq_bytes + t.tile_bytes);
-    a.part_ml = reinterpret_cast<float2*>(ws + t.q_bytes + t.seq_bytes + t.tile_bytes + t.acc_bytes);
+    a.seq = reinterpret_cast<int4*>(ws + t.q_bytes);
+    a.seq_ok = reinterpret_cast<int32_t*>(ws + t.q_bytes + t.seq_bytes);
+    a.part_acc = reinterpret_cast<float*>(ws + t.q_bytes + t.seq_bytes + t.ok_bytes);
+    a.part_ml = reinterpret_cast<float2*>(ws + t.q_bytes + t.seq_bytes + t.ok_bytes + t.acc_bytes);
     a.qkv_stride = q.qkv_stride ? q.qkv_stride : (int64_t) hidden;
     a.batch = q.batch;
     a.num_heads = q.num_heads;
