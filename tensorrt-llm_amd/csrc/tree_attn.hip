@@ -436,6 +436,9 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
     constexpr int TILE_BYTES = TREE_KT * ROWB, STAGE_BYTES = 2 * TILE_BYTES;
     constexpr int XW = 4 / KW;                      // 16-key subtiles per wave
     constexpr int X2 = XW < 2 ? XW : 2;             // subtiles per compute step: 32 keys, or 16 with four key groups
+    // fragments read from the LDS ahead of their products, as many as the registers hold
+    constexpr bool TIGHT = PARTS == 2 && QT == 2 && DP >= 128;
+    constexpr int KBATCH = TIGHT && X2 == 2 ? 2 : KS, VBATCH = TIGHT && X2 == 2 ? 4 : (DT < 8 ? DT : 8);
     constexpr int WROWS = TREE_KT / 4;              // a wave loads 16 consecutive keys of a tile
     constexpr int RPD = 1024 / ROWB, DPW = WROWS / RPD; // 16-bit caches: rows per DMA instruction, DMAs per wave
     constexpr int CH8 = DP / 16, RPL = 64 / CH8, LPT = WROWS / RPL; // 8-bit caches: rows per 16-byte load, loads per thread
@@ -669,20 +672,37 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
                 for (int qt = 0; qt < QT; ++qt)
                     s[x][qt] = minus_m[qt];
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) // consecutive products go to different accumulators
+            for (int ks0 = 0; ks0 < KS; ks0 += KBATCH)
             {
-                uint4 kf[X2];
+                uint4 kf[KBATCH][X2];
 #pragma unroll
-                for (int x = 0; x < X2; ++x)
-                    kf[x] = tree_lds16((ka ^ (64 * ks)) + 16 * x * ROWB);
-#pragma unroll
-                for (int part = PARTS - 1; part >= 0; --part)
+                for (int ks = 0; ks < KBATCH; ++ks)
 #pragma unroll
                     for (int x = 0; x < X2; ++x)
+                        kf[ks][x] = tree_lds16((ka ^ (64 * (ks0 + ks))) + 16 * x * ROWB);
 #pragma unroll
-                        for (int qt = 0; qt < QT; ++qt)
-                            s[x][qt] = ctx_mfma<C>(kf[x], qf[part][qt][ks], s[x][qt]);
+                for (int ks = 0; ks < KBATCH; ++ks)
+#pragma unroll
+                    for (int part = PARTS - 1; part >= 0; --part)
+#pragma unroll
+                        for (int x = 0; x < X2; ++x) // consecutive products go to different accumulators
+#pragma unroll
+                            for (int qt = 0; qt < QT; ++qt)
+                                s[x][qt] = ctx_mfma<C>(kf[ks][x], qf[part][qt][ks0 + ks], s[x][qt]);
             }
+            // the first V fragments are read while the softmax runs
+            uint2 vf[VBATCH][X2];
+            auto read_v = [&](int d0)
+            {
+#pragma unroll
+                for (int dt = 0; dt < VBATCH; ++dt)
+#pragma unroll
+                    for (int x = 0; x < X2; ++x)
+                        vf[dt][x] = __builtin_bit_cast(uint2,
+                            __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_cs16x4_t*) (uintptr_t) ((va ^ (32 * (d0 + dt))) + 16 * x * ROWB)));
+            };
+            read_v(0);
+            __builtin_amdgcn_sched_barrier(0);
             if (GENERAL && t0 + TREE_KT > past)
             {
 #pragma unroll
@@ -765,24 +785,21 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
             }
             // ---- O^T += V^T . P^T  (A operand rows d = 16 dt + lr by the transposing LDS read)
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
+            for (int d0 = 0; d0 < DT; d0 += VBATCH)
             {
-                const uint2 a2 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_cs16x4_t*) (uintptr_t) (va ^ (32 * dt))));
-                if constexpr (X2 == 2)
-                {
-                    const uint2 b2 = __builtin_bit_cast(uint2,
-                        __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_cs16x4_t*) (uintptr_t) ((va ^ (32 * dt)) + 16 * ROWB)));
+                if (d0)
+                    read_v(d0);
+#pragma unroll
+                for (int dt = 0; dt < VBATCH; ++dt)
 #pragma unroll
                     for (int qt = 0; qt < QT; ++qt)
-                        o[qt][dt] = ctx_mfma<C>(make_uint4(a2.x, a2.y, b2.x, b2.y),
-                            make_uint4(pk[qt][0][0], pk[qt][0][1], pk[qt][X2 - 1][0], pk[qt][X2 - 1][1]), o[qt][dt]);
-                }
-                else
-                {
-#pragma unroll
-                    for (int qt = 0; qt < QT; ++qt)
-                        o[qt][dt] = tree_mfma16<C>(a2, make_uint2(pk[qt][0][0], pk[qt][0][1]), o[qt][dt]);
-                }
+                    {
+                        if constexpr (X2 == 2)
+                            o[qt][d0 + dt] = ctx_mfma<C>(make_uint4(vf[dt][0].x, vf[dt][0].y, vf[dt][X2 - 1].x, vf[dt][X2 - 1].y),
+                                make_uint4(pk[qt][0][0], pk[qt][0][1], pk[qt][X2 - 1][0], pk[qt][X2 - 1][1]), o[qt][d0 + dt]);
+                        else
+                            o[qt][d0 + dt] = tree_mfma16<C>(vf[dt][0], make_uint2(pk[qt][0][0], pk[qt][0][1]), o[qt][d0 + dt]);
+                    }
             }
         };
         // V rows of a tile with nodes, in the LDS: rows past the sequence are zeroed (whatever lies there, 0 * NaN is NaN), and so
@@ -850,7 +867,8 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
             }
         };
         // the first tile and the tiles with nodes go through the general step, the history's others through the short one
-        const int plain_end = min(tile_hi, past / TREE_KT);
+        // (with few rows one copy of the step: fetching code costs more there than a mask test)
+        const int plain_end = KW == 1 ? min(tile_hi, past / TREE_KT) : 0;
         while (i < tile_hi)
         {
             enter_tile();
@@ -861,77 +879,86 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
             for (int kb = 0; kb < 16 * XW; kb += 16 * X2)
                 step(std::true_type{}, stage, kb, t0);
             leave_tile();
-            while (i < plain_end)
-            {
-                enter_tile();
+            if constexpr (KW == 1)
+                while (i < plain_end)
+                {
+                    enter_tile();
 #pragma unroll 1
-                for (int kb = 0; kb < 16 * XW; kb += 16 * X2)
-                    step(std::false_type{}, stage, kb, 0);
-                leave_tile();
-            }
+                    for (int kb = 0; kb < 16 * XW; kb += 16 * X2)
+                        step(std::false_type{}, stage, kb, 0);
+                    leave_tile();
+                }
         }
 
-        float m_run[QT];
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt)
-            m_run[qt] = fresh[qt] ? NEG_BIG : -minus_m[qt][0];
-        // ---- the sum over the 4 lanes of a column, then the key groups of a row group through the LDS
+        // ---- the end of the stretch: the sum over the 4 lanes of a column; the states of the KW key groups meet in the LDS, and
+        // each of their waves joins and stores its share of the output columns
+        constexpr int DTW = DT / KW;
+        const int dt0 = kw * DTW;
+        bool any_nonfinite = false;
+        if constexpr (KVT == 0)
+            for (int w = 0; w < (n + 31) >> 5; ++w)
+                any_nonfinite |= nonfinite[w] != 0;
+        const bool alone = tile_lo == 0 && tile_hi == nt; // nothing of this (sequence, kv head) is elsewhere
+        const float v_deq = KVT ? p.kv_scale_quant_orig[0] : 1.f;
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt)
         {
-            l_run[qt] += __shfl_xor(l_run[qt], 16);
-            l_run[qt] += __shfl_xor(l_run[qt], 32);
-        }
-        if constexpr (KW > 1)
-        {
-            constexpr int STATE = QT * (DT + 1) * 64 * 16; // bytes of one wave's state: float4 per register group and lane
-            static_assert((KW - 1) * RW * STATE <= NS * STAGE_BYTES, "states do not fit the tile buffers");
-            __syncthreads(); // everyone is done with the tiles
-            if (kw > 0)
+            float m = fresh[qt] ? NEG_BIG : -minus_m[qt][0], l = l_run[qt];
+            l += __shfl_xor(l, 16);
+            l += __shfl_xor(l, 32);
+            cf32x4_t acc[DTW];
+            if constexpr (KW == 1)
             {
-                cf32x4_t* st = reinterpret_cast<cf32x4_t*>(lds + ((kw - 1) * RW + rw) * STATE) + lane;
 #pragma unroll
-                for (int qt = 0; qt < QT; ++qt)
-                {
-#pragma unroll
-                    for (int dt = 0; dt < DT; ++dt)
-                        st[(qt * (DT + 1) + dt) * 64] = o[qt][dt];
-                    st[(qt * (DT + 1) + DT) * 64] = cf32x4_t{m_run[qt], l_run[qt], 0.f, 0.f};
-                }
+                for (int dt = 0; dt < DT; ++dt)
+                    acc[dt] = o[qt][dt];
             }
-            __syncthreads();
-            if (kw > 0)
-                continue;
-#pragma unroll
-            for (int k = 1; k < KW; ++k)
+            else
             {
-                const cf32x4_t* st = reinterpret_cast<const cf32x4_t*>(lds + ((k - 1) * RW + rw) * STATE) + lane;
+                constexpr int STATE = (DT + 1) * 64 * 16; // bytes of one wave's state: float4 per register group and lane
+                static_assert(4 * STATE <= NS * STAGE_BYTES, "states do not fit the tile buffers");
+                __syncthreads(); // everyone is done with the tiles, or with the states before
+                cf32x4_t* st = reinterpret_cast<cf32x4_t*>(lds + wave * STATE) + lane;
 #pragma unroll
-                for (int qt = 0; qt < QT; ++qt)
+                for (int dt = 0; dt < DT; ++dt)
+                    st[dt * 64] = o[qt][dt];
+                st[DT * 64] = cf32x4_t{m, l, 0.f, 0.f};
+                __syncthreads();
+                float c[KW], mk[KW], lk[KW];
+#pragma unroll
+                for (int k = 0; k < KW; ++k)
                 {
-                    const cf32x4_t ml = st[(qt * (DT + 1) + DT) * 64];
-                    const float mm = fmaxf(m_run[qt], ml[0]);
-                    const float c0 = __builtin_amdgcn_exp2f(m_run[qt] - mm), c1 = __builtin_amdgcn_exp2f(ml[0] - mm);
-                    m_run[qt] = mm;
-                    l_run[qt] = l_run[qt] * c0 + ml[1] * c1;
+                    const cf32x4_t ml = reinterpret_cast<const cf32x4_t*>(lds + (k * RW + rw) * STATE)[DT * 64 + lane];
+                    mk[k] = ml[0];
+                    lk[k] = ml[1];
+                }
+                m = mk[0];
 #pragma unroll
-                    for (int dt = 0; dt < DT; ++dt)
+                for (int k = 1; k < KW; ++k)
+                    m = fmaxf(m, mk[k]);
+                l = 0.f;
+#pragma unroll
+                for (int k = 0; k < KW; ++k)
+                {
+                    c[k] = __builtin_amdgcn_exp2f(mk[k] - m);
+                    l += lk[k] * c[k];
+                }
+#pragma unroll
+                for (int dt = 0; dt < DTW; ++dt)
+                {
+                    acc[dt] = cf32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int k = 0; k < KW; ++k)
                     {
-                        const cf32x4_t x = st[(qt * (DT + 1) + dt) * 64];
+                        const cf32x4_t x = reinterpret_cast<const cf32x4_t*>(lds + (k * RW + rw) * STATE)[(dt0 + dt) * 64 + lane];
 #pragma unroll
                         for (int rr = 0; rr < 4; ++rr)
-                            o[qt][dt][rr] = o[qt][dt][rr] * c0 + x[rr] * c1;
+                            acc[dt][rr] += x[rr] * c[k];
                     }
                 }
             }
-        }
-        if constexpr (KVT == 0)
-        {
-            const int words = (n + 31) >> 5;
-            bool any = false;
-            for (int w = 0; w < words; ++w)
-                any |= nonfinite[w] != 0;
-            if (any) // uniform, and rare
+            const int in_tile = rw * QT * 16 + 16 * qt + lr, r = min(mt * M + in_tile, n * G - 1), node = r / G;
+            if (any_nonfinite) // uniform, and rare
             {
                 for (int j = 0; j < n; ++j)
                 {
@@ -940,52 +967,43 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
                     const int t = past + j;
                     const size_t at = ((size_t) head_kv << p.tpb_log2) + (t & tpb_mask);
                     const uint16_t* v = reinterpret_cast<const uint16_t*>(vp[t >> p.tpb_log2]) + at * hs;
+                    const bool sees = (p.tree_mask[(size_t) (off + node) * p.mask_words + (j >> 5)] >> (j & 31)) & 1;
 #pragma unroll
-                    for (int qt = 0; qt < QT; ++qt)
-                    {
-                        const int node = min(q0 + 16 * qt + lr, n * G - 1) / G;
-                        const bool sees = (p.tree_mask[(size_t) (off + node) * p.mask_words + (j >> 5)] >> (j & 31)) & 1;
+                    for (int dt = 0; dt < DTW; ++dt)
 #pragma unroll
-                        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                            for (int rr = 0; rr < 4; ++rr)
-                            {
-                                const int d = 16 * dt + 4 * lq + rr;
-                                const uint32_t w = v[min(d, hs - 1)];
-                                o[qt][dt][rr] += sees && d < hs && tree_nonfinite2<T>(w) ? T16<T>::to_float(w) : 0.f;
-                            }
-                    }
+                        for (int rr = 0; rr < 4; ++rr)
+                        {
+                            const int d = 16 * (dt0 + dt) + 4 * lq + rr;
+                            const uint32_t w = v[min(d, hs - 1)];
+                            acc[dt][rr] += sees && d < hs && tree_nonfinite2<T>(w) ? T16<T>::to_float(w) : 0.f;
+                        }
                 }
             }
-        }
-        const bool alone = tile_lo == 0 && tile_hi == nt; // nothing of this (sequence, kv head) is elsewhere
-        const float v_deq = KVT ? p.kv_scale_quant_orig[0] : 1.f;
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt)
-        {
-            const int in_tile = rw * QT * 16 + 16 * qt + lr, r = mt * M + in_tile;
-            if (r >= n * G)
+            if (mt * M + in_tile >= n * G)
                 continue;
             if (alone)
             {
                 // no visible key: the sum is exactly 0, and so is the row (a NaN sum stays a NaN)
-                const float inv = l_run[qt] == 0.f ? 0.f : v_deq / l_run[qt];
-                uint16_t* out = p.out + ((size_t) (off + r / G) * p.num_heads + head_kv * G + r % G) * hs;
+                const float inv = l == 0.f ? 0.f : v_deq / l;
+                uint16_t* out = p.out + ((size_t) (off + node) * p.num_heads + head_kv * G + (r - node * G)) * hs;
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
-                    if (16 * dt + 4 * lq < hs)
-                        *reinterpret_cast<uint2*>(out + 16 * dt + 4 * lq) = make_uint2(
-                            pack2<T>(o[qt][dt][0] * inv, o[qt][dt][1] * inv), pack2<T>(o[qt][dt][2] * inv, o[qt][dt][3] * inv));
+                for (int dt = 0; dt < DTW; ++dt)
+                {
+                    const int d = 16 * (dt0 + dt) + 4 * lq;
+                    if (d < hs)
+                        *reinterpret_cast<uint2*>(out + d)
+                            = make_uint2(pack2<T>(acc[dt][0] * inv, acc[dt][1] * inv), pack2<T>(acc[dt][2] * inv, acc[dt][3] * inv));
+                }
             }
             else
             {
                 const size_t rec = ((size_t) (2 * team + (tile_lo == 0)) * p.mtiles + mt) * M + in_tile;
-                float* acc = p.part_acc + rec * DP;
+                float* part = p.part_acc + rec * DP;
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
-                    *reinterpret_cast<cf32x4_t*>(acc + 16 * dt + 4 * lq) = o[qt][dt];
-                if (lq == 0)
-                    p.part_ml[rec] = make_float2(m_run[qt], l_run[qt]);
+                for (int dt = 0; dt < DTW; ++dt)
+                    *reinterpret_cast<cf32x4_t*>(part + 16 * (dt0 + dt) + 4 * lq) = acc[dt];
+                if (lq == 0 && kw == 0)
+                    p.part_ml[rec] = make_float2(m, l);
             }
         }
     }
