@@ -13,7 +13,8 @@ namespace
 // Every request holds block_counts[b] blocks; past + new tokens need ceil((past + new) / tokens_per_block).  The missing
 // ones come from the front of a ring of free block indices, in request order; a request that ends returns its blocks to
 // the ring's back.  Two launches: the plan (prefix sums over the requests, one workgroup) and the fill (tables, ring,
-// pointers of every pool, slots), which reads only what the plan does not write, so state updated in place is safe.
+// pointers of every pool, slots).  The fill reads no table or ring entry that it writes, and the state only through the
+// plan's records, so updating it in place is safe.
 struct TableArgs
 {
     const int32_t* past_lengths;
@@ -32,7 +33,7 @@ struct TableArgs
     int4* rows; // workspace [batch]: blocks held before, blocks granted (-1: released), first ring position, status
     int64_t block_bytes;
     int batch, max_blocks, num_blocks, num_pools, num_tokens, tpb, tpb_log2;
-    int pools_per_wg;
+    int pools_per_wg, planes, wgs_per_row;
 };
 
 constexpr int PLAN_THREADS = 1024;
@@ -165,60 +166,9 @@ __device__ __forceinline__ int block_index(const TableArgs& p, int b, const int4
     return idx >= 0 && idx < p.num_blocks ? idx : -1;
 }
 
-// grid (ceil(max_blocks / 512), batch, pool groups + 1), 256 threads, two blocks of the table per thread: bound by the
-// pointer stores.  The last z plane does the table and the ring.
-template <bool PAIRS>
-__global__ __launch_bounds__(256) void table_fill_kernel(TableArgs p)
+// the slot of new token t: its request by bisection of the offsets
+__device__ __forceinline__ void write_slot(const TableArgs& p, int t)
 {
-    const int b = blockIdx.y, j = 2 * (blockIdx.x * 256 + threadIdx.x);
-    if (j >= p.max_blocks)
-        return;
-    const int4 row = p.rows[b];
-    if (blockIdx.z == gridDim.z - 1)
-    {
-        for (int k = j; k < min(j + 2, p.max_blocks); ++k)
-        {
-            int32_t* entry = p.block_table + (size_t) b * p.max_blocks + k;
-            if (row.y < 0 && k < row.x) // released
-                p.free_blocks[wrap((int64_t) row.z + k, p.num_blocks)] = *entry;
-            else if (row.y > 0 && k >= row.x && k < row.x + row.y) // granted
-                *entry = p.free_blocks[wrap((int64_t) row.z + k - row.x, p.num_blocks)];
-        }
-        return;
-    }
-    const int i0 = block_index(p, b, row, j), i1 = j + 1 < p.max_blocks ? block_index(p, b, row, j + 1) : -1;
-    const int64_t k0 = i0 * p.block_bytes, k1 = i1 * p.block_bytes, v = p.num_blocks * p.block_bytes;
-    const int lo = blockIdx.z * p.pools_per_wg, hi = min(lo + p.pools_per_wg, p.num_pools);
-    for (int pool = lo; pool < hi; ++pool)
-    {
-        const int64_t base = p.pool_bases[pool];
-        int64_t* out = p.block_pointers + (((size_t) pool * p.batch + b) * 2) * p.max_blocks + j;
-        const longlong2 kk = make_longlong2(i0 < 0 ? 0 : base + k0, i1 < 0 ? 0 : base + k1);
-        const longlong2 vv = make_longlong2(i0 < 0 ? 0 : base + k0 + v, i1 < 0 ? 0 : base + k1 + v);
-        if constexpr (PAIRS)
-        {
-            *reinterpret_cast<longlong2*>(out) = kk;
-            *reinterpret_cast<longlong2*>(out + p.max_blocks) = vv;
-        }
-        else
-        {
-            out[0] = kk.x;
-            out[p.max_blocks] = vv.x;
-            if (j + 1 < p.max_blocks)
-            {
-                out[1] = kk.y;
-                out[p.max_blocks + 1] = vv.y;
-            }
-        }
-    }
-}
-
-// one thread per new token: its request by bisection of the offsets
-__global__ __launch_bounds__(256) void table_slots_kernel(TableArgs p)
-{
-    const int t = blockIdx.x * 256 + threadIdx.x;
-    if (t >= p.num_tokens)
-        return;
     int64_t slot = -1;
     if (t < p.token_offsets[p.batch])
     {
@@ -241,6 +191,63 @@ __global__ __launch_bounds__(256) void table_slots_kernel(TableArgs p)
         }
     }
     p.slot_map[t] = slot;
+}
+
+// grid: a 1-D list of workgroups of 256 threads, first (ceil(max_blocks / 512), batch, pool groups + 1) of them with two blocks of
+// the table per thread (the last pool group does the table and the ring), then those of the slots, one token per thread.
+// Bound by the pointer stores.
+template <bool PAIRS>
+__global__ __launch_bounds__(256) void table_fill_kernel(TableArgs p)
+{
+    const uint32_t per_plane = p.wgs_per_row * p.batch, plane = blockIdx.x / per_plane, in_plane = blockIdx.x % per_plane;
+    if ((int) plane > p.planes)
+    {
+        const int64_t t = ((int64_t) blockIdx.x - (int64_t) per_plane * (p.planes + 1)) * 256 + threadIdx.x;
+        if (t < p.num_tokens)
+            write_slot(p, (int) t);
+        return;
+    }
+    const int b = in_plane / p.wgs_per_row, j = 2 * (in_plane % p.wgs_per_row * 256 + threadIdx.x);
+    if (j >= p.max_blocks)
+        return;
+    const int4 row = p.rows[b];
+    if ((int) plane == p.planes)
+    {
+        for (int k = j; k < min(j + 2, p.max_blocks); ++k)
+        {
+            int32_t* entry = p.block_table + (size_t) b * p.max_blocks + k;
+            if (row.y < 0 && k < row.x) // released
+                p.free_blocks[wrap((int64_t) row.z + k, p.num_blocks)] = *entry;
+            else if (row.y > 0 && k >= row.x && k < row.x + row.y) // granted
+                *entry = p.free_blocks[wrap((int64_t) row.z + k - row.x, p.num_blocks)];
+        }
+        return;
+    }
+    const int i0 = block_index(p, b, row, j), i1 = j + 1 < p.max_blocks ? block_index(p, b, row, j + 1) : -1;
+    const int64_t k0 = i0 * p.block_bytes, k1 = i1 * p.block_bytes, v = p.num_blocks * p.block_bytes;
+    const int lo = plane * p.pools_per_wg, hi = min(lo + p.pools_per_wg, p.num_pools);
+    for (int pool = lo; pool < hi; ++pool)
+    {
+        const int64_t base = p.pool_bases[pool];
+        int64_t* out = p.block_pointers + (((size_t) pool * p.batch + b) * 2) * p.max_blocks + j;
+        const longlong2 kk = make_longlong2(i0 < 0 ? 0 : base + k0, i1 < 0 ? 0 : base + k1);
+        const longlong2 vv = make_longlong2(i0 < 0 ? 0 : base + k0 + v, i1 < 0 ? 0 : base + k1 + v);
+        if constexpr (PAIRS)
+        {
+            *reinterpret_cast<longlong2*>(out) = kk;
+            *reinterpret_cast<longlong2*>(out + p.max_blocks) = vv;
+        }
+        else
+        {
+            out[0] = kk.x;
+            out[p.max_blocks] = vv.x;
+            if (j + 1 < p.max_blocks)
+            {
+                out[1] = kk.y;
+                out[p.max_blocks + 1] = vv.y;
+            }
+        }
+    }
 }
 
 // ---------------------------------------------------------------------------------------------- accepted path
@@ -451,24 +458,21 @@ void kv_block_tables(const mi355q_kv_block_tables_params& q, hipStream_t stream)
     a.num_pools = q.num_pools;
     a.num_tokens = q.num_tokens;
     a.tpb = q.tokens_per_block;
+    // the pools are dealt over enough workgroups to fill the chip (a table entry is read once per group)
+    a.wgs_per_row = (q.max_blocks_per_seq + 511) / 512;
+    const int64_t per_pool = (int64_t) a.wgs_per_row * q.batch;
+    const int pool_groups = (int) std::max<int64_t>(1, std::min<int64_t>(q.num_pools, (1024 + per_pool - 1) / per_pool));
+    a.pools_per_wg = std::max(1, (q.num_pools + pool_groups - 1) / pool_groups);
+    a.planes = (q.num_pools + a.pools_per_wg - 1) / a.pools_per_wg;
+    const int64_t grid = per_pool * (a.planes + 1) + ((int64_t) q.num_tokens + 255) / 256;
+    MQ_CHECK(grid < (1ll << 31), "block tables: %d requests x %d blocks x %d pools", q.batch, q.max_blocks_per_seq, q.num_pools);
     hipLaunchKernelGGL(table_plan_kernel, dim3(1), dim3(std::min(PLAN_THREADS, (q.batch + 63) / 64 * 64)), 0, stream, a);
     MQ_HIP(hipGetLastError());
-    // the pools are dealt over enough workgroups to fill the chip (a table entry is read once per group)
-    const int per_pool = (q.max_blocks_per_seq + 511) / 512 * q.batch;
-    const int pool_groups = std::max(1, std::min(q.num_pools, (1024 + per_pool - 1) / per_pool));
-    a.pools_per_wg = std::max(1, (q.num_pools + pool_groups - 1) / pool_groups);
-    const int planes = q.num_pools ? (q.num_pools + a.pools_per_wg - 1) / a.pools_per_wg : 0;
-    const dim3 g((q.max_blocks_per_seq + 511) / 512, q.batch, planes + 1);
     if (q.max_blocks_per_seq % 2 == 0 && (reinterpret_cast<uintptr_t>(q.block_pointers) & 15) == 0)
-        hipLaunchKernelGGL(table_fill_kernel<true>, g, dim3(256), 0, stream, a);
+        hipLaunchKernelGGL(table_fill_kernel<true>, dim3((unsigned) grid), dim3(256), 0, stream, a);
     else
-        hipLaunchKernelGGL(table_fill_kernel<false>, g, dim3(256), 0, stream, a);
+        hipLaunchKernelGGL(table_fill_kernel<false>, dim3((unsigned) grid), dim3(256), 0, stream, a);
     MQ_HIP(hipGetLastError());
-    if (q.num_tokens > 0)
-    {
-        hipLaunchKernelGGL(table_slots_kernel, dim3((q.num_tokens + 255) / 256), dim3(256), 0, stream, a);
-        MQ_HIP(hipGetLastError());
-    }
 }
 
 void draft_tree_accept(const mi355q_draft_tree_accept_params& q, hipStream_t stream)

@@ -62,6 +62,7 @@ struct TreeArgs
     uint16_t* q_ws;      // [tokens][Hq][1 or 2 parts][DP]: rotated, times the score scale (and the K dequantisation) and log2(e)
     int4* seq;           // [batch + 1]: key tiles of the sequences before this one, nodes, first row, history; [batch].x: all tiles
     int32_t* seq_ok;     // [batch]: the sequence's blocks are all there
+    int4* join;          // [teams]: the (sequence, kv head) whose first part is the team's last: first row, nodes, kv head, parts (0: none)
     float* part_acc;     // partial states: [team][first | last stretch][m-tile][row][DP]
     float2* part_ml;     // their (running maximum in the log2 domain, sum)
     int64_t qkv_stride;
@@ -458,15 +459,18 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
 
     // swizzle of the 16-byte chunk index by the row, K and V alike.  The banks see a 16-byte read of 64 lanes in groups of rows
     // 0-3, 12-15 at one chunk with rows 4-11 at its neighbour (K fragments: row = lane & 15), and a transposing read in groups of
-    // 4 rows x 2 chunks (V): both fall on all banks once.  It depends on the row modulo 16 only.
+    // 4 rows x 2 chunks (V): both fall on all banks once; so do the writes of every other chunk of two neighbouring rows (8-bit
+    // caches).  It depends on the row modulo 16 only.
     auto sw = [](int row)
     {
         const int x = (row >> 2) & 3;
-        return CH >= 16 ? (row & 3) << 2 | ((x ^ x >> 1) & 1) << 1 | x >> 1 : ((row >> 1) & 3) << 1;
+        return CH >= 16 ? (row & 3) << 2 | ((x ^ x >> 1) & 1) << 1 | (x >> 1 ^ (row & 1)) : ((row >> 1) & 3) << 1;
     };
 
     // ---- the team's stretch of units (sequence, kv head, tile).  A lane holds the record of one of 64 sequences; the one at work
     // is a lane read away
+    int4 join = make_int4(0, 0, 0, 0);
+    int chunk = 0, unit = 0; // unit: the stretch's first one still to do
     int b = 0, hk = 0, tile = 0, left, b0; // left: tiles of the stretch still to do; b0: the first sequence in the lanes
     int4 info;
     int info_next, info_ok;
@@ -488,12 +492,17 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
     {
         fetch_info(0);
         const int units = p.seq[p.batch].x * p.num_kv_heads;
-        const int chunk = tree_chunk(p, units);
+        chunk = tree_chunk(p, units);
         const int64_t u0 = (int64_t) team * chunk;
         left = (int) min((int64_t) chunk, units - u0);
         if (left <= 0)
+        {
+            if (mt == 0 && tid == 0)
+                p.join[team] = join;
             return;
-        const int at = (int) u0 / p.num_kv_heads; // the sequences that end at or before this tile
+        }
+        unit = (int) u0;
+        const int at = unit / p.num_kv_heads; // the sequences that end at or before this tile
         for (;;)
         {
             const uint64_t done = __ballot(b0 + lane < p.batch && info_next <= at);
@@ -504,7 +513,7 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
         }
         b = __builtin_amdgcn_readfirstlane(b);
         const int start = __builtin_amdgcn_readlane(info.x, b - b0), nt = __builtin_amdgcn_readlane(info_next, b - b0) - start;
-        const int in_seq = (int) u0 - start * p.num_kv_heads;
+        const int in_seq = unit - start * p.num_kv_heads;
         hk = in_seq / nt;
         tile = in_seq % nt;
     }
@@ -535,7 +544,9 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
         const int at = b - b0, seq = b, head_kv = hk;
         const int nt = __builtin_amdgcn_readlane(info_next, at) - __builtin_amdgcn_readlane(info.x, at);
         const int tile_lo = tile, tile_hi = min(nt, left < INT32_MAX - nt ? tile + left : nt);
+        const int unit0 = unit;
         left -= tile_hi - tile_lo;
+        unit += tile_hi - tile_lo;
         tile = 0;
         if (p.whole)
             left = 0;
@@ -548,6 +559,8 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
         if (tile_hi <= tile_lo || mt * M >= n * G) // an empty sequence, one that is skipped, or no rows for this m-tile
             continue;
         const int off = __builtin_amdgcn_readlane(info.z, at), past = __builtin_amdgcn_readlane(info.w, at), total = past + n;
+        if (!p.whole && tile_lo == 0 && tile_hi < nt)
+            join = make_int4(off, n, head_kv, (unit0 + nt - 1) / chunk - team + 1);
         const int64_t* const kp = p.block_ptrs + (size_t) seq * 2 * p.max_blocks;
         const int64_t* const vp = kp + p.max_blocks;
 
@@ -1007,34 +1020,30 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
             }
         }
     }
+    if (!p.whole && mt == 0 && tid == 0)
+        p.join[team] = join;
 }
 
 // ---------------------------------------------------------------------------------------------- 3. combine
-// grid (max_draft, batch, ceil(heads / 4)): a wave joins one (token, head), if its keys lay in more than one stretch.  The
-// parts are summed in the keys' order, 8 loads in flight.
+// grid (ceil(rows of a (sequence, kv head) / 8), teams): the (sequence, kv head) that begins in the team's stretch and goes on
+// in the next ones.  Half a wave joins one row; the parts are summed in the keys' order, 4 in flight.
 template <typename T, int DP>
 __global__ __launch_bounds__(TREE_THREADS) void tree_combine_kernel(TreeArgs p, bool quantised)
 {
-    const int b = blockIdx.y, i = blockIdx.x, lane = threadIdx.x & 63;
-    const int h = blockIdx.z * (TREE_THREADS / 64) + (threadIdx.x >> 6);
-    const int4 info = p.seq[b];
-    if (i >= info.y || h >= p.num_heads || !p.seq_ok[b])
+    const int team = blockIdx.y, lane = threadIdx.x & 31;
+    const int4 join = p.join[team];
+    const int S = join.w, G = p.group, r = blockIdx.x * (TREE_THREADS / 32) + (threadIdx.x >> 5);
+    if (S <= 1 || r >= join.y * G)
         return;
-    const int chunk = tree_chunk(p, p.seq[p.batch].x * p.num_kv_heads);
-    const int nt = p.seq[b + 1].x - info.x;
-    const int u0 = info.x * p.num_kv_heads + h / p.group * nt;
-    const int team0 = u0 / chunk, S = (u0 + nt - 1) / chunk - team0 + 1;
-    if (S <= 1)
-        return;
-    const int M = p.rows_per_wg, r = i * p.group + h % p.group;
+    const int M = p.rows_per_wg;
     // record of part s: the last stretch of the first team, the first stretch of the others
-    auto record = [&](int s) { return ((size_t) (2 * (team0 + s) + (s == 0)) * p.mtiles + r / M) * M + r % M; };
-    constexpr int E = DP / 64, U = 8;
+    auto record = [&](int s) { return ((size_t) (2 * (team + s) + (s == 0)) * p.mtiles + r / M) * M + r % M; };
+    constexpr int E = DP / 32, U = 4;
     float mm = NEG_BIG, l = 0.f;
-    for (int s = lane; s < S; s += 64)
+    for (int s = lane; s < S; s += 32)
         mm = fmaxf(mm, p.part_ml[record(s)].x);
 #pragma unroll
-    for (int x = 32; x >= 1; x >>= 1)
+    for (int x = 16; x >= 1; x >>= 1)
         mm = fmaxf(mm, __shfl_xor(mm, x));
     float acc[E] = {};
     for (int s0 = 0; s0 < S; s0 += U)
@@ -1062,11 +1071,11 @@ __global__ __launch_bounds__(TREE_THREADS) void tree_combine_kernel(TreeArgs p, 
             }
     }
     const float inv = l == 0.f ? 0.f : (quantised ? p.kv_scale_quant_orig[0] : 1.f) / l;
-    const size_t head = (size_t) (info.z + i) * p.num_heads + h;
+    uint16_t* out = p.out + ((size_t) (join.x + r / G) * p.num_heads + join.z * G + r % G) * p.hs + E * lane;
 #pragma unroll
-    for (int e = 0; e < E; ++e)
+    for (int e = 0; e < E; e += 2)
         if (E * lane + e < p.hs)
-            p.out[head * p.hs + E * lane + e] = T16<T>::from_float(acc[e] * inv);
+            *reinterpret_cast<uint32_t*>(out + e) = pack2<T>(acc[e] * inv, acc[e + 1] * inv);
 }
 
 // ---------------------------------------------------------------------------------------------- host
@@ -1074,10 +1083,10 @@ struct TreePlan
 {
     int dp, rows_per_wg, mtiles, stages; // padded head size; query rows per workgroup; m-tiles of a (sequence, kv head); LDS ring
     int teams, min_chunk, whole;
-    size_t q_bytes, seq_bytes, ok_bytes, acc_bytes, ml_bytes;
+    size_t q_bytes, seq_bytes, ok_bytes, join_bytes, acc_bytes, ml_bytes;
     size_t total() const
     {
-        return q_bytes + seq_bytes + ok_bytes + acc_bytes + ml_bytes;
+        return q_bytes + seq_bytes + ok_bytes + join_bytes + acc_bytes + ml_bytes;
     }
 };
 size_t round256(size_t x)
@@ -1119,14 +1128,14 @@ TreePlan tree_plan(const mi355q_tree_attention_params& q)
     // two workgroups live on a CU (one with heads beyond 128): as many teams as fill 256 CUs, of at least 2 tiles each (a
     // stretch costs its prologue and a partial state), and no (sequence, kv head) over more teams than the combine reads
     const int64_t slots = t.dp > 128 ? 256 : 512;
-    int64_t teams = std::max<int64_t>(slots / t.mtiles, 1);
+    int64_t teams = std::max<int64_t>(slots / t.mtiles, 1); // (at most 512: a grid dimension of the combine kernel)
     t.min_chunk = std::max(2, (max_tiles + TREE_MAX_SPLITS - 2) / (TREE_MAX_SPLITS - 1));
     if (q.multi_block_mode > 0)
     {
         // that many stretches to the longest history
         t.min_chunk = std::max(1, (max_tiles + q.multi_block_mode - 1) / q.multi_block_mode);
         t.min_chunk = std::max(t.min_chunk, (max_tiles + TREE_MAX_SPLITS - 2) / (TREE_MAX_SPLITS - 1));
-        teams = groups * ((max_tiles + t.min_chunk - 1) / t.min_chunk);
+        teams = std::min<int64_t>(groups * ((max_tiles + t.min_chunk - 1) / t.min_chunk), 65535);
     }
     // short histories: one team per (sequence, kv head), nothing to join
     t.whole = q.multi_block_mode == 1 || (q.multi_block_mode == 0 && max_tiles <= 4);
@@ -1138,6 +1147,7 @@ TreePlan tree_plan(const mi355q_tree_attention_params& q)
     t.ok_bytes = round256((size_t) q.batch * sizeof(int32_t));
     if (!t.whole)
     {
+        t.join_bytes = round256((size_t) t.teams * sizeof(int4));
         const size_t records = (size_t) 2 * t.teams * t.mtiles * t.rows_per_wg;
         t.acc_bytes = round256(records * t.dp * sizeof(float));
         t.ml_bytes = round256(records * sizeof(float2));
@@ -1180,7 +1190,7 @@ void tree_launch(const mi355q_tree_attention_params& q, const TreeArgs& a, const
         tree_launch_attn<T, KVT, 256>(a, t, stream);
     if (!t.whole)
     {
-        const dim3 g(q.max_draft_length, q.batch, (q.num_heads + 3) / 4), b(TREE_THREADS);
+        const dim3 g((t.mtiles * t.rows_per_wg + 7) / 8, t.teams), b(TREE_THREADS);
         if (t.dp == 64)
             hipLaunchKernelGGL((tree_combine_kernel<T, 64>), g, b, 0, stream, a, KVT != 0);
         else if (t.dp == 128)
@@ -1260,11 +1270,18 @@ void tree_attention(const mi355q_tree_attention_params& q, hipStream_t stream)
     a.kv_scale_orig_quant = q.kv_scale_orig_quant;
     a.kv_scale_quant_orig = q.kv_scale_quant_orig;
     char* ws = static_cast<char*>(q.workspace);
-    a.q_ws = reinterpret_cast<uint16_t*>(ws);
-    a.seq = reinterpret_cast<int4*>(ws + t.q_bytes);
-    a.seq_ok = reinterpret_cast<int32_t*>(ws + t.q_bytes + t.seq_bytes);
-    a.part_acc = reinterpret_cast<float*>(ws + t.q_bytes + t.seq_bytes + t.ok_bytes);
-    a.part_ml = reinterpret_cast<float2*>(ws + t.q_bytes + t.seq_bytes + t.ok_bytes + t.acc_bytes);
+    auto carve = [&](size_t bytes)
+    {
+        char* at = ws;
+        ws += bytes;
+        return at;
+    };
+    a.q_ws = reinterpret_cast<uint16_t*>(carve(t.q_bytes));
+    a.seq = reinterpret_cast<int4*>(carve(t.seq_bytes));
+    a.seq_ok = reinterpret_cast<int32_t*>(carve(t.ok_bytes));
+    a.join = reinterpret_cast<int4*>(carve(t.join_bytes));
+    a.part_acc = reinterpret_cast<float*>(carve(t.acc_bytes));
+    a.part_ml = reinterpret_cast<float2*>(carve(t.ml_bytes));
     a.qkv_stride = q.qkv_stride ? q.qkv_stride : (int64_t) hidden;
     a.batch = q.batch;
     a.num_heads = q.num_heads;

@@ -416,35 +416,33 @@ def gpt_attention(plugin, *, qkv, sequence_length, host_past_key_value_lengths, 
 
 
 # ----------------------------------------------------------------------------- speculative decoding (device state only)
-def _check_tensor(name, t, device, dtype=None, shape=None):
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, expected {device}")
-    if dtype is not None and t.dtype != dtype:
-        raise ValueError(f"{name} is {t.dtype}, expected {dtype}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name} is not contiguous")
+def _ptr(name, t, index, dtype, shape):
+    """Address of a contiguous tensor of this type and shape on GPU `index` (a serving step makes these calls per layer: one
+    condition on the good path)."""
+    if t.get_device() != index or t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on cuda:{index}, got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}" + ("" if t.is_contiguous() else ", not contiguous"))
     return t.data_ptr()
 
 
 class _On:
-    """The tensors' device made current for one call (a call may come while another device is), and its current stream."""
+    """GPU `index` made current for one call (a call may come while another device is), and its current stream."""
+
+    __slots__ = ("index", "previous")
 
     def __init__(self, t):
         if not t.is_cuda:
             raise ValueError(f"tensors must be on the GPU, got {t.device}")
-        self.index = t.device.index
-        self.previous = None
+        self.index = t.get_device()
 
     def __enter__(self):
-        if torch.cuda.current_device() != self.index:
-            self.previous = torch.cuda.current_device()
+        self.previous = torch.cuda.current_device()
+        if self.previous != self.index:
             torch.cuda.set_device(self.index)
         return C.c_void_p(torch.cuda.current_stream(self.index).cuda_stream)
 
     def __exit__(self, *exc):
-        if self.previous is not None:
+        if self.previous != self.index:
             torch.cuda.set_device(self.previous)
 
 
@@ -496,36 +494,37 @@ class TreeAttention:
     def __call__(self, qkv, past_lengths, draft_offsets, tree_mask, block_pointers, *, max_draft_length, max_past_length,
                  position_offsets=None, qkv_bias=None, kv_scale_orig_quant=None, kv_scale_quant_orig=None, out=None,
                  workspace=None):
-        dev, i32 = qkv.device, torch.int32
-        if qkv.dim() != 2 or qkv.dtype != self.dtype or qkv.shape[1] != self.hidden or (qkv.numel() and qkv.stride(1) != 1):
+        on = _On(qkv)
+        dev, i32 = on.index, torch.int32
+        if qkv.dim() != 2 or qkv.dtype is not self.dtype or qkv.shape[1] != self.hidden or (qkv.numel() and qkv.stride(1) != 1):
             raise ValueError(f"qkv must be {self.dtype} [num_tokens, {self.hidden}] with contiguous rows, got {qkv.dtype} "
                              f"{tuple(qkv.shape)} strides {qkv.stride()}")
-        tokens, batch = qkv.shape[0], past_lengths.shape[0]
-        if tree_mask.dim() != 2 or block_pointers.dim() != 3:
-            raise ValueError("tree_mask must be [num_tokens, words], block_pointers [batch, 2, max_blocks]")
-        p = self._params(batch, tokens, max_draft_length, max_past_length, block_pointers.shape[2], tree_mask.shape[1])
-        p.past_lengths = _check_tensor("past_lengths", past_lengths, dev, i32, (batch,))
-        p.draft_offsets = _check_tensor("draft_offsets", draft_offsets, dev, i32, (batch + 1,))
-        if tree_mask.dtype not in (torch.int32, torch.uint32):
-            raise ValueError(f"tree_mask is {tree_mask.dtype}, expected int32")
-        p.tree_mask = _check_tensor("tree_mask", tree_mask, dev, None, (tokens, tree_mask.shape[1]))
-        p.block_pointers = _check_tensor("block_pointers", block_pointers, dev, torch.int64, (batch, 2, block_pointers.shape[2]))
+        if past_lengths.dim() != 1 or tree_mask.dim() != 2 or block_pointers.dim() != 3:
+            raise ValueError("past_lengths must be [batch], tree_mask [num_tokens, words], block_pointers [batch, 2, max_blocks]")
+        tokens, batch, words, blocks = qkv.shape[0], past_lengths.shape[0], tree_mask.shape[1], block_pointers.shape[2]
+        p = self._params(batch, tokens, max_draft_length, max_past_length, blocks, words)
+        p.past_lengths = _ptr("past_lengths", past_lengths, dev, i32, (batch,))
+        p.draft_offsets = _ptr("draft_offsets", draft_offsets, dev, i32, (batch + 1,))
+        p.tree_mask = _ptr("tree_mask", tree_mask, dev, torch.uint32 if tree_mask.dtype is torch.uint32 else i32, (tokens, words))
+        p.block_pointers = _ptr("block_pointers", block_pointers, dev, torch.int64, (batch, 2, blocks))
         if position_offsets is not None:
-            p.position_offsets = _check_tensor("position_offsets", position_offsets, dev, i32, (tokens,))
+            p.position_offsets = _ptr("position_offsets", position_offsets, dev, i32, (tokens,))
         if qkv_bias is not None:
-            p.qkv_bias = _check_tensor("qkv_bias", qkv_bias, dev, self.dtype, (self.hidden,))
+            p.qkv_bias = _ptr("qkv_bias", qkv_bias, dev, self.dtype, (self.hidden,))
         if kv_scale_orig_quant is not None:
-            p.kv_scale_orig_quant = _check_tensor("kv_scale_orig_quant", kv_scale_orig_quant, dev, torch.float32, (1,))
-            p.kv_scale_quant_orig = _check_tensor("kv_scale_quant_orig", kv_scale_quant_orig, dev, torch.float32, (1,))
+            p.kv_scale_orig_quant = _ptr("kv_scale_orig_quant", kv_scale_orig_quant, dev, torch.float32, (1,))
+        if kv_scale_quant_orig is not None:
+            p.kv_scale_quant_orig = _ptr("kv_scale_quant_orig", kv_scale_quant_orig, dev, torch.float32, (1,))
         p.qkv, p.qkv_stride = qkv.data_ptr(), qkv.stride(0) if tokens > 1 else 0
-        with _On(qkv) as stream:
+        with on as stream:
             if out is None:
-                out = torch.empty(tokens, self.out_hidden, dtype=self.dtype, device=dev)
-            p.out = _check_tensor("out", out, dev, self.dtype, (tokens, self.out_hidden))
-            need = L.lib().mi355q_tree_attention_workspace_size(C.byref(p))
+                out = torch.empty((tokens, self.out_hidden), dtype=self.dtype, device=qkv.device)
+            p.out = _ptr("out", out, dev, self.dtype, (tokens, self.out_hidden))
             if workspace is None:  # from torch's allocator: ordered on this stream, kept by a graph that captures the call
-                workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
-            p.workspace, p.workspace_bytes = _check_tensor("workspace", workspace, dev), workspace.numel() * workspace.element_size()
+                need = L.lib().mi355q_tree_attention_workspace_size(C.byref(p))
+                workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=qkv.device)
+            p.workspace = _ptr("workspace", workspace, dev, torch.uint8, workspace.shape)
+            p.workspace_bytes = workspace.numel()
             L.check(L.lib().mi355q_tree_attention(C.byref(p), stream))
         return out
 
@@ -538,33 +537,31 @@ def kv_block_tables(past_lengths, new_lengths, block_table, block_counts, free_b
     place, block_counts and free_state too unless *_out is given.  num_tokens: rows of the slot map (at least the sum of the
     positive new_lengths for all of them to be there).  Returns (block_pointers int64 [pools, batch, 2, max_blocks],
     token_offsets int32 [batch + 1], slot_map int64 [num_tokens], status int32 [batch])."""
-    dev, i32 = past_lengths.device, torch.int32
-    if block_table.dim() != 2 or free_blocks.dim() != 1 or pool_bases.dim() != 1:
-        raise ValueError("block_table must be [batch, max_blocks], free_blocks [num_blocks], pool_bases [pools]")
+    on = _On(past_lengths)
+    dev, i32 = on.index, torch.int32
+    if past_lengths.dim() != 1 or block_table.dim() != 2 or free_blocks.dim() != 1 or pool_bases.dim() != 1:
+        raise ValueError("past_lengths must be [batch], block_table [batch, max_blocks], free_blocks [num_blocks], pool_bases [pools]")
     batch, max_blocks, pools = past_lengths.shape[0], block_table.shape[1], pool_bases.shape[0]
-    block_counts_out = block_counts if block_counts_out is None else block_counts_out
-    free_state_out = free_state if free_state_out is None else free_state_out
-    p = L.KvBlockTablesParams()
-    p.past_lengths = _check_tensor("past_lengths", past_lengths, dev, i32, (batch,))
-    p.new_lengths = _check_tensor("new_lengths", new_lengths, dev, i32, (batch,))
-    p.block_table = _check_tensor("block_table", block_table, dev, i32, (batch, max_blocks))
-    p.block_counts = _check_tensor("block_counts", block_counts, dev, i32, (batch,))
-    p.block_counts_out = _check_tensor("block_counts_out", block_counts_out, dev, i32, (batch,))
-    p.free_blocks = _check_tensor("free_blocks", free_blocks, dev, i32)
-    p.free_state = _check_tensor("free_state", free_state, dev, i32, (2,))
-    p.free_state_out = _check_tensor("free_state_out", free_state_out, dev, i32, (2,))
-    p.pool_bases = _check_tensor("pool_bases", pool_bases, dev, torch.int64)
-    p.block_bytes, p.batch, p.max_blocks_per_seq, p.num_blocks = block_bytes, batch, max_blocks, free_blocks.shape[0]
-    p.num_pools, p.num_tokens, p.tokens_per_block = pools, num_tokens, tokens_per_block
-    with _On(past_lengths) as stream:
-        pointers = torch.empty(pools, batch, 2, max_blocks, dtype=torch.int64, device=dev)
-        offsets = torch.empty(batch + 1, dtype=i32, device=dev)
-        slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
-        status = torch.empty(batch, dtype=i32, device=dev)
-        p.workspace_bytes = L.lib().mi355q_kv_block_tables_workspace_size(batch)
-        workspace = torch.empty(max(p.workspace_bytes, 16), dtype=torch.uint8, device=dev)
-        p.block_pointers, p.token_offsets, p.slot_map, p.status = (t.data_ptr() for t in (pointers, offsets, slots, status))
-        p.workspace = workspace.data_ptr()
+    row = (batch,)
+    counts_out = block_counts if block_counts_out is None else block_counts_out
+    state_out = free_state if free_state_out is None else free_state_out
+    with on as stream:
+        where = past_lengths.device
+        pointers = torch.empty((pools, batch, 2, max_blocks), dtype=torch.int64, device=where)
+        slots = torch.empty(num_tokens, dtype=torch.int64, device=where)
+        # offsets, status and the workspace in one allocation, the workspace first (16-byte aligned)
+        need = L.lib().mi355q_kv_block_tables_workspace_size(batch)
+        small = torch.empty(need // 4 + 2 * batch + 1, dtype=i32, device=where)
+        offsets, status = small[need // 4:need // 4 + batch + 1], small[need // 4 + batch + 1:]
+        at = small.data_ptr()
+        p = L.KvBlockTablesParams(
+            _ptr("past_lengths", past_lengths, dev, i32, row), _ptr("new_lengths", new_lengths, dev, i32, row),
+            _ptr("block_table", block_table, dev, i32, (batch, max_blocks)), _ptr("block_counts", block_counts, dev, i32, row),
+            _ptr("block_counts_out", counts_out, dev, i32, row), _ptr("free_blocks", free_blocks, dev, i32, free_blocks.shape),
+            _ptr("free_state", free_state, dev, i32, (2,)), _ptr("free_state_out", state_out, dev, i32, (2,)),
+            _ptr("pool_bases", pool_bases, dev, torch.int64, pool_bases.shape), pointers.data_ptr(), at + need, slots.data_ptr(),
+            at + need + 4 * (batch + 1), at, need, block_bytes, batch, max_blocks, free_blocks.shape[0], pools, num_tokens,
+            tokens_per_block)
         L.check(L.lib().mi355q_kv_block_tables(C.byref(p), stream))
     return pointers, offsets, slots, status
 
@@ -573,20 +570,21 @@ def draft_tree_accept(draft_tokens, parents, target_tokens, draft_offsets, max_p
     """The path along which the model agrees with a tree of drafted tokens (mi355q_draft_tree_accept in mi355q.h): int32
     tensors, draft_tokens / parents / target_tokens [num_tokens], draft_offsets [batch + 1].  Returns (accept_path [batch,
     max_path], accept_counts [batch], accepted_tokens [batch, max_path]), -1 behind the counts."""
-    dev, i32 = draft_tokens.device, torch.int32
-    tokens, batch = draft_tokens.shape[0], draft_offsets.shape[0] - 1
-    p = L.DraftTreeAcceptParams()
-    p.draft_tokens = _check_tensor("draft_tokens", draft_tokens, dev, i32, (tokens,))
-    p.parents = _check_tensor("parents", parents, dev, i32, (tokens,))
-    p.target_tokens = _check_tensor("target_tokens", target_tokens, dev, i32, (tokens,))
-    p.draft_offsets = _check_tensor("draft_offsets", draft_offsets, dev, i32, (batch + 1,))
-    p.batch, p.num_tokens, p.max_path = batch, tokens, max_path
-    with _On(draft_tokens) as stream:
-        path = torch.empty(batch, max_path, dtype=i32, device=dev)
-        counts = torch.empty(batch, dtype=i32, device=dev)
-        emitted = torch.empty(batch, max_path, dtype=i32, device=dev)
-        p.accept_path, p.accept_counts, p.accepted_tokens = path.data_ptr(), counts.data_ptr(), emitted.data_ptr()
+    on = _On(draft_tokens)
+    dev, i32 = on.index, torch.int32
+    if draft_tokens.dim() != 1 or draft_offsets.dim() != 1 or draft_offsets.shape[0] < 1 or max_path < 1:
+        raise ValueError("draft_tokens must be [num_tokens], draft_offsets [batch + 1], max_path at least 1")
+    flat, batch = draft_tokens.shape, draft_offsets.shape[0] - 1
+    with on as stream:
+        both = torch.empty((2, batch, max_path), dtype=i32, device=draft_tokens.device)
+        counts = torch.empty(batch, dtype=i32, device=draft_tokens.device)
+        at = both.data_ptr()
+        p = L.DraftTreeAcceptParams(
+            _ptr("draft_tokens", draft_tokens, dev, i32, flat), _ptr("parents", parents, dev, i32, flat),
+            _ptr("target_tokens", target_tokens, dev, i32, flat), _ptr("draft_offsets", draft_offsets, dev, i32, (batch + 1,)),
+            at, counts.data_ptr(), at + 4 * batch * max_path, batch, flat[0], max_path)
         L.check(L.lib().mi355q_draft_tree_accept(C.byref(p), stream))
+    path, emitted = both.unbind(0)
     return path, counts, emitted
 
 
@@ -594,19 +592,18 @@ def kv_commit_path(block_pointers, past_lengths, accept_path, accept_counts, *, 
                    kv_dtype):
     """Moves the keys and values of the accepted path to the end of every sequence's history, in every pool, in place
     (mi355q_kv_commit_path in mi355q.h).  block_pointers int64 [pools, batch, 2, max_blocks].  Returns the new lengths."""
-    dev, i32 = block_pointers.device, torch.int32
+    on = _On(block_pointers)
+    dev, i32 = on.index, torch.int32
     if block_pointers.dim() != 4 or accept_path.dim() != 2:
         raise ValueError("block_pointers must be [pools, batch, 2, max_blocks], accept_path [batch, max_path]")
     pools, batch, _, max_blocks = block_pointers.shape
-    p = L.KvCommitPathParams()
-    p.block_pointers = _check_tensor("block_pointers", block_pointers, dev, torch.int64, (pools, batch, 2, max_blocks))
-    p.past_lengths = _check_tensor("past_lengths", past_lengths, dev, i32, (batch,))
-    p.accept_path = _check_tensor("accept_path", accept_path, dev, i32, (batch, accept_path.shape[1]))
-    p.accept_counts = _check_tensor("accept_counts", accept_counts, dev, i32, (batch,))
-    p.batch, p.num_pools, p.max_blocks_per_seq, p.tokens_per_block = batch, pools, max_blocks, tokens_per_block
-    p.num_kv_heads, p.head_size, p.max_path, p.kv_type = num_kv_heads, head_size, accept_path.shape[1], torch_dtype_to_trt(kv_dtype)
-    with _On(block_pointers) as stream:
-        lengths = torch.empty(batch, dtype=i32, device=dev)
-        p.new_lengths = lengths.data_ptr()
+    max_path = accept_path.shape[1]
+    with on as stream:
+        lengths = torch.empty(batch, dtype=i32, device=block_pointers.device)
+        p = L.KvCommitPathParams(
+            _ptr("block_pointers", block_pointers, dev, torch.int64, (pools, batch, 2, max_blocks)),
+            _ptr("past_lengths", past_lengths, dev, i32, (batch,)), _ptr("accept_path", accept_path, dev, i32, (batch, max_path)),
+            _ptr("accept_counts", accept_counts, dev, i32, (batch,)), lengths.data_ptr(), batch, pools, max_blocks, tokens_per_block,
+            num_kv_heads, head_size, max_path, torch_dtype_to_trt(kv_dtype))
         L.check(L.lib().mi355q_kv_commit_path(C.byref(p), stream))
     return lengths
