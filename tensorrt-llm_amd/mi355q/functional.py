@@ -425,6 +425,10 @@ def _ptr(name, t, index, dtype, shape):
     return t.data_ptr()
 
 
+# the handle of a GPU's current stream without a Stream object around it (1 us a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
 class _On:
     """GPU `index` made current for one call (a call may come while another device is), and its current stream."""
 
@@ -439,7 +443,7 @@ class _On:
         self.previous = torch.cuda.current_device()
         if self.previous != self.index:
             torch.cuda.set_device(self.index)
-        return C.c_void_p(torch.cuda.current_stream(self.index).cuda_stream)
+        return C.c_void_p(_raw_stream(self.index))
 
     def __exit__(self, *exc):
         if self.previous != self.index:
@@ -476,6 +480,7 @@ class TreeAttention:
             rotary_embedding_scale=rotary_embedding_scale, rotary_embedding_max_positions=rotary_embedding_max_positions,
             multi_block_mode=multi_block_mode)
         self._template = bytes(L.TreeAttentionParams(**self._fields))
+        self._sizes = {}  # bounds of a call -> workspace bytes
 
     def _params(self, batch, num_tokens, max_draft_length, max_past_length, max_blocks, mask_words):
         p = L.TreeAttentionParams.from_buffer_copy(self._template)
@@ -521,7 +526,12 @@ class TreeAttention:
                 out = torch.empty((tokens, self.out_hidden), dtype=self.dtype, device=qkv.device)
             p.out = _ptr("out", out, dev, self.dtype, (tokens, self.out_hidden))
             if workspace is None:  # from torch's allocator: ordered on this stream, kept by a graph that captures the call
-                need = L.lib().mi355q_tree_attention_workspace_size(C.byref(p))
+                bounds = (batch, tokens, max_draft_length, max_past_length, blocks)
+                need = self._sizes.get(bounds)
+                if need is None:
+                    if len(self._sizes) >= 1024:
+                        self._sizes.clear()
+                    need = self._sizes[bounds] = L.lib().mi355q_tree_attention_workspace_size(C.byref(p))
                 workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=qkv.device)
             p.workspace = _ptr("workspace", workspace, dev, torch.uint8, workspace.shape)
             p.workspace_bytes = workspace.numel()
