@@ -130,11 +130,81 @@ __device__ __forceinline__ int tree_chunk(const TreeArgs& p, int units)
     return max((units + p.teams - 1) / p.teams, p.min_chunk);
 }
 
+// 8 elements from d0 on of one head of a qkv row, bias added, rotated: in fp32 or in 64 bits (R).  angle(j, c, s) gives cosine
+// and sine of pair j.
+template <typename T, typename R, typename Angle>
+__device__ __forceinline__ void tree_chunk8(
+    const TreeArgs& p, const uint16_t* src, int vec, int d0, int half, bool rope, R (&y)[8], Angle&& angle)
+{
+    const int at = vec * p.hs;
+    auto elements = [&](int d, R (&x)[8])
+    {
+        const uint4 r = *reinterpret_cast<const uint4*>(src + at + d);
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            x[e] = (e & 1) ? T16<T>::hi(w[e >> 1]) : T16<T>::lo(w[e >> 1]);
+        if (p.qkv_bias)
+        {
+            const uint4 rb = *reinterpret_cast<const uint4*>(p.qkv_bias + at + d);
+            const uint32_t wb[4] = {rb.x, rb.y, rb.z, rb.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                x[e] += (e & 1) ? T16<T>::hi(wb[e >> 1]) : T16<T>::lo(wb[e >> 1]);
+        }
+    };
+    elements(d0, y);
+    if (!rope || d0 >= p.rot_dim)
+        return;
+    R c, s;
+    if (p.pos_type == 1) // GPT-J pairs (2 j, 2 j + 1)
+    {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2)
+            if (d0 + e < p.rot_dim)
+            {
+                angle((d0 + e) >> 1, c, s);
+                const R a = y[e], b = y[e + 1];
+                y[e] = a * c - b * s;
+                y[e + 1] = b * c + a * s;
+            }
+    }
+    else if (half % 8 == 0) // NeoX pairs (j, j + rot_dim / 2): the partners are a chunk of their own
+    {
+        const bool first = d0 < half;
+        R other[8];
+        elements(first ? d0 + half : d0 - half, other);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+        {
+            angle(d0 + e - (first ? 0 : half), c, s);
+            y[e] = y[e] * c + (first ? -other[e] : other[e]) * s;
+        }
+    }
+    else
+    {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+        {
+            const int d = d0 + e;
+            if (d < p.rot_dim)
+            {
+                const bool first = d < half;
+                const int o = at + (first ? d + half : d - half);
+                R other = T16<T>::to_float(src[o]);
+                if (p.qkv_bias)
+                    other += T16<T>::to_float(p.qkv_bias[o]);
+                angle(first ? d : d - half, c, s);
+                y[e] = y[e] * c + (first ? -other : other) * s;
+            }
+        }
+    }
+}
+
 // ---------------------------------------------------------------------------------------------- 1. prepare
-// grid (max_draft + 2, batch, parts of the heads).  Rotation and quantisation of K / V run in 64 bits: the angle of a far position has no
-// correct digits left in fp32 (position 2^17, fp32 angle: error 2^-8 rad), and a value next to a rounding border of the
-// cache's type lands on the side the definition says.  It costs nothing that shows: 2 Hkv Dh values per token against the
-// whole history that the attention reads.
+// grid (max_draft + 2, batch, parts of the heads).  Angles, and rotation and quantisation of K / V, run in 64 bits: the angle of a
+// far position has few correct digits left in fp32 (position 2^17: error 2^-8 rad), and a value next to a rounding border
+// of the cache's type lands on the side the definition says.  The queries, the larger part, are rotated in fp32.
 template <typename T, int KVT>
 __global__ __launch_bounds__(TREE_THREADS) void tree_prepare_kernel(TreeArgs p, int dp)
 {
@@ -172,6 +242,7 @@ __global__ __launch_bounds__(TREE_THREADS) void tree_prepare_kernel(TreeArgs p, 
     const bool rope = p.pos_type == 1 || p.pos_type == 2;
     const int half = p.rot_dim >> 1;
     __shared__ double cs_tab[128], sn_tab[128];
+    __shared__ float2 q_tab[128]; // the same in fp32, for the queries
     if (rope && (int) threadIdx.x < half)
     {
         const int pos = past + (p.position_offsets ? p.position_offsets[row] : i);
@@ -191,6 +262,7 @@ __global__ __launch_bounds__(TREE_THREADS) void tree_prepare_kernel(TreeArgs p, 
         sincospi(2.0 * (turns - rint(turns)), &sn, &cs);
         cs_tab[threadIdx.x] = cs;
         sn_tab[threadIdx.x] = sn;
+        q_tab[threadIdx.x] = make_float2((float) cs, (float) sn);
     }
     __syncthreads();
     const uint16_t* src = p.qkv + (size_t) row * p.qkv_stride;
@@ -211,89 +283,27 @@ __global__ __launch_bounds__(TREE_THREADS) void tree_prepare_kernel(TreeArgs p, 
                     qdst[part * dp / 8] = make_uint4(0, 0, 0, 0);
             continue;
         }
-        // the 8 elements from d on of this head, bias added: exact in 64 bits
-        auto elements = [&](int d, double (&x)[8])
-        {
-            const uint4 r = *reinterpret_cast<const uint4*>(src + vec * hs + d);
-            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                x[e] = (e & 1) ? T16<T>::hi(w[e >> 1]) : T16<T>::lo(w[e >> 1]);
-            if (p.qkv_bias)
-            {
-                const uint4 rb = *reinterpret_cast<const uint4*>(p.qkv_bias + vec * hs + d);
-                const uint32_t wb[4] = {rb.x, rb.y, rb.z, rb.w};
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    x[e] += (e & 1) ? T16<T>::hi(wb[e >> 1]) : T16<T>::lo(wb[e >> 1]);
-            }
-        };
-        double x[8], y[8];
-        elements(d0, x);
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            y[e] = x[e];
-        if (rope && vec < Hq + Hkv && d0 < p.rot_dim)
-        {
-            if (p.pos_type == 1) // GPT-J pairs (2 j, 2 j + 1)
-            {
-#pragma unroll
-                for (int e = 0; e < 8; e += 2)
-                    if (d0 + e < p.rot_dim)
-                    {
-                        const int j = (d0 + e) >> 1;
-                        y[e] = x[e] * cs_tab[j] - x[e + 1] * sn_tab[j];
-                        y[e + 1] = x[e + 1] * cs_tab[j] + x[e] * sn_tab[j];
-                    }
-            }
-            else if (half % 8 == 0) // NeoX pairs (j, j + rot_dim / 2): the partners are a chunk of their own
-            {
-                const bool first = d0 < half;
-                double other[8];
-                elements(first ? d0 + half : d0 - half, other);
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                {
-                    const int j = d0 + e - (first ? 0 : half);
-                    y[e] = x[e] * cs_tab[j] + (first ? -other[e] : other[e]) * sn_tab[j];
-                }
-            }
-            else
-            {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                {
-                    const int d = d0 + e;
-                    if (d < p.rot_dim)
-                    {
-                        const bool first = d < half;
-                        const int j = first ? d : d - half, at = vec * hs + (first ? d + half : d - half);
-                        double other = T16<T>::to_float(src[at]);
-                        if (p.qkv_bias)
-                            other += T16<T>::to_float(p.qkv_bias[at]);
-                        y[e] = x[e] * cs_tab[j] + (first ? -other : other) * sn_tab[j];
-                    }
-                }
-            }
-        }
         if (vec < Hq)
         {
             // q carries the score scale, the K dequantisation and log2(e): the matrix product then IS the exponent
-            float hi[8], lo[8];
+            float y[8], hi[8], lo[8];
+            tree_chunk8<T>(p, src, vec, d0, half, rope, y, [&](int j, float& c, float& s) { c = q_tab[j].x, s = q_tab[j].y; });
 #pragma unroll
             for (int e = 0; e < 8; ++e)
             {
-                double z = y[e] * qscale;
+                float z = y[e] * qscale;
                 if constexpr (!T16<C>::is_bf16) // a finite query stays finite in fp16
-                    z = fabs(z) > 65504.0 && fabs(z) < HUGE_VAL ? copysign(65504.0, z) : z;
-                hi[e] = T16<C>::to_float(T16<C>::from_float((float) z));
-                lo[e] = fabsf(hi[e]) < HUGE_VALF ? (float) (z - hi[e]) : 0.f;
+                    z = fabsf(z) > 65504.f && fabsf(z) < HUGE_VALF ? copysignf(65504.f, z) : z;
+                hi[e] = T16<C>::to_float(T16<C>::from_float(z));
+                lo[e] = fabsf(hi[e]) < HUGE_VALF ? z - hi[e] : 0.f;
             }
             *qdst = make_uint4(pack2<C>(hi[0], hi[1]), pack2<C>(hi[2], hi[3]), pack2<C>(hi[4], hi[5]), pack2<C>(hi[6], hi[7]));
             if constexpr (PARTS == 2)
                 qdst[dp / 8] = make_uint4(pack2<C>(lo[0], lo[1]), pack2<C>(lo[2], lo[3]), pack2<C>(lo[4], lo[5]), pack2<C>(lo[6], lo[7]));
             continue;
         }
+        double y[8];
+        tree_chunk8<T>(p, src, vec, d0, half, rope && vec < Hq + Hkv, y, [&](int j, double& c, double& s) { c = cs_tab[j], s = sn_tab[j]; });
         const int kv = (vec - Hq) / Hkv, hk = (vec - Hq) % Hkv;
         char* const base = kv ? vdst : kdst;
         if (!base)
