@@ -327,65 +327,91 @@ __global__ __launch_bounds__(256) void tree_accept_kernel(const int32_t* draft_t
 // Slot past + i of every pool takes the keys and values of slot past + path[i].  In place: paths rise strictly (a parent's
 // index is below its children's), so slot past + i is never a source of a later entry, and a thread owns the same bytes
 // of a row for all entries: it loads 8 entries, then stores them.
-// grid (batch, pools), 256 threads over K / V x heads x row chunks: bound by the rows it moves.
+// grid (batch, pools), 256 threads over K / V x heads x row chunks.  One wave reads the path, checks it and finds the rows'
+// addresses, 64 entries at a time, all of a lane's loads side by side: what bounds the call is that chain of three round trips
+// (lengths and path, block pointers, rows), then the rows it moves.
+typedef __attribute__((ext_vector_type(4))) uint32_t commit_vec16;
+typedef __attribute__((ext_vector_type(2))) uint32_t commit_vec8;
 template <typename V>
 __global__ __launch_bounds__(256) void commit_path_kernel(const int64_t* block_pointers, const int32_t* past_lengths,
     const int32_t* accept_path, const int32_t* accept_counts, int32_t* new_lengths, int batch, int max_blocks, int tpb_log2,
     int num_kv_heads, int row_bytes, int max_path)
 {
-    constexpr int E = 8; // entries per round
-    __shared__ int64_t src[2][E], dst[2][E];
+    constexpr int C = 64, E = 8; // entries per pass of the wave, per round of loads and stores
+    __shared__ int64_t src[2][C], dst[2][C];
+    __shared__ int refused;
     const int b = blockIdx.x, pool = blockIdx.y, tid = threadIdx.x;
-    const int past = past_lengths[b];
-    const int count = min(accept_counts[b], max_path);
+    const int past = past_lengths[b], given = accept_counts[b];
     const int32_t* path = accept_path + (size_t) b * max_path;
     const int64_t* kp = block_pointers + ((size_t) pool * batch + b) * 2 * max_blocks;
-    bool bad = past < 0 || count < 0;
-    for (int i = tid; i < count && !bad; i += 256)
-    {
-        const int node = path[i];
-        const int64_t pos = (int64_t) past + node;
-        bad = node < 0 || (i > 0 && path[i - 1] >= node) || (pos >> tpb_log2) >= max_blocks;
-        if (!bad)
-            for (int kv = 0; kv < 2; ++kv)
-                bad |= kp[kv * max_blocks + (pos >> tpb_log2)] == 0 || kp[kv * max_blocks + ((past + i) >> tpb_log2)] == 0;
-    }
-    bad = __syncthreads_or(bad);
-    if (pool == 0 && tid == 0)
-        new_lengths[b] = bad ? past : past + count;
-    if (bad)
-        return;
+    const int count = min(given, max_path);
     const int tpb_mask = (1 << tpb_log2) - 1;
-    const int chunks = row_bytes / (int) sizeof(V), work = 2 * num_kv_heads * chunks;
-    for (int i0 = 0; i0 < count; i0 += E)
+    // entries c0 .. c0 + 63: their addresses into src / dst; true if one of them cannot be moved
+    auto find = [&](int c0)
     {
-        __syncthreads(); // the previous round's addresses have been read
-        if (tid < 2 * E)
+        const int i = c0 + tid, node = path[min(i, max_path - 1)], before = i > 0 ? path[min(i, max_path) - 1] : -1;
+        bool bad = past < 0 || given < 0;
+        if (!bad && i < count)
         {
-            const int kv = tid / E, i = i0 + tid % E;
-            if (i < count)
+            const int64_t s = (int64_t) past + node, d = (int64_t) past + i;
+            bad = node <= before || (s >> tpb_log2) >= max_blocks; // (rising from 0 on: d <= s)
+            if (!bad)
             {
-                const int s = past + path[i], d = past + i;
-                src[kv][tid % E] = kp[kv * max_blocks + (s >> tpb_log2)] + (int64_t) (s & tpb_mask) * row_bytes;
-                dst[kv][tid % E] = kp[kv * max_blocks + (d >> tpb_log2)] + (int64_t) (d & tpb_mask) * row_bytes;
+                const int64_t ks = kp[s >> tpb_log2], vs = kp[max_blocks + (s >> tpb_log2)];
+                const int64_t kd = kp[d >> tpb_log2], vd = kp[max_blocks + (d >> tpb_log2)];
+                bad = ks == 0 || vs == 0 || kd == 0 || vd == 0;
+                src[0][tid] = ks + (s & tpb_mask) * row_bytes;
+                src[1][tid] = vs + (s & tpb_mask) * row_bytes;
+                dst[0][tid] = kd + (d & tpb_mask) * row_bytes;
+                dst[1][tid] = vd + (d & tpb_mask) * row_bytes;
             }
-            else
-                src[kv][tid % E] = dst[kv][tid % E] = 0;
         }
-        __syncthreads();
+        return __any(bad);
+    };
+    if (tid < 64)
+    {
+        bool bad = false;
+        // the first entries last: their addresses stay
+        for (int c0 = count > C ? (count - 1) / C * C : 0; c0 >= 0; c0 -= C)
+            bad |= find(c0);
+        if (tid == 0)
+        {
+            refused = bad;
+            if (pool == 0)
+                new_lengths[b] = bad ? past : past + count;
+        }
+    }
+    __syncthreads();
+    if (refused)
+        return;
+    const int chunks = row_bytes / (int) sizeof(V), work = 2 * num_kv_heads * chunks;
+    for (int c0 = 0; c0 < count; c0 += C)
+    {
+        if (c0 > 0)
+        {
+            __syncthreads(); // the addresses before have been read
+            if (tid < 64)
+                find(c0);
+            __syncthreads();
+        }
+        const int here = min(count - c0, C);
         for (int w = tid; w < work; w += 256)
         {
             const int kv = w / (num_kv_heads * chunks), hc = w % (num_kv_heads * chunks), h = hc / chunks, c = hc % chunks;
             const int64_t at = ((int64_t) h << tpb_log2) * row_bytes + (int64_t) c * sizeof(V);
-            V x[E];
+            typedef __attribute__((address_space(1))) V global_v;
+            for (int i0 = 0; i0 < here; i0 += E)
+            {
+                V x[E];
 #pragma unroll
-            for (int e = 0; e < E; ++e)
-                if (src[kv][e] != dst[kv][e])
-                    x[e] = *reinterpret_cast<const V*>(src[kv][e] + at);
+                for (int e = 0; e < E; ++e)
+                    if (i0 + e < here && src[kv][i0 + e] != dst[kv][i0 + e])
+                        x[e] = *(const global_v*) (src[kv][i0 + e] + at);
 #pragma unroll
-            for (int e = 0; e < E; ++e)
-                if (src[kv][e] != dst[kv][e])
-                    *reinterpret_cast<V*>(dst[kv][e] + at) = x[e];
+                for (int e = 0; e < E; ++e)
+                    if (i0 + e < here && src[kv][i0 + e] != dst[kv][i0 + e])
+                        *(global_v*) (dst[kv][i0 + e] + at) = x[e];
+            }
         }
     }
 }
@@ -507,10 +533,10 @@ void kv_commit_path(const mi355q_kv_commit_path_params& q, hipStream_t stream)
     const int row_bytes = q.head_size * (int) dtype_size(q.kv_type);
     const dim3 g(q.batch, q.num_pools);
     if (row_bytes % 16 == 0)
-        hipLaunchKernelGGL(commit_path_kernel<uint4>, g, dim3(256), 0, stream, q.block_pointers, q.past_lengths, q.accept_path,
+        hipLaunchKernelGGL(commit_path_kernel<commit_vec16>, g, dim3(256), 0, stream, q.block_pointers, q.past_lengths, q.accept_path,
             q.accept_counts, q.new_lengths, q.batch, q.max_blocks_per_seq, tpb_log2, q.num_kv_heads, row_bytes, q.max_path);
     else
-        hipLaunchKernelGGL(commit_path_kernel<uint2>, g, dim3(256), 0, stream, q.block_pointers, q.past_lengths, q.accept_path,
+        hipLaunchKernelGGL(commit_path_kernel<commit_vec8>, g, dim3(256), 0, stream, q.block_pointers, q.past_lengths, q.accept_path,
             q.accept_counts, q.new_lengths, q.batch, q.max_blocks_per_seq, tpb_log2, q.num_kv_heads, row_bytes, q.max_path);
     MQ_HIP(hipGetLastError());
 }

@@ -217,6 +217,33 @@ def test_commit(cuda, kv, D, tpb):
     assert lengths.tolist() == [int(past[b]) + (0 if b in refused else len(paths[b])) for b in range(B)]
 
 
+def test_commit_long_paths(cuda):
+    # more entries than one pass finds (64): every third node of 400, a chain that is accepted whole, and one refused at its end
+    kv, D, tpb, Hkv, layers, max_blocks = torch.float16, 64, 32, 2, 2, 16
+    paths = [list(range(0, 400, 3)), list(range(150)), list(range(0, 260, 2)) + [257], list(range(1, 66))]
+    B, P = len(paths), max(map(len, paths))
+    past, blocks = np.array([7, 0, 11, 100]), B * max_blocks
+    rs = np.random.RandomState(0)
+    pool = torch.from_numpy(rs.randint(0, 1000, (layers, 2, blocks, Hkv, tpb, D))).to(kv)
+    table, bb = rs.permutation(blocks).reshape(B, max_blocks), Hkv * tpb * D * 2
+    on, idx = pool.to(cuda), torch.from_numpy(table.astype(np.int64))
+    ptr = torch.stack([idx, idx + blocks], 1)[None] * bb + (on.data_ptr() + torch.arange(layers) * (2 * blocks * bb))[:, None, None, None]
+    path = np.full((B, P), -1)
+    for b, x in enumerate(paths):
+        path[b, :len(x)] = x
+    lengths = F.kv_commit_path(ptr.contiguous().to(cuda), dev_t(past, cuda), dev_t(path, cuda), dev_t([len(x) for x in paths], cuda),
+                               num_kv_heads=Hkv, head_size=D, tokens_per_block=tpb, kv_dtype=kv)
+    torch.cuda.synchronize()
+    want = pool.clone()
+    for b, x in enumerate(paths):
+        if b != 2:
+            for i, node in enumerate(x):
+                s, t = past[b] + node, past[b] + i
+                want[:, :, table[b, t // tpb], :, t % tpb] = pool[:, :, table[b, s // tpb], :, s % tpb]
+    assert torch.equal(on.cpu(), want)
+    assert lengths.tolist() == [int(p) + (0 if b == 2 else len(x)) for b, (p, x) in enumerate(zip(past, paths))]
+
+
 # ------------------------------------------------------------------------------------------------ the whole step
 @pytest.mark.parametrize("kv", [torch.bfloat16, torch.int8])
 def test_speculative_steps(cuda, kv):
