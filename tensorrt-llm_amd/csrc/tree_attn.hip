@@ -416,7 +416,7 @@ __device__ __forceinline__ uint64_t tree_mask64(const uint32_t* row, int words, 
     if (sh)
         v |= (uint64_t) w[2] << (64 - sh);
     if (s0 < 0)
-        v |= s0 <= -64 ? ~0ull : (1ull << -s0) - 1;
+        v |= (1ull << -s0) - 1; // (s0 > -64)
     const int live = n - s0; // keys of the window that exist
     return live >= 64 ? v : (live <= 0 ? 0ull : v & ((1ull << live) - 1));
 }
@@ -435,8 +435,8 @@ __device__ __forceinline__ uint64_t tree_mask64(const uint32_t* row, int words, 
 // Softmax in the log2 domain with the running maximum as the C operand of the first product: what comes out is already
 // s - m, and as long as no column grows past m + 8 (p <= 256: harmless in fp16 / bf16 and in the fp32 sums) nothing is rescaled.
 // Whether one does is an integer maximum over the raw bits (negative floats are negative integers).
-template <typename T, int KVT, int DP, int RW, int KW, int QT, int NS>
-__global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP > 128 || NS > 2 ? 1 : 2))) void tree_attn_kernel(TreeArgs p)
+template <typename T, int KVT, int DP, int RW, int KW, int QT>
+__global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP > 128 ? 1 : 2))) void tree_attn_kernel(TreeArgs p)
 {
     static_assert(RW * KW == 4, "4 waves");
     typedef typename TreeCompute<T, KVT>::type C;
@@ -453,7 +453,7 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
     constexpr int WROWS = TREE_KT / 4;              // a wave loads 16 consecutive keys of a tile
     constexpr int RPD = 1024 / ROWB, DPW = WROWS / RPD; // 16-bit caches: rows per DMA instruction, DMAs per wave
     constexpr int CH8 = DP / 16, RPL = 64 / CH8, LPT = WROWS / RPL; // 8-bit caches: rows per 16-byte load, loads per thread
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[NS * STAGE_BYTES];
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE_BYTES]; // a tile that is computed, a tile that arrives
     __shared__ uint32_t nonfinite[TREE_MAX_DRAFT / 32]; // nodes of the stretch whose V row has an infinity or NaN
 
     const int tid = threadIdx.x, lane = tid & 63;
@@ -627,15 +627,9 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
         __syncthreads(); // everyone is done with the LDS of the stretch before
         if (KVT == 0 && tid < TREE_MAX_DRAFT / 32)
             nonfinite[tid] = 0; // (the barrier of the first tile comes before the first use)
-        constexpr int AHEAD = KVT ? 1 : NS - 1; // tiles in flight
         find_tile(tile_lo);
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i)
-        {
-            if (tile_lo + i < tile_hi)
-                load_tile(i * STAGE_BYTES);
-            find_tile(min(tile_lo + i + 1, tile_hi - 1));
-        }
+        load_tile(0);
+        find_tile(min(tile_lo + 1, tile_hi - 1));
         // ---- Q^T fragments (B operand): column = row q0 + 16 qt + lr, k = d = 32 ks + 8 lq + j
         const int q0 = mt * M + rw * QT * 16;
         uint4 qf[PARTS][QT][KS];
@@ -865,23 +859,17 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
         auto enter_tile = [&]()
         {
             if constexpr (KVT == 0)
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // my share of tile i has landed
+            __syncthreads();                                     // everyone's has, and everyone is done with tile i - 1
+            if (i + 1 < tile_hi)
             {
-                // my share of tile i has landed; up to NS - 2 later tiles stay in flight
-                if (NS > 2 && tile_hi - i > NS - 2)
-                    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 2) * 2 * DPW) : "memory");
-                else
-                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            }
-            __syncthreads(); // everyone's has, and everyone is done with tile i - 1
-            if (i + AHEAD < tile_hi)
-            {
-                load_tile(stage == 0 ? (NS - 1) * STAGE_BYTES : stage - STAGE_BYTES);
-                find_tile(min(i + AHEAD + 1, tile_hi - 1));
+                load_tile(STAGE_BYTES - stage);
+                find_tile(min(i + 2, tile_hi - 1));
             }
         };
         auto leave_tile = [&]()
         {
-            stage = stage + STAGE_BYTES == NS * STAGE_BYTES ? 0 : stage + STAGE_BYTES;
+            stage = STAGE_BYTES - stage;
             ++i;
             if constexpr (KVT != 0)
             {
@@ -939,7 +927,7 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
             else
             {
                 constexpr int STATE = (DT + 1) * 64 * 16; // bytes of one wave's state: float4 per register group and lane
-                static_assert(4 * STATE <= NS * STAGE_BYTES, "states do not fit the tile buffers");
+                static_assert(4 * STATE <= 2 * STAGE_BYTES, "states do not fit the tile buffers");
                 __syncthreads(); // everyone is done with the tiles, or with the states before
                 cf32x4_t* st = reinterpret_cast<cf32x4_t*>(lds + wave * STATE) + lane;
 #pragma unroll
@@ -1091,7 +1079,7 @@ __global__ __launch_bounds__(TREE_THREADS) void tree_combine_kernel(TreeArgs p, 
 // ---------------------------------------------------------------------------------------------- host
 struct TreePlan
 {
-    int dp, rows_per_wg, mtiles, stages; // padded head size; query rows per workgroup; m-tiles of a (sequence, kv head); LDS ring
+    int dp, rows_per_wg, mtiles; // padded head size; query rows per workgroup; m-tiles of a (sequence, kv head)
     int teams, min_chunk, whole;
     size_t q_bytes, seq_bytes, ok_bytes, join_bytes, acc_bytes, ml_bytes;
     size_t total() const
@@ -1132,7 +1120,6 @@ TreePlan tree_plan(const mi355q_tree_attention_params& q)
     // few rows: the 4 waves of a workgroup share the keys of a tile instead of the rows
     t.rows_per_wg = rows <= 16 ? 16 : (rows <= 32 ? 32 : (rows <= 64 || t.dp > 128 ? 64 : 128));
     t.mtiles = (rows + t.rows_per_wg - 1) / t.rows_per_wg;
-    t.stages = 2;
     const int max_tiles = std::max((q.max_past_length + q.max_draft_length + TREE_KT - 1) / TREE_KT, 1);
     const int64_t groups = (int64_t) q.batch * q.num_kv_heads;
     // two workgroups live on a CU (one with heads beyond 128): as many teams as fill 256 CUs, of at least 2 tiles each (a
@@ -1174,13 +1161,13 @@ void tree_launch_attn(const TreeArgs& a, const TreePlan& t, hipStream_t stream)
     // 32 rows a wave; 16 with heads beyond 128, whose accumulators take twice the registers
     constexpr int QT = DP > 128 ? 1 : 2;
     if (t.rows_per_wg == 16)
-        hipLaunchKernelGGL((tree_attn_kernel<T, KVT, DP, 1, 4, 1, 2>), g, b, 0, stream, a);
-    else if (t.rows_per_wg == 16 * QT)
-        hipLaunchKernelGGL((tree_attn_kernel<T, KVT, DP, 1, 4, QT, 2>), g, b, 0, stream, a);
+        hipLaunchKernelGGL((tree_attn_kernel<T, KVT, DP, 1, 4, 1>), g, b, 0, stream, a);
+    else if (t.rows_per_wg == 32)
+        hipLaunchKernelGGL((tree_attn_kernel<T, KVT, DP, 2, 2, 1>), g, b, 0, stream, a);
     else if (t.rows_per_wg == 32 * QT)
-        hipLaunchKernelGGL((tree_attn_kernel<T, KVT, DP, 2, 2, QT, 2>), g, b, 0, stream, a);
+        hipLaunchKernelGGL((tree_attn_kernel<T, KVT, DP, 2, 2, QT>), g, b, 0, stream, a);
     else
-        hipLaunchKernelGGL((tree_attn_kernel<T, KVT, DP, 4, 1, QT, 2>), g, b, 0, stream, a);
+        hipLaunchKernelGGL((tree_attn_kernel<T, KVT, DP, 4, 1, QT>), g, b, 0, stream, a);
     MQ_HIP(hipGetLastError());
 }
 
