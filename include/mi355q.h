@@ -508,8 +508,8 @@ extern "C"
      * that sees nothing is 0.  What a row does not see does not reach it, infinities and NaN included.  K / V are read back
      * from the cache, so an 8-bit cache attends to the quantised nodes.
      * A sequence whose device-side lengths do not fit (past_lengths outside 0 .. max_past_length, more than
-     * max_draft_length nodes, rows outside num_tokens, keys beyond the block table) or whose table lacks a block (pointer 0)
-     * is skipped: its rows of out stay as they were.  Rows of qkv / out outside every sequence are not touched. */
+     * max_draft_length nodes, rows outside num_tokens, keys beyond the block table) or whose table lacks a block (pointer 0, or
+     * not 16-byte aligned) is skipped: its rows of out stay as they were.  Rows of qkv / out outside every sequence are not touched. */
     typedef struct
     {
         const void* qkv;            /* [num_tokens, (Hq+2Hkv)*Dh] act type, row stride qkv_stride; q | k | v */
@@ -598,7 +598,8 @@ extern "C"
 
     /* Slot past_lengths[b] + i takes the keys and values of slot past_lengths[b] + accept_path[b][i], i < accept_counts[b], in
      * every pool; new_lengths[b] = past_lengths[b] + accept_counts[b].  A path has to rise strictly and stay inside the
-     * sequence's blocks; otherwise nothing of that sequence moves and new_lengths[b] = past_lengths[b]. */
+     * sequence's blocks; otherwise nothing of that sequence moves and new_lengths[b] = past_lengths[b].  (A pool whose table
+     * lacks a block that the others have moves nothing either; new_lengths follows pool 0.)  Blocks are 16-byte aligned. */
     typedef struct
     {
         const int64_t* block_pointers; /* device [num_pools, batch, 2, max_blocks_per_seq] */

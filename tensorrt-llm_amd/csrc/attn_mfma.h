@@ -38,7 +38,7 @@ __device__ __forceinline__ float ctx_max3(float a, float b, float c)
 // the two results are [x0 x0 x2 x2] / [x1 x1 x3 x3] by rows of 16 lanes (W = 16) or [lo lo] / [hi hi] by halves
 // (W = 32), so their max is the pairwise all-reduce.  The swap and the max sit in ONE asm statement: given the builtin,
 // hipcc treats the swap's two results as the same value when its operands are copies of each other and emits
-// max(r0, r0) -- every lane then ends up with the first row's maximum instead of the column's (found in round 2: a
+// max(r0, r0) -- every lane then ends up with the first row's maximum instead of the column's (a
 // consistent but too small running maximum, harmless until a sliding window leaves that row with nothing but masked
 // scores).  s_nop 1 either side: a VALU write needs 2 wait states before the swap reads it, and the swap's results
 // 2 before a VALU reads them; the compiler cannot see inside the statement to add them.

@@ -491,7 +491,7 @@ void kv_block_tables(const mi355q_kv_block_tables_params& q, hipStream_t stream)
     a.pools_per_wg = std::max(1, (q.num_pools + pool_groups - 1) / pool_groups);
     a.planes = (q.num_pools + a.pools_per_wg - 1) / a.pools_per_wg;
     const int64_t grid = per_pool * (a.planes + 1) + ((int64_t) q.num_tokens + 255) / 256;
-    MQ_CHECK(grid < (1ll << 31), "block tables: %d requests x %d blocks x %d pools", q.batch, q.max_blocks_per_seq, q.num_pools);
+    MQ_CHECK(grid < (1ll << 24), "block tables: %d requests x %d blocks x %d pools", q.batch, q.max_blocks_per_seq, q.num_pools);
     hipLaunchKernelGGL(table_plan_kernel, dim3(1), dim3(std::min(PLAN_THREADS, (q.batch + 63) / 64 * 64)), 0, stream, a);
     MQ_HIP(hipGetLastError());
     if (q.max_blocks_per_seq % 2 == 0 && (reinterpret_cast<uintptr_t>(q.block_pointers) & 15) == 0)
@@ -503,7 +503,7 @@ void kv_block_tables(const mi355q_kv_block_tables_params& q, hipStream_t stream)
 
 void draft_tree_accept(const mi355q_draft_tree_accept_params& q, hipStream_t stream)
 {
-    MQ_CHECK(q.batch >= 0 && q.num_tokens >= 0 && q.max_path > 0, "batch %d, num_tokens %d, max_path %d", q.batch, q.num_tokens, q.max_path);
+    MQ_CHECK(q.batch >= 0 && q.batch <= (1 << 24) && q.num_tokens >= 0 && q.max_path > 0, "batch %d, num_tokens %d, max_path %d", q.batch, q.num_tokens, q.max_path);
     if (q.batch == 0)
         return;
     MQ_CHECK(q.draft_offsets && q.accept_path && q.accept_counts && q.accepted_tokens, "null tensor");
@@ -515,7 +515,7 @@ void draft_tree_accept(const mi355q_draft_tree_accept_params& q, hipStream_t str
 
 void kv_commit_path(const mi355q_kv_commit_path_params& q, hipStream_t stream)
 {
-    MQ_CHECK(q.batch >= 0 && q.num_pools > 0 && q.num_pools <= 65535 && q.max_path > 0, "batch %d, num_pools %d, max_path %d", q.batch,
+    MQ_CHECK(q.batch >= 0 && q.batch < (1 << 24) && q.num_pools > 0 && q.num_pools <= 65535 && q.max_path > 0, "batch %d, num_pools %d, max_path %d", q.batch,
         q.num_pools, q.max_path);
     MQ_CHECK(q.max_blocks_per_seq > 0 && q.num_kv_heads > 0, "max_blocks_per_seq %d, num_kv_heads %d", q.max_blocks_per_seq, q.num_kv_heads);
     MQ_CHECK(q.kv_type == MI355Q_HALF || q.kv_type == MI355Q_BF16 || q.kv_type == MI355Q_INT8 || q.kv_type == MI355Q_FP8, "kv cache type %d",

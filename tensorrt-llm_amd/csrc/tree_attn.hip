@@ -225,11 +225,11 @@ __global__ __launch_bounds__(TREE_THREADS) void tree_prepare_kernel(TreeArgs p, 
     {
         if (blockIdx.z > 0)
             return;
-        // every block the sequence's keys live in has to be there (0 = not allocated)
+        // every block the sequence's keys live in has to be there (0 = not allocated) and aligned like the loads from it
         bool bad = !ok;
         if (ok)
             for (int j = threadIdx.x; j < (past + n + tpb - 1) >> p.tpb_log2; j += TREE_THREADS)
-                bad |= kp[j] == 0 || kp[p.max_blocks + j] == 0;
+                bad |= kp[j] == 0 || kp[p.max_blocks + j] == 0 || ((kp[j] | kp[p.max_blocks + j]) & 15) != 0;
         bad = __syncthreads_or(bad);
         if (threadIdx.x == 0)
             p.seq_ok[b] = !bad;
@@ -306,7 +306,7 @@ __global__ __launch_bounds__(TREE_THREADS) void tree_prepare_kernel(TreeArgs p, 
         tree_chunk8<T>(p, src, vec, d0, half, rope && vec < Hq + Hkv, y, [&](int j, double& c, double& s) { c = cs_tab[j], s = sn_tab[j]; });
         const int kv = (vec - Hq) / Hkv, hk = (vec - Hq) % Hkv;
         char* const base = kv ? vdst : kdst;
-        if (!base)
+        if (!base || (reinterpret_cast<uintptr_t>(base) & 15))
             continue;
         const size_t e0 = ((size_t) hk * tpb + tin) * hs + d0;
         if constexpr (KVT == 0)
@@ -891,7 +891,14 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
                 step(std::true_type{}, stage, kb, t0);
             leave_tile();
             if constexpr (KW == 1)
-                while (i < plain_end)
+            {
+                // (scores of -inf only, of an overflow in fp32: the column has no maximum yet, the general step goes on)
+                bool open = false;
+#pragma unroll
+                for (int qt = 0; qt < QT; ++qt)
+                    open |= fresh[qt];
+                const bool settled = !__any(open);
+                while (settled && i < plain_end)
                 {
                     enter_tile();
 #pragma unroll 1
@@ -899,6 +906,7 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
                         step(std::false_type{}, stage, kb, 0);
                     leave_tile();
                 }
+            }
         }
 
         // ---- the end of the stretch: the sum over the 4 lanes of a column; the states of the KW key groups meet in the LDS, and
@@ -1130,7 +1138,8 @@ TreePlan tree_plan(const mi355q_tree_attention_params& q)
     if (q.multi_block_mode > 0)
     {
         // that many stretches to the longest history
-        t.min_chunk = std::max(1, (max_tiles + q.multi_block_mode - 1) / q.multi_block_mode);
+        const int splits = std::min(q.multi_block_mode, max_tiles);
+        t.min_chunk = (max_tiles + splits - 1) / splits;
         t.min_chunk = std::max(t.min_chunk, (max_tiles + TREE_MAX_SPLITS - 2) / (TREE_MAX_SPLITS - 1));
         teams = std::min<int64_t>(groups * ((max_tiles + t.min_chunk - 1) / t.min_chunk), 65535);
     }
@@ -1156,7 +1165,7 @@ template <typename T, int KVT, int DP>
 void tree_launch_attn(const TreeArgs& a, const TreePlan& t, hipStream_t stream)
 {
     const int64_t grid = ((int64_t) t.teams + 7) / 8 * 8 * t.mtiles;
-    MQ_CHECK(grid < (1ll << 31), "tree attention grid %lld", (long long) grid);
+    MQ_CHECK(grid < (1ll << 24), "tree attention grid %lld", (long long) grid); // 2^32 threads
     const dim3 g((unsigned) grid), b(TREE_THREADS);
     // 32 rows a wave; 16 with heads beyond 128, whose accumulators take twice the registers
     constexpr int QT = DP > 128 ? 1 : 2;

@@ -504,6 +504,8 @@ class TreeAttention:
         if qkv.dim() != 2 or qkv.dtype is not self.dtype or qkv.shape[1] != self.hidden or (qkv.numel() and qkv.stride(1) != 1):
             raise ValueError(f"qkv must be {self.dtype} [num_tokens, {self.hidden}] with contiguous rows, got {qkv.dtype} "
                              f"{tuple(qkv.shape)} strides {qkv.stride()}")
+        if qkv.shape[0] > 1 and qkv.stride(0) < self.hidden:
+            raise ValueError(f"rows of qkv overlap: strides {qkv.stride()}")
         if past_lengths.dim() != 1 or tree_mask.dim() != 2 or block_pointers.dim() != 3:
             raise ValueError("past_lengths must be [batch], tree_mask [num_tokens, words], block_pointers [batch, 2, max_blocks]")
         tokens, batch, words, blocks = qkv.shape[0], past_lengths.shape[0], tree_mask.shape[1], block_pointers.shape[2]

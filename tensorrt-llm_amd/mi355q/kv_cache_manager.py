@@ -285,6 +285,8 @@ class DeviceBlocksManager:
         sizes = {p.nelement() * p.element_size() // (2 * blocks) for p in memory_pools}
         if len(sizes) != 1 or any(p.device != dev for p in memory_pools):
             raise ValueError("the pools must have one block size and lie on one device")
+        if any(p.nelement() % (2 * blocks) or not p.is_contiguous() for p in memory_pools):
+            raise ValueError(f"the pools must be contiguous and hold {blocks} K and {blocks} V blocks each")
         self.memory_pools, self.blocks, self.tokens_per_block = memory_pools, blocks, tokens_per_block
         self.block_bytes = sizes.pop()
         t = lambda v, dt=torch.int32: torch.tensor(v, dtype=dt, device=dev)

@@ -156,7 +156,8 @@ class TreeCase:
                     ab = w[:, ~strange] @ v[~strange].abs()
                     for t in torch.nonzero(strange).flatten().tolist():
                         o[~hidden[:, t]] += w[~hidden[:, t], t][:, None] * v[t]
-                    amax = (q.abs() @ torch.nan_to_num(k).abs().t()).masked_fill(hidden, 0.0).amax(1, keepdim=True)
+                    # (a key whose weight is 0 in 64 bits adds nothing, however its score is rounded)
+                    amax = (q.abs() @ torch.nan_to_num(k).abs().t()).masked_fill(hidden | (w == 0), 0.0).amax(1, keepdim=True)
                     cols = slice((h * G + g) * D, (h * G + g + 1) * D)
                     out[lo:lo + n, cols] = o
                     bound[lo:lo + n, cols] = (torch.expm1(2 * u * amax) + 2 * u + 2.0 ** -16) * ab + 1e-7

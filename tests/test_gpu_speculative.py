@@ -291,3 +291,71 @@ def test_speculative_steps(cuda, kv):
                     s, t = host_past[b] + want_path[b, i], host_past[b] + i
                     mirror[layer][:, table[b, t // tpb], :, t % tpb] = before[:, table[b, s // tpb], :, s % tpb]
             assert torch.equal(pool[layer].cpu().view(torch.uint8), mirror[layer].view(torch.uint8))
+
+
+def test_captured_steps_on_two_streams(cuda):
+    """A whole step captured once per batch, state updated in place, replayed on two streams at once with eager work in
+    between: results and caches equal those of the same steps run eagerly, bit for bit."""
+    layers, B, Hq, Hkv, D, tpb, max_blocks, blocks, P, n = 2, 4, 8, 2, 64, 16, 12, 60, 5, 9
+    op = F.TreeAttention(num_heads=Hq, num_kv_heads=Hkv, head_size=D, dtype=torch.bfloat16, tokens_per_block=tpb,
+                         position_embedding_type=2, rotary_embedding_dim=D)
+
+    class State:
+        def __init__(self, seed):
+            g = torch.Generator().manual_seed(seed)
+            self.pool = [torch.randn(2, blocks, Hkv, tpb, D, generator=g).to(torch.bfloat16).to(cuda) for _ in range(layers)]
+            self.mgr = DeviceBlocksManager(self.pool, blocks, tpb, max_blocks, batch_size=B)
+            self.past = torch.tensor([0, 21, 40, 64], dtype=I32, device=cuda)
+            self.mgr.step(torch.zeros_like(self.past), self.past, num_tokens=1)
+            rs = np.random.RandomState(seed)
+            self.new = dev_t([n, n, 0, n], cuda)  # a row of a padded batch that drafts nothing
+            trees = [R.tree_rows(random_tree(rs, n)) for _ in range(3)]
+            self.mask = dev_t(np.concatenate([R.pack_rows(rows, 1) for rows, _ in trees]).view(np.int32), cuda)
+            self.depth = dev_t(np.concatenate([depth for _, depth in trees]), cuda)
+            self.qkv = torch.zeros(layers, 3 * n, (Hq + 2 * Hkv) * D, dtype=torch.bfloat16, device=cuda)
+            self.tokens, self.target = (torch.zeros(3 * n, dtype=I32, device=cuda) for _ in range(2))
+            self.parents = dev_t(np.concatenate([random_tree(rs, n) for _ in range(3)]), cuda)
+
+        def inputs(self, step):
+            g = torch.Generator().manual_seed(100 + step)
+            self.qkv.copy_(torch.randn(self.qkv.shape, generator=g))
+            for t in (self.tokens, self.target):
+                t.copy_(torch.randint(0, 2, t.shape, generator=g))
+
+        def step(self):
+            ptr, offsets, _, _ = self.mgr.step(self.past, self.new, num_tokens=3 * n)
+            outs = [op(self.qkv[i], self.past, offsets, self.mask, ptr[i], max_draft_length=n, max_past_length=150,
+                       position_offsets=self.depth) for i in range(layers)]
+            path, counts, said = F.draft_tree_accept(self.tokens, self.parents, self.target, offsets, P)
+            self.past.copy_(F.kv_commit_path(ptr, self.past, path, counts, num_kv_heads=Hkv, head_size=D, tokens_per_block=tpb,
+                                             kv_dtype=torch.bfloat16))
+            return outs + [path, counts, said, ptr - self.mgr.pool_bases.view(-1, 1, 1, 1) * (ptr != 0)]
+
+        def all(self):
+            return self.pool + [self.past, self.mgr.block_table, self.mgr.block_counts, self.mgr.free_ring, self.mgr.free_state]
+
+    graphs, eager = [State(1), State(2)], [State(1), State(2)]
+    streams, captured = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for s, stream in zip(graphs, streams):
+        stream.wait_stream(torch.cuda.current_stream())
+        before = [t.clone() for t in s.all()]
+        with torch.cuda.stream(stream):
+            s.step()  # outside the capture once
+            for t, b in zip(s.all(), before):
+                t.copy_(b)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                got = s.step()
+        captured.append((graph, got))
+    torch.cuda.synchronize()
+    for step in range(4):
+        for s in graphs + eager:
+            s.inputs(step)
+        torch.cuda.synchronize()
+        for (graph, _), stream in zip(captured, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for s, e, (_, got) in zip(graphs, eager, captured):
+            for x, y in zip(got + s.all(), e.step() + e.all()):
+                assert torch.equal(x.view(torch.uint8), y.view(torch.uint8)), step

@@ -207,6 +207,40 @@ def test_sequences_that_do_not_fit_are_skipped(cuda):
     compare(c, out, pool, ref, bound, ref_pool)
 
 
+@pytest.mark.parametrize("Hq,n", [(2, 4), (2, 12), (2, 24), (2, 40)])
+def test_scores_beyond_fp32(cuda, Hq, n):
+    # the first keys' scores are -1e40 / 8, -inf in fp32: weight 0; so is the only maximum the first tiles could have
+    c = TreeCase([300, 130], trees([n, n]), Hq, 1, 64, BF)
+    c.qkv[:, 0:Hq * 64:64] = 1e20
+    c.qkv[:, Hq * 64] = 0.0
+    for b, p in enumerate(c.past):
+        for t in range(p):
+            c.pool[0, c.table[b, t // c.tpb], :, t % c.tpb, 0] = -1e20 if t < 129 else 0.0
+    check(c, cuda, rms=False)
+
+
+def test_a_block_that_is_not_aligned(cuda):
+    # the sequence is skipped and nothing goes to that block
+    c = TreeCase([40, 50], trees([8, 8]), 4, 2, 64, BF, tpb=16)
+    ref, bound, ref_pool = c.reference(skip=(1,))
+    pool = c.pool.to(cuda)
+    args, kw = device_args(c, cuda, pool)
+    args[4][1, :, 3] += 8  # positions 48 .. 63: all of its nodes'
+    out = torch.full((c.tokens, c.Hq * c.D), 7.0, dtype=BF, device=cuda)
+    make_op(c)(*args, out=out, **kw)
+    torch.cuda.synchronize()
+    compare(c, out, pool, ref, bound, ref_pool)
+
+
+def test_rows_that_overlap_are_refused(cuda):
+    c = TreeCase([40], trees([4]), 4, 2, 64, BF)
+    args, kw = device_args(c, cuda, c.pool.to(cuda))
+    rows = args[0]
+    for bad in (rows[:1].expand(4, -1), rows.view(-1).as_strided(rows.shape, (8, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            make_op(c)(bad, *args[1:], **kw)
+
+
 def test_repeats_are_equal_and_other_streams(cuda):
     c = TreeCase([900, 40, 333], trees([30, 64, 5]), 8, 2, 128, BF, F8, rope=2)
     pool = c.pool.to(cuda)
