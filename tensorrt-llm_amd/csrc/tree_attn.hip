@@ -879,6 +879,7 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
         };
         // the first tile and the tiles with nodes go through the general step, the history's others through the short one
         // (with few rows one copy of the step: fetching code costs more there than a mask test)
+        const bool has_rows = q0 < n * G; // a wave without rows (a smaller tree than the largest) only loads
         const int plain_end = KW == 1 ? min(tile_hi, past / TREE_KT) : 0;
         while (i < tile_hi)
         {
@@ -887,7 +888,7 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
             if (t0 + TREE_KT > past)
                 clean_tail(stage, t0);
 #pragma unroll 1
-            for (int kb = 0; kb < 16 * XW; kb += 16 * X2)
+            for (int kb = has_rows ? 0 : 16 * XW; kb < 16 * XW; kb += 16 * X2)
                 step(std::true_type{}, stage, kb, t0);
             leave_tile();
             if constexpr (KW == 1)
