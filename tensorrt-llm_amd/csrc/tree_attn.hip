@@ -1126,11 +1126,15 @@ TreePlan tree_plan(const mi355q_tree_attention_params& q)
     TreePlan t{};
     t.dp = q.head_size <= 64 ? 64 : (q.head_size <= 128 ? 128 : 256);
     const int rows = std::max(q.max_draft_length, 1) * (q.num_heads / q.num_kv_heads);
-    // few rows: the 4 waves of a workgroup share the keys of a tile instead of the rows
-    t.rows_per_wg = rows <= 16 ? 16 : (rows <= 32 ? 32 : (rows <= 64 || t.dp > 128 ? 64 : 128));
-    t.mtiles = (rows + t.rows_per_wg - 1) / t.rows_per_wg;
     const int max_tiles = std::max((q.max_past_length + q.max_draft_length + TREE_KT - 1) / TREE_KT, 1);
     const int64_t groups = (int64_t) q.batch * q.num_kv_heads;
+    // Few rows: the 4 waves of a workgroup share the keys of a tile instead of the rows.  Whole calls, us, with 16 / 32 / 64 / 128 rows
+    // a workgroup (bf16, Dh 128, 32 sequences of 2048 tokens, 32 heads): 16 nodes 235 / 235 / 238 / 240, 32 nodes 278 / 245 / 253 /
+    // 253, 64 nodes 402 / 290 / 273 / 279, 128 nodes 741 / 460 / 369 / 337.
+    // 33 to 64 rows of fewer than 256 (sequence, kv head) pairs go as two tiles of 32: half as many teams, so fewer states to
+    // join (8 nodes x 8 heads over 4096 tokens, 4 / 8 / 16 sequences: 32.8 / 41.1 / 68.7 us, as one tile of 64 34.3 / 46.9 / 70.5)
+    t.rows_per_wg = rows <= 16 ? 16 : (rows <= 32 || (rows <= 64 && t.dp <= 128 && groups < 256) ? 32 : (rows <= 64 || t.dp > 128 ? 64 : 128));
+    t.mtiles = (rows + t.rows_per_wg - 1) / t.rows_per_wg;
     // two workgroups live on a CU (one with heads beyond 128): as many teams as fill 256 CUs, of at least 2 tiles each (a
     // stretch costs its prologue and a partial state), and no (sequence, kv head) over more teams than the combine reads
     const int64_t slots = t.dp > 128 ? 256 : 512;
@@ -1144,8 +1148,10 @@ TreePlan tree_plan(const mi355q_tree_attention_params& q)
         t.min_chunk = std::max(t.min_chunk, (max_tiles + TREE_MAX_SPLITS - 2) / (TREE_MAX_SPLITS - 1));
         teams = std::min<int64_t>(groups * ((max_tiles + t.min_chunk - 1) / t.min_chunk), 65535);
     }
-    // short histories: one team per (sequence, kv head), nothing to join
-    t.whole = q.multi_block_mode == 1 || (q.multi_block_mode == 0 && max_tiles <= 4);
+    // short histories, and with pairs enough for every CU those up to 2048 tokens: one team per pair, nothing to join.  us whole
+    // / in stretches (8 nodes, 32 heads): 1 sequence of 440 tokens 13.1 / 17.0, of 1000 18.4 / 16.0; (16 nodes) 8 of 1000 30.8 /
+    // 35.6, 8 of 250 .. 2000 38.5 / 44.8, 32 of 250 .. 2000 151 / 160, 8 of 1000 .. 8000 172 / 147
+    t.whole = q.multi_block_mode == 1 || (q.multi_block_mode == 0 && max_tiles <= (groups >= 256 ? 32 : 8));
     t.teams = (int) std::min<int64_t>(t.whole ? groups : std::min(teams, (groups * max_tiles + t.min_chunk - 1) / t.min_chunk), INT32_MAX / 16);
     t.teams = std::max(t.teams, 1);
     const bool two_parts = q.kv_type == q.act_type || q.act_type == MI355Q_HALF; // TREE_Q2
