@@ -1148,10 +1148,13 @@ TreePlan tree_plan(const mi355q_tree_attention_params& q)
         t.min_chunk = std::max(t.min_chunk, (max_tiles + TREE_MAX_SPLITS - 2) / (TREE_MAX_SPLITS - 1));
         teams = std::min<int64_t>(groups * ((max_tiles + t.min_chunk - 1) / t.min_chunk), 65535);
     }
-    // short histories, and with pairs enough for every CU those up to 2048 tokens: one team per pair, nothing to join.  us whole
-    // / in stretches (8 nodes, 32 heads): 1 sequence of 440 tokens 13.1 / 17.0, of 1000 18.4 / 16.0; (16 nodes) 8 of 1000 30.8 /
-    // 35.6, 8 of 250 .. 2000 38.5 / 44.8, 32 of 250 .. 2000 151 / 160, 8 of 1000 .. 8000 172 / 147
-    t.whole = q.multi_block_mode == 1 || (q.multi_block_mode == 0 && max_tiles <= (groups >= 256 ? 32 : 8));
+    // One team per (sequence, kv head), nothing to join, for short histories: up to 512 tokens, and up to 4096 the longer the more
+    // workgroups there are to even the lengths out (64 tiles with the chip's 512).  us whole / in stretches, histories of t / 6 .. t
+    // tokens: 128 workgroups (4 sequences, 32 heads, 16 nodes) t = 600 17.5 / 23.3, t = 1000 21.5 / 25.2; 256 (8 of 32 heads, 16 nodes)
+    // 2100 40.6 / 47.5, 3400 66.2 / 62.0; 512 (16 of 32 heads, 64 nodes) 2100 96.9 / 117.9, 4100 167.8 / 188.4; 1024 4100 280.3 / 277.9;
+    // 32 (one sequence) 1000 18.3 / 16.1
+    const int64_t whole_tiles = std::min<int64_t>(std::max<int64_t>(groups * t.mtiles / 8, 8), 64);
+    t.whole = q.multi_block_mode == 1 || (q.multi_block_mode == 0 && max_tiles <= whole_tiles);
     t.teams = (int) std::min<int64_t>(t.whole ? groups : std::min(teams, (groups * max_tiles + t.min_chunk - 1) / t.min_chunk), INT32_MAX / 16);
     t.teams = std::max(t.teams, 1);
     const bool two_parts = q.kv_type == q.act_type || q.act_type == MI355Q_HALF; // TREE_Q2
