@@ -21,7 +21,7 @@ namespace
 
 constexpr int TREE_KT = 64;         // keys per tile
 constexpr int TREE_THREADS = 256;   // 4 waves
-constexpr int TREE_MAX_SPLITS = 128; // teams that share a (sequence, kv head): what the combine kernel reads
+constexpr int TREE_MAX_SPLITS = 128; // parts of a (sequence, kv head): what the combine kernel reads
 constexpr int TREE_MAX_DRAFT = 1024;
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -60,17 +60,18 @@ struct TreeArgs
     const float* kv_scale_orig_quant;
     const float* kv_scale_quant_orig;
     uint16_t* q_ws;      // [tokens][Hq][1 or 2 parts][DP]: rotated, times the score scale (and the K dequantisation) and log2(e)
-    int4* seq;           // [batch + 1]: key tiles of the sequences before this one, nodes, first row, history; [batch].x: all tiles
+    int4* seq;           // [batch + 1]: items before this sequence, nodes, first row, history; [batch].x: all items
+    int2* split;         // [batch]: parts of each of its (sequence, kv head) pairs, records before it
     int32_t* seq_ok;     // [batch]: the sequence's blocks are all there
-    int4* join;          // [teams]: the (sequence, kv head) whose first part is the team's last: first row, nodes, kv head, parts (0: none)
-    float* part_acc;     // partial states: [team][first | last stretch][m-tile][row][DP]
+    int4* join;          // [pairs_bound][2]: the pairs of several parts: first row, nodes, kv head, parts (0: none) | record, sequence
+    float* part_acc;     // partial states: [record][m-tile][row][DP]
     float2* part_ml;     // their (running maximum in the log2 domain, sum)
     int64_t qkv_stride;
     int batch, num_heads, num_kv_heads, group, hs;
     int num_tokens, max_draft, max_past, mask_words;
     int max_blocks, tpb_log2;
-    int mtiles, rows_per_wg, teams, min_chunk;
-    int whole; // a team takes one (sequence, kv head) from end to end: nothing is joined
+    int mtiles, rows_per_wg, target_items, part_tiles, items_bound, pairs_bound;
+    int whole; // every (sequence, kv head) is one item: nothing is joined
     int pos_type, rot_dim, rot_scale_type, rot_max_pos;
     double rot_log2_base, rot_scale;
     float score_scale;
@@ -88,46 +89,84 @@ __device__ __forceinline__ bool tree_seq(const TreeArgs& p, int b, int& off, int
         && keys <= ((int64_t) p.max_blocks << p.tpb_log2);
 }
 
-// the key tiles before every sequence, by one workgroup
-__device__ __forceinline__ void tree_count_tiles(const TreeArgs& p)
+// The items of the attention kernel, by one workgroup: a (sequence, kv head) pair is cut into parts of about equally many tiles, so
+// many that about target_items come out (part_tiles: the least a part should have; -1 times the most if the caller says how many)
+__device__ __forceinline__ void tree_plan_items(const TreeArgs& p)
 {
-    __shared__ int wave_sum[TREE_THREADS / 64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int carry = 0;
+    constexpr int WAVES = TREE_THREADS / 64;
+    __shared__ int wave_sum[3][WAVES];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, H = p.num_kv_heads;
+    auto tiles = [&](int b, int& off, int& n, int& past)
+    { return b < p.batch && tree_seq(p, b, off, n, past) ? (past + n + TREE_KT - 1) / TREE_KT : 0; };
+    int target = p.whole ? INT32_MAX : -p.part_tiles;
+    if (!p.whole && p.part_tiles > 0)
+    {
+        int all = 0, off, n, past;
+        for (int b = threadIdx.x; b < p.batch; b += TREE_THREADS)
+            all += tiles(b, off, n, past);
+#pragma unroll
+        for (int o = 32; o; o >>= 1)
+            all += __shfl_xor(all, o);
+        if (lane == 0)
+            wave_sum[0][wave] = all;
+        __syncthreads();
+        all = 0;
+        for (int w = 0; w < WAVES; ++w)
+            all += wave_sum[0][w];
+        target = max((all * H + p.target_items - 1) / p.target_items, p.part_tiles);
+        __syncthreads();
+    }
+    int carry[3] = {0, 0, 0}; // items, records, pairs of several parts
     for (int b0 = 0; b0 < p.batch; b0 += TREE_THREADS)
     {
         const int b = b0 + threadIdx.x;
-        int off, n, past, x = 0;
-        if (b < p.batch && tree_seq(p, b, off, n, past))
-            x = (past + n + TREE_KT - 1) / TREE_KT;
-        const int mine = x;
+        int off = 0, n = 0, past = 0;
+        const int nt = tiles(b, off, n, past);
+        int parts = 0;
+        if (nt > 0)
+            parts = p.whole ? 1 : (p.part_tiles < 0 ? (nt - 1) / target + 1 : max((2 * nt + target) / (2 * target), 1));
+        const int mine[3] = {parts * H, parts > 1 ? parts * H : 0, parts > 1 ? H : 0};
+        int x[3] = {mine[0], mine[1], mine[2]};
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1)
-        {
-            const int y = __shfl_up(x, o);
-            x += lane >= o ? y : 0;
-        }
+#pragma unroll
+            for (int i = 0; i < 3; ++i)
+            {
+                const int y = __shfl_up(x[i], o);
+                x[i] += lane >= o ? y : 0;
+            }
         if (lane == 63)
-            wave_sum[wave] = x;
+#pragma unroll
+            for (int i = 0; i < 3; ++i)
+                wave_sum[i][wave] = x[i];
         __syncthreads();
-        int before = carry;
-        for (int w = 0; w < TREE_THREADS / 64; ++w)
+        int before[3];
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
         {
-            before += w < wave ? wave_sum[w] : 0;
-            carry += wave_sum[w];
+            before[i] = carry[i] + x[i] - mine[i];
+            for (int w = 0; w < WAVES; ++w)
+            {
+                before[i] += w < wave ? wave_sum[i][w] : 0;
+                carry[i] += wave_sum[i][w];
+            }
         }
         if (b < p.batch)
-            p.seq[b] = make_int4(before + x - mine, mine ? n : 0, off, past);
+        {
+            p.seq[b] = make_int4(before[0], nt ? n : 0, off, past);
+            p.split[b] = make_int2(parts, before[1]);
+            for (int h = 0; h < (parts > 1 ? H : 0); ++h)
+            {
+                p.join[2 * (before[2] + h)] = make_int4(off, n, h, parts);
+                p.join[2 * (before[2] + h) + 1] = make_int4(before[1] + h * parts, b, 0, 0);
+            }
+        }
         __syncthreads();
     }
     if (threadIdx.x == 0)
-        p.seq[p.batch] = make_int4(carry, 0, 0, 0);
-}
-
-// tiles of a team's stretch: all (sequence, kv head, tile) units in equal parts
-__device__ __forceinline__ int tree_chunk(const TreeArgs& p, int units)
-{
-    return max((units + p.teams - 1) / p.teams, p.min_chunk);
+        p.seq[p.batch] = make_int4(carry[0], 0, 0, 0);
+    for (int i = carry[2] + threadIdx.x; i < p.pairs_bound; i += TREE_THREADS)
+        p.join[2 * i] = make_int4(0, 0, 0, 0);
 }
 
 // 8 elements from d0 on of one head of a qkv row, bias added, rotated: in fp32 or in 64 bits (R).  angle(j, c, s) gives cosine
@@ -215,7 +254,7 @@ __global__ __launch_bounds__(TREE_THREADS) void tree_prepare_kernel(TreeArgs p, 
     if (i == p.max_draft + 1)
     {
         if (b == 0 && blockIdx.z == 0)
-            tree_count_tiles(p);
+            tree_plan_items(p);
         return;
     }
     const bool ok = tree_seq(p, b, off, n, past);
@@ -421,12 +460,10 @@ __device__ __forceinline__ uint64_t tree_mask64(const uint32_t* row, int words, 
     return live >= 64 ? v : (live <= 0 ? 0ull : v & ((1ull << live) - 1));
 }
 
-// grid: 1-D, ((team / 8) * mtiles + m) * 8 + team % 8: workgroups are dealt to the 8 XCDs round-robin, so a team -- the m-tiles
-// that walk the same keys -- runs on one XCD and reads them from HBM once.
-// The keys of all sequences and kv heads, as one line of 64-key tiles, are cut into equal stretches, one per team: ragged
-// batches and single long sequences load the chip alike.  A stretch that covers a (sequence, kv head) entirely writes
-// its output; a part of one leaves its state for the combine kernel (a team has at most two such parts: its first and
-// its last).
+// grid: 1-D, ((item / 8) * mtiles + m) * 8 + item % 8: workgroups are dealt to the 8 XCDs round-robin, so the m-tiles of an item, which
+// walk the same keys, run on one XCD and read them from HBM once.
+// An item is a (sequence, kv head) pair or a part of its key tiles.  Whole pairs write their output; parts leave their state
+// for the combine kernel.
 // A workgroup = RW * QT * 16 query rows (row r = node r / G, head r % G of the kv head's G query heads).  Its 4 waves are RW row
 // groups x KW key groups: with few rows the waves share the keys of a tile instead of idling, and merge their states at
 // the end.
@@ -454,15 +491,15 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
     constexpr int RPD = 1024 / ROWB, DPW = WROWS / RPD; // 16-bit caches: rows per DMA instruction, DMAs per wave
     constexpr int CH8 = DP / 16, RPL = 64 / CH8, LPT = WROWS / RPL; // 8-bit caches: rows per 16-byte load, loads per thread
     __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE_BYTES]; // a tile that is computed, a tile that arrives
-    __shared__ uint32_t nonfinite[TREE_MAX_DRAFT / 32]; // nodes of the stretch whose V row has an infinity or NaN
+    __shared__ uint32_t nonfinite[TREE_MAX_DRAFT / 32]; // nodes whose V row has an infinity or NaN
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int rw = wave % RW, kw = wave / RW;
     const int lr = lane & 15, lq = lane >> 4;
     const int mt = (blockIdx.x >> 3) % p.mtiles;
-    const int team = (blockIdx.x >> 3) / p.mtiles * 8 + (blockIdx.x & 7);
-    if (team >= p.teams)
+    const int item = (blockIdx.x >> 3) / p.mtiles * 8 + (blockIdx.x & 7);
+    if (item >= p.items_bound)
         return;
     const int G = p.group, hs = p.hs, tpb_mask = (1 << p.tpb_log2) - 1;
     const int row_bytes = hs * (KVT ? 1 : 2); // of a head in the cache
@@ -477,58 +514,39 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
         return CH >= 16 ? (row & 3) << 2 | ((x ^ x >> 1) & 1) << 1 | (x >> 1 ^ (row & 1)) : ((row >> 1) & 3) << 1;
     };
 
-    // ---- the team's stretch of units (sequence, kv head, tile).  A lane holds the record of one of 64 sequences; the one at work
-    // is a lane read away
-    int4 join = make_int4(0, 0, 0, 0);
-    int chunk = 0, unit = 0; // unit: the stretch's first one still to do
-    int b = 0, hk = 0, tile = 0, left, b0; // left: tiles of the stretch still to do; b0: the first sequence in the lanes
-    int4 info;
-    int info_next, info_ok;
-    auto fetch_info = [&](int first)
-    {
-        b0 = first;
-        info = p.seq[min(first + lane, p.batch)];
-        info_next = p.seq[min(first + lane + 1, p.batch)].x;
-        info_ok = p.seq_ok[min(first + lane, p.batch - 1)];
-    };
+    // ---- the item's sequence.  64 lanes look at the items before 64 sequences (or before every len / 64th of more)
+    int b0 = 0;
     if (p.whole)
-    {
-        b = team / p.num_kv_heads;
-        hk = team % p.num_kv_heads;
-        fetch_info(b & ~63);
-        left = INT32_MAX;
-    }
+        b0 = item / p.num_kv_heads & ~63;
     else
-    {
-        fetch_info(0);
-        const int units = p.seq[p.batch].x * p.num_kv_heads;
-        chunk = tree_chunk(p, units);
-        const int64_t u0 = (int64_t) team * chunk;
-        left = (int) min((int64_t) chunk, units - u0);
-        if (left <= 0)
+        for (int len = p.batch; len > 64;)
         {
-            if (mt == 0 && tid == 0)
-                p.join[team] = join;
-            return;
+            const int step = (len + 63) / 64;
+            const int at = b0 + (lane + 1) * step;
+            b0 += step * __builtin_popcountll(__ballot(at < p.batch && p.seq[min(at, p.batch)].x <= item));
+            len = step;
         }
-        unit = (int) u0;
-        const int at = unit / p.num_kv_heads; // the sequences that end at or before this tile
-        for (;;)
-        {
-            const uint64_t done = __ballot(b0 + lane < p.batch && info_next <= at);
-            b = b0 + __builtin_popcountll(done);
-            if (done != ~0ull)
-                break;
-            fetch_info(b0 + 64);
-        }
-        b = __builtin_amdgcn_readfirstlane(b);
-        const int start = __builtin_amdgcn_readlane(info.x, b - b0), nt = __builtin_amdgcn_readlane(info_next, b - b0) - start;
-        const int in_seq = unit - start * p.num_kv_heads;
-        hk = in_seq / nt;
-        tile = in_seq % nt;
-    }
+    const int4 info = p.seq[min(b0 + lane, p.batch)];
+    const int info_next = p.seq[min(b0 + lane + 1, p.batch)].x;
+    const int2 info_split = p.split[min(b0 + lane, p.batch - 1)];
+    const int info_ok = p.seq_ok[min(b0 + lane, p.batch - 1)];
+    const int at = __builtin_amdgcn_readfirstlane(
+        p.whole ? item / p.num_kv_heads - b0 : __builtin_popcountll(__ballot(b0 + lane < p.batch && info_next <= item)));
+    if (b0 + at >= p.batch) // behind the last item
+        return;
+    const int b = b0 + at, n = __builtin_amdgcn_readlane(info_ok, at) ? __builtin_amdgcn_readlane(info.y, at) : 0;
+    if (mt * M >= n * G) // an empty sequence, one that is skipped, or no rows for this m-tile
+        return;
+    const int off = __builtin_amdgcn_readlane(info.z, at), past = __builtin_amdgcn_readlane(info.w, at), total = past + n;
+    const int nt = (total + TREE_KT - 1) / TREE_KT, parts = __builtin_amdgcn_readlane(info_split.x, at);
+    const int in_seq = p.whole ? item % p.num_kv_heads : item - __builtin_amdgcn_readlane(info.x, at);
+    const int head_kv = in_seq / parts, part_no = in_seq % parts;
+    const int tile_lo = nt / parts * part_no + min(part_no, nt % parts), tile_hi = tile_lo + nt / parts + (part_no < nt % parts);
+    const int64_t* const kp = p.block_ptrs + (size_t) b * 2 * p.max_blocks;
+    const int64_t* const vp = kp + p.max_blocks;
+    const bool long_tree = n > 64;
 
-    // ---- what does not change from stretch to stretch
+    // ---- LDS and cache offsets
     const uint32_t lds_base = __builtin_amdgcn_readfirstlane((uint32_t) (uintptr_t) (ctx_lds_void_t*) lds);
     const int last_chunk = row_bytes / 16 - 1; // heads narrower than DP: the padding re-reads the last chunk (q is 0 there)
     constexpr int LOADS = KVT ? LPT : DPW;
@@ -547,504 +565,470 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
     const uint32_t v_addr = lds_base + TILE_BYTES + ROWB * (kb0 + 4 * lq + rq) + 16 * ((rp >> 1) ^ sw(4 * lq + rq)) + 8 * (rp & 1);
     typedef const __attribute__((address_space(4))) int64_t* scalar_ptr;
 
-    while (left > 0)
+    // ---- tile loads.  A wave loads 16 consecutive keys, which lie in one block (tokens_per_block >= 16): the block's address
+    // is a scalar load, issued a tile ahead, and a lane adds a fixed 32-bit offset.  16-bit caches: LDS-DMA, instruction d of
+    // a tile fills LDS bytes [1024 d, +1024), the swizzle applied on the source address.  8-bit caches: through registers,
+    // converted on the way into the LDS.  Keys past the sequence are whatever its last block holds there.
+    int64_t kbase = 0, vbase = 0; // where the wave's 16 keys of the tile to be loaded next begin
+    auto find_tile = [&](int i)
     {
-        if (b >= b0 + 64)
-            fetch_info(b);
-        const int at = b - b0, seq = b, head_kv = hk;
-        const int nt = __builtin_amdgcn_readlane(info_next, at) - __builtin_amdgcn_readlane(info.x, at);
-        const int tile_lo = tile, tile_hi = min(nt, left < INT32_MAX - nt ? tile + left : nt);
-        const int unit0 = unit;
-        left -= tile_hi - tile_lo;
-        unit += tile_hi - tile_lo;
-        tile = 0;
-        if (p.whole)
-            left = 0;
-        else if (++hk == p.num_kv_heads)
-        {
-            hk = 0;
-            ++b;
-        }
-        const int n = __builtin_amdgcn_readlane(info_ok, at) ? __builtin_amdgcn_readlane(info.y, at) : 0;
-        if (tile_hi <= tile_lo || mt * M >= n * G) // an empty sequence, one that is skipped, or no rows for this m-tile
-            continue;
-        const int off = __builtin_amdgcn_readlane(info.z, at), past = __builtin_amdgcn_readlane(info.w, at), total = past + n;
-        if (!p.whole && tile_lo == 0 && tile_hi < nt)
-            join = make_int4(off, n, head_kv, (unit0 + nt - 1) / chunk - team + 1);
-        const int64_t* const kp = p.block_ptrs + (size_t) seq * 2 * p.max_blocks;
-        const int64_t* const vp = kp + p.max_blocks;
-
-        // ---- tile loads.  A wave loads 16 consecutive keys, which lie in one block (tokens_per_block >= 16): the block's address
-        // is a scalar load, issued a tile ahead, and a lane adds a fixed 32-bit offset.  16-bit caches: LDS-DMA, instruction d of
-        // a tile fills LDS bytes [1024 d, +1024), the swizzle applied on the source address.  8-bit caches: through registers,
-        // converted on the way into the LDS.  Keys past the sequence are whatever its last block holds there.
-        int64_t kbase = 0, vbase = 0; // where the wave's 16 keys of the tile to be loaded next begin
-        auto find_tile = [&](int i)
-        {
-            const int t0 = i * TREE_KT + wave * WROWS;
-            const int blk = __builtin_amdgcn_readfirstlane(min(t0, total - 1) >> p.tpb_log2);
-            const int64_t in_block = (((int64_t) head_kv << p.tpb_log2) + (t0 & tpb_mask)) * row_bytes;
-            kbase = ((scalar_ptr) kp)[blk] + in_block;
-            vbase = ((scalar_ptr) vp)[blk] + in_block;
-        };
-        uint4 kreg[KVT ? LPT : 1], vreg[KVT ? LPT : 1];
-        auto load_tile = [&](uint32_t stage)
-        {
+        const int t0 = i * TREE_KT + wave * WROWS;
+        const int blk = __builtin_amdgcn_readfirstlane(min(t0, total - 1) >> p.tpb_log2);
+        const int64_t in_block = (((int64_t) head_kv << p.tpb_log2) + (t0 & tpb_mask)) * row_bytes;
+        kbase = ((scalar_ptr) kp)[blk] + in_block;
+        vbase = ((scalar_ptr) vp)[blk] + in_block;
+    };
+    uint4 kreg[KVT ? LPT : 1], vreg[KVT ? LPT : 1];
+    auto load_tile = [&](uint32_t stage)
+    {
 #pragma unroll
-            for (int d = 0; d < LOADS; ++d)
+        for (int d = 0; d < LOADS; ++d)
+        {
+            if constexpr (KVT == 0)
             {
-                if constexpr (KVT == 0)
-                {
-                    const uint32_t dst = lds_base + stage + (wave * DPW + d) * 1024;
-                    tree_dma16(kbase, lane_off[d], dst);
-                    tree_dma16(vbase, lane_off[d], dst + TILE_BYTES);
-                }
-                else
-                {
-                    kreg[d] = tree_load16(kbase + lane_off[d]);
-                    vreg[d] = tree_load16(vbase + lane_off[d]);
-                }
+                const uint32_t dst = lds_base + stage + (wave * DPW + d) * 1024;
+                tree_dma16(kbase, lane_off[d], dst);
+                tree_dma16(vbase, lane_off[d], dst + TILE_BYTES);
             }
-        };
-        auto store_tile = [&](uint32_t stage) // 8-bit caches
-        {
-            if constexpr (KVT != 0)
+            else
             {
-#pragma unroll
-                for (int d = 0; d < LPT; ++d)
-                {
-                    const int r = d * RPL + lane / CH8, ch = 2 * (lane % CH8);
-                    uint8_t* kt = lds + stage + ROWB * (wave * WROWS + r);
-                    uint8_t* vt = kt + TILE_BYTES;
-                    *reinterpret_cast<uint4*>(kt + 16 * (ch ^ sw(r))) = tree_kv8_to_f16<KVT>(kreg[d].x, kreg[d].y);
-                    *reinterpret_cast<uint4*>(kt + 16 * ((ch + 1) ^ sw(r))) = tree_kv8_to_f16<KVT>(kreg[d].z, kreg[d].w);
-                    *reinterpret_cast<uint4*>(vt + 16 * (ch ^ sw(r))) = tree_kv8_to_f16<KVT>(vreg[d].x, vreg[d].y);
-                    *reinterpret_cast<uint4*>(vt + 16 * ((ch + 1) ^ sw(r))) = tree_kv8_to_f16<KVT>(vreg[d].z, vreg[d].w);
-                }
+                kreg[d] = tree_load16(kbase + lane_off[d]);
+                vreg[d] = tree_load16(vbase + lane_off[d]);
             }
-        };
-
-        __syncthreads(); // everyone is done with the LDS of the stretch before
-        if (KVT == 0 && tid < TREE_MAX_DRAFT / 32)
-            nonfinite[tid] = 0; // (the barrier of the first tile comes before the first use)
-        find_tile(tile_lo);
-        load_tile(0);
-        find_tile(min(tile_lo + 1, tile_hi - 1));
-        // ---- Q^T fragments (B operand): column = row q0 + 16 qt + lr, k = d = 32 ks + 8 lq + j
-        const int q0 = mt * M + rw * QT * 16;
-        uint4 qf[PARTS][QT][KS];
-        uint64_t mask_row[QT]; // the first 64 nodes' bits
-        const bool long_tree = n > 64;
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt)
-        {
-            const int r = min(q0 + 16 * qt + lr, n * G - 1); // rows past the last re-read it; never stored
-            const uint32_t* mrow = p.tree_mask + (size_t) (off + r / G) * p.mask_words;
-            mask_row[qt] = (uint64_t) mrow[p.mask_words > 1 ? 1 : 0] << 32 | mrow[0];
-            if (n < 64)
-                mask_row[qt] &= (1ull << n) - 1;
-            const uint16_t* q = p.q_ws + ((size_t) (off + r / G) * p.num_heads + head_kv * G + r % G) * PARTS * DP;
-#pragma unroll
-            for (int part = 0; part < PARTS; ++part)
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks)
-                    qf[part][qt][ks] = *reinterpret_cast<const uint4*>(q + part * DP + 32 * ks + 8 * lq);
         }
-        // end the compiler's own bookkeeping of these loads here, before the loop's (to it invisible) DMAs
+    };
+    auto store_tile = [&](uint32_t stage) // 8-bit caches
+    {
+        if constexpr (KVT != 0)
+        {
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt)
-            asm volatile("" : "+v"(mask_row[qt]));
+            for (int d = 0; d < LPT; ++d)
+            {
+                const int r = d * RPL + lane / CH8, ch = 2 * (lane % CH8);
+                uint8_t* kt = lds + stage + ROWB * (wave * WROWS + r);
+                uint8_t* vt = kt + TILE_BYTES;
+                *reinterpret_cast<uint4*>(kt + 16 * (ch ^ sw(r))) = tree_kv8_to_f16<KVT>(kreg[d].x, kreg[d].y);
+                *reinterpret_cast<uint4*>(kt + 16 * ((ch + 1) ^ sw(r))) = tree_kv8_to_f16<KVT>(kreg[d].z, kreg[d].w);
+                *reinterpret_cast<uint4*>(vt + 16 * (ch ^ sw(r))) = tree_kv8_to_f16<KVT>(vreg[d].x, vreg[d].y);
+                *reinterpret_cast<uint4*>(vt + 16 * ((ch + 1) ^ sw(r))) = tree_kv8_to_f16<KVT>(vreg[d].z, vreg[d].w);
+            }
+        }
+    };
+
+    if (KVT == 0 && tid < TREE_MAX_DRAFT / 32)
+        nonfinite[tid] = 0; // (the barrier of the first tile comes before the first use)
+    find_tile(tile_lo);
+    load_tile(0);
+    find_tile(min(tile_lo + 1, tile_hi - 1));
+    // ---- Q^T fragments (B operand): column = row q0 + 16 qt + lr, k = d = 32 ks + 8 lq + j
+    const int q0 = mt * M + rw * QT * 16;
+    uint4 qf[PARTS][QT][KS];
+    uint64_t mask_row[QT]; // the first 64 nodes' bits
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt)
+    {
+        const int r = min(q0 + 16 * qt + lr, n * G - 1); // rows past the last re-read it; never stored
+        const uint32_t* mrow = p.tree_mask + (size_t) (off + r / G) * p.mask_words;
+        mask_row[qt] = (uint64_t) mrow[p.mask_words > 1 ? 1 : 0] << 32 | mrow[0];
+        if (n < 64)
+            mask_row[qt] &= (1ull << n) - 1;
+        const uint16_t* q = p.q_ws + ((size_t) (off + r / G) * p.num_heads + head_kv * G + r % G) * PARTS * DP;
 #pragma unroll
         for (int part = 0; part < PARTS; ++part)
 #pragma unroll
-            for (int qt = 0; qt < QT; ++qt)
+            for (int ks = 0; ks < KS; ++ks)
+                qf[part][qt][ks] = *reinterpret_cast<const uint4*>(q + part * DP + 32 * ks + 8 * lq);
+    }
+    // end the compiler's own bookkeeping of these loads here, before the loop's (to it invisible) DMAs
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks)
-                    asm volatile("" : "+v"(qf[part][qt][ks].x), "+v"(qf[part][qt][ks].y), "+v"(qf[part][qt][ks].z), "+v"(qf[part][qt][ks].w));
+    for (int qt = 0; qt < QT; ++qt)
+        asm volatile("" : "+v"(mask_row[qt]));
+#pragma unroll
+    for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+                asm volatile("" : "+v"(qf[part][qt][ks].x), "+v"(qf[part][qt][ks].y), "+v"(qf[part][qt][ks].z), "+v"(qf[part][qt][ks].w));
 
-        float l_run[QT];
-        cf32x4_t minus_m[QT]; // C operand of the scores: minus the running maximum
-        bool fresh[QT];       // the column has no maximum yet (minus_m is 0)
-        cf32x4_t o[QT][DT];
+    float l_run[QT];
+    cf32x4_t minus_m[QT]; // C operand of the scores: minus the running maximum
+    bool fresh[QT];       // the column has no maximum yet (minus_m is 0)
+    cf32x4_t o[QT][DT];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt)
+    {
+        fresh[qt] = true;
+        l_run[qt] = 0.f;
+        minus_m[qt] = cf32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+            o[qt][dt] = cf32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // One compute step: X2 subtiles from key `kb` of the tile in `stage` on.  GENERAL: columns may still be fresh, keys hidden.
+    auto step = [&](auto general, uint32_t stage, int kb, int t0)
+    {
+        constexpr bool GENERAL = decltype(general)::value;
+        const uint32_t ka = k_addr + stage + kb * ROWB, va = v_addr + stage + kb * ROWB;
+        cf32x4_t s[X2][QT];
+#pragma unroll
+        for (int x = 0; x < X2; ++x)
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt)
+                s[x][qt] = minus_m[qt];
+#pragma unroll
+        for (int ks0 = 0; ks0 < KS; ks0 += KBATCH)
+        {
+            uint4 kf[KBATCH][X2];
+#pragma unroll
+            for (int ks = 0; ks < KBATCH; ++ks)
+#pragma unroll
+                for (int x = 0; x < X2; ++x)
+                    kf[ks][x] = tree_lds16((ka ^ (64 * (ks0 + ks))) + 16 * x * ROWB);
+#pragma unroll
+            for (int ks = 0; ks < KBATCH; ++ks)
+#pragma unroll
+                for (int part = PARTS - 1; part >= 0; --part)
+#pragma unroll
+                    for (int x = 0; x < X2; ++x) // consecutive products go to different accumulators
+#pragma unroll
+                        for (int qt = 0; qt < QT; ++qt)
+                            s[x][qt] = ctx_mfma<C>(kf[ks][x], qf[part][qt][ks0 + ks], s[x][qt]);
+        }
+        // the first V fragments are read while the softmax runs
+        uint2 vf[VBATCH][X2];
+        auto read_v = [&](int d0)
+        {
+#pragma unroll
+            for (int dt = 0; dt < VBATCH; ++dt)
+#pragma unroll
+                for (int x = 0; x < X2; ++x)
+                    vf[dt][x] = __builtin_bit_cast(uint2,
+                        __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_cs16x4_t*) (uintptr_t) ((va ^ (32 * (d0 + dt))) + 16 * x * ROWB)));
+        };
+        read_v(0);
+        __builtin_amdgcn_sched_barrier(0);
+        if (GENERAL && t0 + TREE_KT > past)
+        {
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt)
+            {
+                const int s0 = t0 - past; // > -64
+                uint64_t seen;
+                if (long_tree) // uniform
+                {
+                    const int node = min(q0 + 16 * qt + lr, n * G - 1) / G;
+                    seen = tree_mask64(p.tree_mask + (size_t) (off + node) * p.mask_words, p.mask_words, n, s0);
+                }
+                else // the history's keys are seen
+                    seen = s0 < 0 ? mask_row[qt] << -s0 | ((1ull << -s0) - 1) : (s0 < 64 ? mask_row[qt] >> s0 : 0);
+                seen >>= kb0 + kb + 4 * lq;
+#pragma unroll
+                for (int x = 0; x < X2; ++x)
+#pragma unroll
+                    for (int rr = 0; rr < 4; ++rr)
+                        s[x][qt][rr] = (seen >> (16 * x + rr)) & 1 ? s[x][qt][rr] : -__builtin_inff();
+            }
+        }
+        uint32_t pk[QT][X2][2];
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt)
         {
-            fresh[qt] = true;
-            l_run[qt] = 0.f;
-            minus_m[qt] = cf32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
-                o[qt][dt] = cf32x4_t{0.f, 0.f, 0.f, 0.f};
-        }
-
-        // One compute step: X2 subtiles from key `kb` of the tile in `stage` on.  GENERAL: columns may still be fresh, keys hidden.
-        auto step = [&](auto general, uint32_t stage, int kb, int t0)
-        {
-            constexpr bool GENERAL = decltype(general)::value;
-            const uint32_t ka = k_addr + stage + kb * ROWB, va = v_addr + stage + kb * ROWB;
-            cf32x4_t s[X2][QT];
+            int mx = 0; // the largest positive s - m, as raw bits
 #pragma unroll
             for (int x = 0; x < X2; ++x)
 #pragma unroll
-                for (int qt = 0; qt < QT; ++qt)
-                    s[x][qt] = minus_m[qt];
-#pragma unroll
-            for (int ks0 = 0; ks0 < KS; ks0 += KBATCH)
+                for (int rr = 0; rr < 4; ++rr)
+                    mx = max(mx, __builtin_bit_cast(int, (float) s[x][qt][rr]));
+            const bool first = GENERAL && fresh[qt];
+            if (__any(first || mx > 0x41000000 /* 8.0f */)) // wave-uniform
             {
-                uint4 kf[KBATCH][X2];
-#pragma unroll
-                for (int ks = 0; ks < KBATCH; ++ks)
-#pragma unroll
-                    for (int x = 0; x < X2; ++x)
-                        kf[ks][x] = tree_lds16((ka ^ (64 * (ks0 + ks))) + 16 * x * ROWB);
-#pragma unroll
-                for (int ks = 0; ks < KBATCH; ++ks)
-#pragma unroll
-                    for (int part = PARTS - 1; part >= 0; --part)
-#pragma unroll
-                        for (int x = 0; x < X2; ++x) // consecutive products go to different accumulators
-#pragma unroll
-                            for (int qt = 0; qt < QT; ++qt)
-                                s[x][qt] = ctx_mfma<C>(kf[ks][x], qf[part][qt][ks0 + ks], s[x][qt]);
-            }
-            // the first V fragments are read while the softmax runs
-            uint2 vf[VBATCH][X2];
-            auto read_v = [&](int d0)
-            {
-#pragma unroll
-                for (int dt = 0; dt < VBATCH; ++dt)
-#pragma unroll
-                    for (int x = 0; x < X2; ++x)
-                        vf[dt][x] = __builtin_bit_cast(uint2,
-                            __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_cs16x4_t*) (uintptr_t) ((va ^ (32 * (d0 + dt))) + 16 * x * ROWB)));
-            };
-            read_v(0);
-            __builtin_amdgcn_sched_barrier(0);
-            if (GENERAL && t0 + TREE_KT > past)
-            {
-#pragma unroll
-                for (int qt = 0; qt < QT; ++qt)
-                {
-                    const int s0 = t0 - past; // > -64
-                    uint64_t seen;
-                    if (long_tree) // uniform
-                    {
-                        const int node = min(q0 + 16 * qt + lr, n * G - 1) / G;
-                        seen = tree_mask64(p.tree_mask + (size_t) (off + node) * p.mask_words, p.mask_words, n, s0);
-                    }
-                    else // the history's keys are seen
-                        seen = s0 < 0 ? mask_row[qt] << -s0 | ((1ull << -s0) - 1) : (s0 < 64 ? mask_row[qt] >> s0 : 0);
-                    seen >>= kb0 + kb + 4 * lq;
-#pragma unroll
-                    for (int x = 0; x < X2; ++x)
-#pragma unroll
-                        for (int rr = 0; rr < 4; ++rr)
-                            s[x][qt][rr] = (seen >> (16 * x + rr)) & 1 ? s[x][qt][rr] : -__builtin_inff();
-                }
-            }
-            uint32_t pk[QT][X2][2];
-#pragma unroll
-            for (int qt = 0; qt < QT; ++qt)
-            {
-                int mx = 0; // the largest positive s - m, as raw bits
+                // the column's maximum of these keys, over its 4 lanes (a NaN stays out of the comparison and in the scores)
+                float top = -__builtin_inff();
 #pragma unroll
                 for (int x = 0; x < X2; ++x)
 #pragma unroll
                     for (int rr = 0; rr < 4; ++rr)
-                        mx = max(mx, __builtin_bit_cast(int, (float) s[x][qt][rr]));
-                const bool first = GENERAL && fresh[qt];
-                if (__any(first || mx > 0x41000000 /* 8.0f */)) // wave-uniform
+                        top = fmaxf(top, s[x][qt][rr]);
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                if (top != -__builtin_inff())
                 {
-                    // the column's maximum of these keys, over its 4 lanes (a NaN stays out of the comparison and in the scores)
-                    float top = -__builtin_inff();
+                    const float up = first ? top : fmaxf(top, 0.f);
+                    const float corr = first ? 0.f : __builtin_amdgcn_exp2f(-up); // (nothing was summed before the first maximum)
+                    const float mm = minus_m[qt][0] - up;
+                    minus_m[qt] = cf32x4_t{mm, mm, mm, mm};
+                    if constexpr (GENERAL)
+                        fresh[qt] = false;
+                    l_run[qt] *= corr;
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                        for (int rr = 0; rr < 4; ++rr)
+                            o[qt][dt][rr] *= corr;
 #pragma unroll
                     for (int x = 0; x < X2; ++x)
 #pragma unroll
                         for (int rr = 0; rr < 4; ++rr)
-                            top = fmaxf(top, s[x][qt][rr]);
-                    top = fmaxf(top, __shfl_xor(top, 16));
-                    top = fmaxf(top, __shfl_xor(top, 32));
-                    if (top != -__builtin_inff())
-                    {
-                        const float up = first ? top : fmaxf(top, 0.f);
-                        const float corr = first ? 0.f : __builtin_amdgcn_exp2f(-up); // (nothing was summed before the first maximum)
-                        const float mm = minus_m[qt][0] - up;
-                        minus_m[qt] = cf32x4_t{mm, mm, mm, mm};
-                        if constexpr (GENERAL)
-                            fresh[qt] = false;
-                        l_run[qt] *= corr;
-#pragma unroll
-                        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                            for (int rr = 0; rr < 4; ++rr)
-                                o[qt][dt][rr] *= corr;
-#pragma unroll
-                        for (int x = 0; x < X2; ++x)
-#pragma unroll
-                            for (int rr = 0; rr < 4; ++rr)
-                                s[x][qt][rr] -= up;
-                    }
+                            s[x][qt][rr] -= up;
                 }
+            }
 #pragma unroll
-                for (int x = 0; x < X2; ++x)
+            for (int x = 0; x < X2; ++x)
+            {
+                float e[4];
+#pragma unroll
+                for (int rr = 0; rr < 4; ++rr)
                 {
-                    float e[4];
-#pragma unroll
-                    for (int rr = 0; rr < 4; ++rr)
-                    {
-                        e[rr] = __builtin_amdgcn_exp2f(s[x][qt][rr]);
-                        l_run[qt] += e[rr];
-                    }
-                    // P in the compute type: its rounding (half a step, relative) averages out over the keys
-                    pk[qt][x][0] = pack2<C>(e[0], e[1]);
-                    pk[qt][x][1] = pack2<C>(e[2], e[3]);
+                    e[rr] = __builtin_amdgcn_exp2f(s[x][qt][rr]);
+                    l_run[qt] += e[rr];
                 }
+                // P in the compute type: its rounding (half a step, relative) averages out over the keys
+                pk[qt][x][0] = pack2<C>(e[0], e[1]);
+                pk[qt][x][1] = pack2<C>(e[2], e[3]);
             }
-            // ---- O^T += V^T . P^T  (A operand rows d = 16 dt + lr by the transposing LDS read)
+        }
+        // ---- O^T += V^T . P^T  (A operand rows d = 16 dt + lr by the transposing LDS read)
 #pragma unroll
-            for (int d0 = 0; d0 < DT; d0 += VBATCH)
-            {
-                if (d0)
-                    read_v(d0);
+        for (int d0 = 0; d0 < DT; d0 += VBATCH)
+        {
+            if (d0)
+                read_v(d0);
 #pragma unroll
-                for (int dt = 0; dt < VBATCH; ++dt)
-#pragma unroll
-                    for (int qt = 0; qt < QT; ++qt)
-                    {
-                        if constexpr (X2 == 2)
-                            o[qt][d0 + dt] = ctx_mfma<C>(make_uint4(vf[dt][0].x, vf[dt][0].y, vf[dt][X2 - 1].x, vf[dt][X2 - 1].y),
-                                make_uint4(pk[qt][0][0], pk[qt][0][1], pk[qt][X2 - 1][0], pk[qt][X2 - 1][1]), o[qt][d0 + dt]);
-                        else
-                            o[qt][d0 + dt] = tree_mfma16<C>(vf[dt][0], make_uint2(pk[qt][0][0], pk[qt][0][1]), o[qt][d0 + dt]);
-                    }
-            }
-        };
-        // V rows of a tile with nodes, in the LDS: rows past the sequence are zeroed (whatever lies there, 0 * NaN is NaN), and so
-        // are nodes' elements that are not finite, which must not reach the columns that do not see them; the others get them
-        // at the end.  History rows are seen by every column and stay as they are.
-        auto clean_tail = [&](uint32_t stage, int t0)
-        {
-            for (int c = max(past - t0, 0) * CH + tid; c < TREE_KT * CH; c += TREE_THREADS)
-            {
-                const int row = c / CH, t = t0 + row;
-                uint4* at = reinterpret_cast<uint4*>(lds + stage + TILE_BYTES + 16 * c);
-                if (t >= total)
-                    *at = make_uint4(0, 0, 0, 0);
-                else if (KVT == 0 && t >= past)
-                {
-                    uint4 w = *at;
-                    uint32_t* x = reinterpret_cast<uint32_t*>(&w);
-                    if (tree_nonfinite2<T>(x[0]) || tree_nonfinite2<T>(x[1]) || tree_nonfinite2<T>(x[2]) || tree_nonfinite2<T>(x[3]))
-                    {
-                        constexpr uint32_t EXP = T16<T>::is_bf16 ? 0x7f80u : 0x7c00u;
-                        for (int e = 0; e < 4; ++e)
-                        {
-                            if ((x[e] & EXP) == EXP)
-                                x[e] &= 0xffff0000u;
-                            if (((x[e] >> 16) & EXP) == EXP)
-                                x[e] &= 0xffffu;
-                        }
-                        *at = w;
-                        atomicOr(&nonfinite[(t - past) >> 5], 1u << ((t - past) & 31));
-                    }
-                }
-            }
-            __syncthreads();
-        };
-
-        if constexpr (KVT != 0)
-            store_tile(0);
-        uint32_t stage = 0; // of the tile that is computed
-        int i = tile_lo;
-        auto enter_tile = [&]()
-        {
-            if constexpr (KVT == 0)
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // my share of tile i has landed
-            __syncthreads();                                     // everyone's has, and everyone is done with tile i - 1
-            if (i + 1 < tile_hi)
-            {
-                load_tile(STAGE_BYTES - stage);
-                find_tile(min(i + 2, tile_hi - 1));
-            }
-        };
-        auto leave_tile = [&]()
-        {
-            stage = STAGE_BYTES - stage;
-            ++i;
-            if constexpr (KVT != 0)
-            {
-                if (i < tile_hi)
-                    store_tile(stage);
-            }
-        };
-        // the first tile and the tiles with nodes go through the general step, the history's others through the short one
-        // (with few rows one copy of the step: fetching code costs more there than a mask test)
-        const bool has_rows = q0 < n * G; // a wave without rows (a smaller tree than the largest) only loads
-        const int plain_end = KW == 1 ? min(tile_hi, past / TREE_KT) : 0;
-        while (i < tile_hi)
-        {
-            enter_tile();
-            const int t0 = i * TREE_KT;
-            if (t0 + TREE_KT > past)
-                clean_tail(stage, t0);
-#pragma unroll 1
-            for (int kb = has_rows ? 0 : 16 * XW; kb < 16 * XW; kb += 16 * X2)
-                step(std::true_type{}, stage, kb, t0);
-            leave_tile();
-            if constexpr (KW == 1)
-            {
-                // (scores of -inf only, of an overflow in fp32: the column has no maximum yet, the general step goes on)
-                bool open = false;
+            for (int dt = 0; dt < VBATCH; ++dt)
 #pragma unroll
                 for (int qt = 0; qt < QT; ++qt)
-                    open |= fresh[qt];
-                const bool settled = !__any(open);
-                while (settled && i < plain_end)
                 {
-                    enter_tile();
-#pragma unroll 1
-                    for (int kb = 0; kb < 16 * XW; kb += 16 * X2)
-                        step(std::false_type{}, stage, kb, 0);
-                    leave_tile();
+                    if constexpr (X2 == 2)
+                        o[qt][d0 + dt] = ctx_mfma<C>(make_uint4(vf[dt][0].x, vf[dt][0].y, vf[dt][X2 - 1].x, vf[dt][X2 - 1].y),
+                            make_uint4(pk[qt][0][0], pk[qt][0][1], pk[qt][X2 - 1][0], pk[qt][X2 - 1][1]), o[qt][d0 + dt]);
+                    else
+                        o[qt][d0 + dt] = tree_mfma16<C>(vf[dt][0], make_uint2(pk[qt][0][0], pk[qt][0][1]), o[qt][d0 + dt]);
+                }
+        }
+    };
+    // V rows of a tile with nodes, in the LDS: rows past the sequence are zeroed (whatever lies there, 0 * NaN is NaN), and so
+    // are nodes' elements that are not finite, which must not reach the columns that do not see them; the others get them
+    // at the end.  History rows are seen by every column and stay as they are.
+    auto clean_tail = [&](uint32_t stage, int t0)
+    {
+        for (int c = max(past - t0, 0) * CH + tid; c < TREE_KT * CH; c += TREE_THREADS)
+        {
+            const int row = c / CH, t = t0 + row;
+            uint4* at = reinterpret_cast<uint4*>(lds + stage + TILE_BYTES + 16 * c);
+            if (t >= total)
+                *at = make_uint4(0, 0, 0, 0);
+            else if (KVT == 0 && t >= past)
+            {
+                uint4 w = *at;
+                uint32_t* x = reinterpret_cast<uint32_t*>(&w);
+                if (tree_nonfinite2<T>(x[0]) || tree_nonfinite2<T>(x[1]) || tree_nonfinite2<T>(x[2]) || tree_nonfinite2<T>(x[3]))
+                {
+                    constexpr uint32_t EXP = T16<T>::is_bf16 ? 0x7f80u : 0x7c00u;
+                    for (int e = 0; e < 4; ++e)
+                    {
+                        if ((x[e] & EXP) == EXP)
+                            x[e] &= 0xffff0000u;
+                        if (((x[e] >> 16) & EXP) == EXP)
+                            x[e] &= 0xffffu;
+                    }
+                    *at = w;
+                    atomicOr(&nonfinite[(t - past) >> 5], 1u << ((t - past) & 31));
                 }
             }
         }
+        __syncthreads();
+    };
 
-        // ---- the end of the stretch: the sum over the 4 lanes of a column; the states of the KW key groups meet in the LDS, and
-        // each of their waves joins and stores its share of the output columns
-        constexpr int DTW = DT / KW;
-        const int dt0 = kw * DTW;
-        bool any_nonfinite = false;
+    if constexpr (KVT != 0)
+        store_tile(0);
+    uint32_t stage = 0; // of the tile that is computed
+    int i = tile_lo;
+    auto enter_tile = [&]()
+    {
         if constexpr (KVT == 0)
-            for (int w = 0; w < (n + 31) >> 5; ++w)
-                any_nonfinite |= nonfinite[w] != 0;
-        const bool alone = tile_lo == 0 && tile_hi == nt; // nothing of this (sequence, kv head) is elsewhere
-        const float v_deq = KVT ? p.kv_scale_quant_orig[0] : 1.f;
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt)
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // my share of tile i has landed
+        __syncthreads();                                     // everyone's has, and everyone is done with tile i - 1
+        if (i + 1 < tile_hi)
         {
-            float m = fresh[qt] ? NEG_BIG : -minus_m[qt][0], l = l_run[qt];
-            l += __shfl_xor(l, 16);
-            l += __shfl_xor(l, 32);
-            cf32x4_t acc[DTW];
-            if constexpr (KW == 1)
+            load_tile(STAGE_BYTES - stage);
+            find_tile(min(i + 2, tile_hi - 1));
+        }
+    };
+    auto leave_tile = [&]()
+    {
+        stage = STAGE_BYTES - stage;
+        ++i;
+        if constexpr (KVT != 0)
+        {
+            if (i < tile_hi)
+                store_tile(stage);
+        }
+    };
+    // the first tile and the tiles with nodes go through the general step, the history's others through the short one
+    // (with few rows one copy of the step: fetching code costs more there than a mask test)
+    const bool has_rows = q0 < n * G; // a wave without rows (a smaller tree than the largest) only loads
+    const int plain_end = KW == 1 ? min(tile_hi, past / TREE_KT) : 0;
+    while (i < tile_hi)
+    {
+        enter_tile();
+        const int t0 = i * TREE_KT;
+        if (t0 + TREE_KT > past)
+            clean_tail(stage, t0);
+#pragma unroll 1
+        for (int kb = has_rows ? 0 : 16 * XW; kb < 16 * XW; kb += 16 * X2)
+            step(std::true_type{}, stage, kb, t0);
+        leave_tile();
+        if constexpr (KW == 1)
+        {
+            // (scores of -inf only, of an overflow in fp32: the column has no maximum yet, the general step goes on)
+            bool open = false;
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt)
+                open |= fresh[qt];
+            const bool settled = !__any(open);
+            while (settled && i < plain_end)
             {
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
-                    acc[dt] = o[qt][dt];
-            }
-            else
-            {
-                constexpr int STATE = (DT + 1) * 64 * 16; // bytes of one wave's state: float4 per register group and lane
-                static_assert(4 * STATE <= 2 * STAGE_BYTES, "states do not fit the tile buffers");
-                __syncthreads(); // everyone is done with the tiles, or with the states before
-                cf32x4_t* st = reinterpret_cast<cf32x4_t*>(lds + wave * STATE) + lane;
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
-                    st[dt * 64] = o[qt][dt];
-                st[DT * 64] = cf32x4_t{m, l, 0.f, 0.f};
-                __syncthreads();
-                float c[KW], mk[KW], lk[KW];
-#pragma unroll
-                for (int k = 0; k < KW; ++k)
-                {
-                    const cf32x4_t ml = reinterpret_cast<const cf32x4_t*>(lds + (k * RW + rw) * STATE)[DT * 64 + lane];
-                    mk[k] = ml[0];
-                    lk[k] = ml[1];
-                }
-                m = mk[0];
-#pragma unroll
-                for (int k = 1; k < KW; ++k)
-                    m = fmaxf(m, mk[k]);
-                l = 0.f;
-#pragma unroll
-                for (int k = 0; k < KW; ++k)
-                {
-                    c[k] = __builtin_amdgcn_exp2f(mk[k] - m);
-                    l += lk[k] * c[k];
-                }
-#pragma unroll
-                for (int dt = 0; dt < DTW; ++dt)
-                {
-                    acc[dt] = cf32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int k = 0; k < KW; ++k)
-                    {
-                        const cf32x4_t x = reinterpret_cast<const cf32x4_t*>(lds + (k * RW + rw) * STATE)[(dt0 + dt) * 64 + lane];
-#pragma unroll
-                        for (int rr = 0; rr < 4; ++rr)
-                            acc[dt][rr] += x[rr] * c[k];
-                    }
-                }
-            }
-            const int in_tile = rw * QT * 16 + 16 * qt + lr, r = min(mt * M + in_tile, n * G - 1), node = r / G;
-            if (any_nonfinite) // uniform, and rare
-            {
-                for (int j = 0; j < n; ++j)
-                {
-                    if (!((nonfinite[j >> 5] >> (j & 31)) & 1))
-                        continue;
-                    const int t = past + j;
-                    const size_t at = ((size_t) head_kv << p.tpb_log2) + (t & tpb_mask);
-                    const uint16_t* v = reinterpret_cast<const uint16_t*>(vp[t >> p.tpb_log2]) + at * hs;
-                    const bool sees = (p.tree_mask[(size_t) (off + node) * p.mask_words + (j >> 5)] >> (j & 31)) & 1;
-#pragma unroll
-                    for (int dt = 0; dt < DTW; ++dt)
-#pragma unroll
-                        for (int rr = 0; rr < 4; ++rr)
-                        {
-                            const int d = 16 * (dt0 + dt) + 4 * lq + rr;
-                            const uint32_t w = v[min(d, hs - 1)];
-                            acc[dt][rr] += sees && d < hs && tree_nonfinite2<T>(w) ? T16<T>::to_float(w) : 0.f;
-                        }
-                }
-            }
-            if (mt * M + in_tile >= n * G)
-                continue;
-            if (alone)
-            {
-                // no visible key: the sum is exactly 0, and so is the row (a NaN sum stays a NaN)
-                const float inv = l == 0.f ? 0.f : v_deq / l;
-                uint16_t* out = p.out + ((size_t) (off + node) * p.num_heads + head_kv * G + (r - node * G)) * hs;
-#pragma unroll
-                for (int dt = 0; dt < DTW; ++dt)
-                {
-                    const int d = 16 * (dt0 + dt) + 4 * lq;
-                    if (d < hs)
-                        *reinterpret_cast<uint2*>(out + d)
-                            = make_uint2(pack2<T>(acc[dt][0] * inv, acc[dt][1] * inv), pack2<T>(acc[dt][2] * inv, acc[dt][3] * inv));
-                }
-            }
-            else
-            {
-                const size_t rec = ((size_t) (2 * team + (tile_lo == 0)) * p.mtiles + mt) * M + in_tile;
-                float* part = p.part_acc + rec * DP;
-#pragma unroll
-                for (int dt = 0; dt < DTW; ++dt)
-                    *reinterpret_cast<cf32x4_t*>(part + 16 * (dt0 + dt) + 4 * lq) = acc[dt];
-                if (lq == 0 && kw == 0)
-                    p.part_ml[rec] = make_float2(m, l);
+                enter_tile();
+#pragma unroll 1
+                for (int kb = 0; kb < 16 * XW; kb += 16 * X2)
+                    step(std::false_type{}, stage, kb, 0);
+                leave_tile();
             }
         }
     }
-    if (!p.whole && mt == 0 && tid == 0)
-        p.join[team] = join;
+
+    // ---- the end of the item: the sum over the 4 lanes of a column; the states of the KW key groups meet in the LDS, and
+    // each of their waves joins and stores its share of the output columns
+    constexpr int DTW = DT / KW;
+    const int dt0 = kw * DTW;
+    bool any_nonfinite = false;
+    if constexpr (KVT == 0)
+        for (int w = 0; w < (n + 31) >> 5; ++w)
+            any_nonfinite |= nonfinite[w] != 0;
+    const float v_deq = KVT ? p.kv_scale_quant_orig[0] : 1.f;
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt)
+    {
+        float m = fresh[qt] ? NEG_BIG : -minus_m[qt][0], l = l_run[qt];
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+        cf32x4_t acc[DTW];
+        if constexpr (KW == 1)
+        {
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+                acc[dt] = o[qt][dt];
+        }
+        else
+        {
+            constexpr int STATE = (DT + 1) * 64 * 16; // bytes of one wave's state: float4 per register group and lane
+            static_assert(4 * STATE <= 2 * STAGE_BYTES, "states do not fit the tile buffers");
+            __syncthreads(); // everyone is done with the tiles, or with the states before
+            cf32x4_t* st = reinterpret_cast<cf32x4_t*>(lds + wave * STATE) + lane;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+                st[dt * 64] = o[qt][dt];
+            st[DT * 64] = cf32x4_t{m, l, 0.f, 0.f};
+            __syncthreads();
+            float c[KW], mk[KW], lk[KW];
+#pragma unroll
+            for (int k = 0; k < KW; ++k)
+            {
+                const cf32x4_t ml = reinterpret_cast<const cf32x4_t*>(lds + (k * RW + rw) * STATE)[DT * 64 + lane];
+                mk[k] = ml[0];
+                lk[k] = ml[1];
+            }
+            m = mk[0];
+#pragma unroll
+            for (int k = 1; k < KW; ++k)
+                m = fmaxf(m, mk[k]);
+            l = 0.f;
+#pragma unroll
+            for (int k = 0; k < KW; ++k)
+            {
+                c[k] = __builtin_amdgcn_exp2f(mk[k] - m);
+                l += lk[k] * c[k];
+            }
+#pragma unroll
+            for (int dt = 0; dt < DTW; ++dt)
+            {
+                acc[dt] = cf32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < KW; ++k)
+                {
+                    const cf32x4_t x = reinterpret_cast<const cf32x4_t*>(lds + (k * RW + rw) * STATE)[(dt0 + dt) * 64 + lane];
+#pragma unroll
+                    for (int rr = 0; rr < 4; ++rr)
+                        acc[dt][rr] += x[rr] * c[k];
+                }
+            }
+        }
+        const int in_tile = rw * QT * 16 + 16 * qt + lr, r = min(mt * M + in_tile, n * G - 1), node = r / G;
+        if (any_nonfinite) // uniform, and rare
+        {
+            for (int j = 0; j < n; ++j)
+            {
+                if (!((nonfinite[j >> 5] >> (j & 31)) & 1))
+                    continue;
+                const int t = past + j;
+                const size_t at = ((size_t) head_kv << p.tpb_log2) + (t & tpb_mask);
+                const uint16_t* v = reinterpret_cast<const uint16_t*>(vp[t >> p.tpb_log2]) + at * hs;
+                const bool sees = (p.tree_mask[(size_t) (off + node) * p.mask_words + (j >> 5)] >> (j & 31)) & 1;
+#pragma unroll
+                for (int dt = 0; dt < DTW; ++dt)
+#pragma unroll
+                    for (int rr = 0; rr < 4; ++rr)
+                    {
+                        const int d = 16 * (dt0 + dt) + 4 * lq + rr;
+                        const uint32_t w = v[min(d, hs - 1)];
+                        acc[dt][rr] += sees && d < hs && tree_nonfinite2<T>(w) ? T16<T>::to_float(w) : 0.f;
+                    }
+            }
+        }
+        if (mt * M + in_tile >= n * G)
+            continue;
+        if (parts == 1)
+        {
+            // no visible key: the sum is exactly 0, and so is the row (a NaN sum stays a NaN)
+            const float inv = l == 0.f ? 0.f : v_deq / l;
+            uint16_t* out = p.out + ((size_t) (off + node) * p.num_heads + head_kv * G + (r - node * G)) * hs;
+#pragma unroll
+            for (int dt = 0; dt < DTW; ++dt)
+            {
+                const int d = 16 * (dt0 + dt) + 4 * lq;
+                if (d < hs)
+                    *reinterpret_cast<uint2*>(out + d)
+                        = make_uint2(pack2<T>(acc[dt][0] * inv, acc[dt][1] * inv), pack2<T>(acc[dt][2] * inv, acc[dt][3] * inv));
+            }
+        }
+        else
+        {
+            const size_t rec = ((size_t) (__builtin_amdgcn_readlane(info_split.y, at) + in_seq) * p.mtiles + mt) * M + in_tile;
+            float* part = p.part_acc + rec * DP;
+#pragma unroll
+            for (int dt = 0; dt < DTW; ++dt)
+                *reinterpret_cast<cf32x4_t*>(part + 16 * (dt0 + dt) + 4 * lq) = acc[dt];
+            if (lq == 0 && kw == 0)
+                p.part_ml[rec] = make_float2(m, l);
+        }
+    }
 }
 
 // ---------------------------------------------------------------------------------------------- 3. combine
-// grid (ceil(rows of a (sequence, kv head) / 8), teams): the (sequence, kv head) that begins in the team's stretch and goes on
-// in the next ones.  Half a wave joins one row; the parts are summed in the keys' order, 4 in flight.
+// grid (ceil(rows of a (sequence, kv head) / 8), pairs of several parts at most).  Half a wave joins one row; the parts are summed in
+// the keys' order, 4 in flight.
 template <typename T, int DP>
 __global__ __launch_bounds__(TREE_THREADS) void tree_combine_kernel(TreeArgs p, bool quantised)
 {
-    const int team = blockIdx.y, lane = threadIdx.x & 31;
-    const int4 join = p.join[team];
+    const int lane = threadIdx.x & 31;
+    const int4 join = p.join[2 * blockIdx.y], where = p.join[2 * blockIdx.y + 1];
     const int S = join.w, G = p.group, r = blockIdx.x * (TREE_THREADS / 32) + (threadIdx.x >> 5);
-    if (S <= 1 || r >= join.y * G)
+    if (S <= 1 || r >= join.y * G || !p.seq_ok[where.y])
         return;
     const int M = p.rows_per_wg;
-    // record of part s: the last stretch of the first team, the first stretch of the others
-    auto record = [&](int s) { return ((size_t) (2 * (team + s) + (s == 0)) * p.mtiles + r / M) * M + r % M; };
+    auto record = [&](int s) { return ((size_t) (where.x + s) * p.mtiles + r / M) * M + r % M; };
     constexpr int E = DP / 32, U = 4;
     float mm = NEG_BIG, l = 0.f;
     for (int s = lane; s < S; s += 32)
@@ -1089,11 +1073,11 @@ __global__ __launch_bounds__(TREE_THREADS) void tree_combine_kernel(TreeArgs p, 
 struct TreePlan
 {
     int dp, rows_per_wg, mtiles; // padded head size; query rows per workgroup; m-tiles of a (sequence, kv head)
-    int teams, min_chunk, whole;
-    size_t q_bytes, seq_bytes, ok_bytes, join_bytes, acc_bytes, ml_bytes;
+    int target_items, part_tiles, items_bound, pairs_bound, records, whole;
+    size_t q_bytes, seq_bytes, split_bytes, ok_bytes, join_bytes, acc_bytes, ml_bytes;
     size_t total() const
     {
-        return q_bytes + seq_bytes + ok_bytes + join_bytes + acc_bytes + ml_bytes;
+        return q_bytes + seq_bytes + split_bytes + ok_bytes + join_bytes + acc_bytes + ml_bytes;
     }
 };
 size_t round256(size_t x)
@@ -1131,40 +1115,48 @@ TreePlan tree_plan(const mi355q_tree_attention_params& q)
     // Few rows: the 4 waves of a workgroup share the keys of a tile instead of the rows.  Whole calls, us, with 16 / 32 / 64 / 128 rows
     // a workgroup (bf16, Dh 128, 32 sequences of 2048 tokens, 32 heads): 16 nodes 235 / 235 / 238 / 240, 32 nodes 278 / 245 / 253 /
     // 253, 64 nodes 402 / 290 / 273 / 279, 128 nodes 741 / 460 / 369 / 337.
-    // 33 to 64 rows of fewer than 256 (sequence, kv head) pairs go as two tiles of 32: half as many teams, so fewer states to
+    // 33 to 64 rows of fewer than 256 (sequence, kv head) pairs go as two tiles of 32: half as many parts, so fewer states to
     // join (8 nodes x 8 heads over 4096 tokens, 4 / 8 / 16 sequences: 32.8 / 41.1 / 68.7 us, as one tile of 64 34.3 / 46.9 / 70.5)
     t.rows_per_wg = rows <= 16 ? 16 : (rows <= 32 || (rows <= 64 && t.dp <= 128 && groups < 256) ? 32 : (rows <= 64 || t.dp > 128 ? 64 : 128));
     t.mtiles = (rows + t.rows_per_wg - 1) / t.rows_per_wg;
-    // two workgroups live on a CU (one with heads beyond 128): as many teams as fill 256 CUs, of at least 2 tiles each (a
-    // stretch costs its prologue and a partial state), and no (sequence, kv head) over more teams than the combine reads
-    const int64_t slots = t.dp > 128 ? 256 : 512;
-    int64_t teams = std::max<int64_t>(slots / t.mtiles, 1); // (at most 512: a grid dimension of the combine kernel)
-    t.min_chunk = std::max(2, (max_tiles + TREE_MAX_SPLITS - 2) / (TREE_MAX_SPLITS - 1));
-    if (q.multi_block_mode > 0)
-    {
-        // that many stretches to the longest history
-        const int splits = std::min(q.multi_block_mode, max_tiles);
-        t.min_chunk = (max_tiles + splits - 1) / splits;
-        t.min_chunk = std::max(t.min_chunk, (max_tiles + TREE_MAX_SPLITS - 2) / (TREE_MAX_SPLITS - 1));
-        teams = std::min<int64_t>(groups * ((max_tiles + t.min_chunk - 1) / t.min_chunk), 65535);
-    }
-    // One team per (sequence, kv head), nothing to join, for short histories: up to 512 tokens, and up to 4096 the longer the more
-    // workgroups there are to even the lengths out (64 tiles with the chip's 512).  us whole / in stretches, histories of t / 6 .. t
+    // One item per (sequence, kv head), nothing to join, for short histories: up to 512 tokens, and up to 4096 the longer the more
+    // workgroups there are to even the lengths out (64 tiles with the chip's 512).  us whole / in parts, histories of t / 6 .. t
     // tokens: 128 workgroups (4 sequences, 32 heads, 16 nodes) t = 600 17.5 / 23.3, t = 1000 21.5 / 25.2; 256 (8 of 32 heads, 16 nodes)
     // 2100 40.6 / 47.5, 3400 66.2 / 62.0; 512 (16 of 32 heads, 64 nodes) 2100 96.9 / 117.9, 4100 167.8 / 188.4; 1024 4100 280.3 / 277.9;
     // 32 (one sequence) 1000 18.3 / 16.1
     const int64_t whole_tiles = std::min<int64_t>(std::max<int64_t>(groups * t.mtiles / 8, 8), 64);
     t.whole = q.multi_block_mode == 1 || (q.multi_block_mode == 0 && max_tiles <= whole_tiles);
-    t.teams = (int) std::min<int64_t>(t.whole ? groups : std::min(teams, (groups * max_tiles + t.min_chunk - 1) / t.min_chunk), INT32_MAX / 16);
-    t.teams = std::max(t.teams, 1);
+    if (t.whole)
+        t.items_bound = (int) std::min<int64_t>(groups, INT32_MAX / 16);
+    else if (q.multi_block_mode > 0)
+    {
+        // that many parts of the longest history
+        const int splits = std::min({q.multi_block_mode, max_tiles, TREE_MAX_SPLITS});
+        t.part_tiles = -((max_tiles + splits - 1) / splits);
+        t.items_bound = (int) std::min<int64_t>(groups * splits, INT32_MAX / 16);
+        t.pairs_bound = (int) std::min<int64_t>(groups, t.items_bound / 2);
+        t.records = t.items_bound;
+    }
+    else
+    {
+        // two workgroups live on a CU (one with heads beyond 128): about as many items as fill 256 CUs, of at least 2 tiles each (an
+        // item costs its prologue and a partial state), and no pair in more parts than the combine kernel reads.  A pair of nt
+        // tiles has round(nt / part) parts where that is 2 or more: at most 4 / 3 nt / part
+        t.target_items = std::max((t.dp > 128 ? 256 : 512) / t.mtiles, 1);
+        t.part_tiles = std::max(2, (max_tiles + TREE_MAX_SPLITS - 1) / TREE_MAX_SPLITS);
+        t.records = t.target_items + t.target_items / 3 + 1;
+        t.pairs_bound = (int) std::min<int64_t>(groups, t.records / 2);
+        t.items_bound = (int) std::min<int64_t>(groups + t.records, INT32_MAX / 16);
+    }
     const bool two_parts = q.kv_type == q.act_type || q.act_type == MI355Q_HALF; // TREE_Q2
     t.q_bytes = round256((size_t) q.num_tokens * q.num_heads * t.dp * 2 * (two_parts ? 2 : 1));
     t.seq_bytes = round256((size_t) (q.batch + 1) * sizeof(int4));
+    t.split_bytes = round256((size_t) q.batch * sizeof(int2));
     t.ok_bytes = round256((size_t) q.batch * sizeof(int32_t));
     if (!t.whole)
     {
-        t.join_bytes = round256((size_t) t.teams * sizeof(int4));
-        const size_t records = (size_t) 2 * t.teams * t.mtiles * t.rows_per_wg;
+        t.join_bytes = round256((size_t) t.pairs_bound * 2 * sizeof(int4));
+        const size_t records = (size_t) t.records * t.mtiles * t.rows_per_wg;
         t.acc_bytes = round256(records * t.dp * sizeof(float));
         t.ml_bytes = round256(records * sizeof(float2));
     }
@@ -1174,7 +1166,7 @@ TreePlan tree_plan(const mi355q_tree_attention_params& q)
 template <typename T, int KVT, int DP>
 void tree_launch_attn(const TreeArgs& a, const TreePlan& t, hipStream_t stream)
 {
-    const int64_t grid = ((int64_t) t.teams + 7) / 8 * 8 * t.mtiles;
+    const int64_t grid = ((int64_t) t.items_bound + 7) / 8 * 8 * t.mtiles;
     MQ_CHECK(grid < (1ll << 24), "tree attention grid %lld", (long long) grid); // 2^32 threads
     const dim3 g((unsigned) grid), b(TREE_THREADS);
     // 32 rows a wave; 16 with heads beyond 128, whose accumulators take twice the registers
@@ -1204,9 +1196,10 @@ void tree_launch(const mi355q_tree_attention_params& q, const TreeArgs& a, const
         tree_launch_attn<T, KVT, 128>(a, t, stream);
     else
         tree_launch_attn<T, KVT, 256>(a, t, stream);
-    if (!t.whole)
+    if (!t.whole && t.pairs_bound)
     {
-        const dim3 g((t.mtiles * t.rows_per_wg + 7) / 8, t.teams), b(TREE_THREADS);
+        MQ_CHECK(t.pairs_bound <= 65535, "tree attention: %d (sequence, kv head) pairs in parts", t.pairs_bound);
+        const dim3 g((t.mtiles * t.rows_per_wg + 7) / 8, t.pairs_bound), b(TREE_THREADS);
         if (t.dp == 64)
             hipLaunchKernelGGL((tree_combine_kernel<T, 64>), g, b, 0, stream, a, KVT != 0);
         else if (t.dp == 128)
@@ -1294,6 +1287,7 @@ void tree_attention(const mi355q_tree_attention_params& q, hipStream_t stream)
     };
     a.q_ws = reinterpret_cast<uint16_t*>(carve(t.q_bytes));
     a.seq = reinterpret_cast<int4*>(carve(t.seq_bytes));
+    a.split = reinterpret_cast<int2*>(carve(t.split_bytes));
     a.seq_ok = reinterpret_cast<int32_t*>(carve(t.ok_bytes));
     a.join = reinterpret_cast<int4*>(carve(t.join_bytes));
     a.part_acc = reinterpret_cast<float*>(carve(t.acc_bytes));
@@ -1313,8 +1307,10 @@ void tree_attention(const mi355q_tree_attention_params& q, hipStream_t stream)
         ++a.tpb_log2;
     a.mtiles = t.mtiles;
     a.rows_per_wg = t.rows_per_wg;
-    a.teams = t.teams;
-    a.min_chunk = t.min_chunk;
+    a.target_items = t.target_items;
+    a.part_tiles = t.part_tiles;
+    a.items_bound = t.items_bound;
+    a.pairs_bound = t.pairs_bound;
     a.whole = t.whole;
     MQ_CHECK((int64_t) q.batch * q.num_kv_heads * ((q.max_past_length + q.max_draft_length + TREE_KT - 1) / TREE_KT) < (1 << 30),
         "tree attention: %d sequences x %d kv heads x %d keys", q.batch, q.num_kv_heads, q.max_past_length);
