@@ -268,6 +268,9 @@ __device__ __forceinline__ void tree_chunk8(
 // grid (max_draft + 2, batch, parts of the heads).  Angles, and rotation and quantisation of K / V, run in 64 bits: the angle of a
 // far position has few correct digits left in fp32 (position 2^17: error 2^-8 rad), and a value next to a rounding border
 // of the cache's type lands on the side the definition says.  The queries, the larger part, are rotated in fp32.
+// Bound by memory: rows in, two parts of q and K / V out, in rows of 256 bytes.  708 tokens of 32 + 64 heads of 128: 14 us for 41 MB;
+// 8 tokens: 4.2 us, a launch, three dependent loads and the angles.  (Loading a thread's elements ahead of the angles, values
+// as plain copies, and more or fewer workgroups than 2048 all cost 1 to 3 us more.)
 template <typename T, int KVT>
 __global__ __launch_bounds__(TREE_THREADS) void tree_prepare_kernel(TreeArgs p, int dp)
 {
@@ -496,6 +499,13 @@ __device__ __forceinline__ uint64_t tree_mask64(const uint32_t* row, int words, 
 // Softmax in the log2 domain with the running maximum as the C operand of the first product: what comes out is already
 // s - m, and as long as no column grows past m + 8 (p <= 256: harmless in fp16 / bf16 and in the fp32 sums) nothing is rescaled.
 // Whether one does is an integer maximum over the raw bits (negative floats are negative integers).
+// Two workgroups live on a CU (64 KiB of LDS: a tile of K and V that is computed, one that arrives), 2 waves a SIMD at 211 to 247
+// registers; what one waits for the other covers.  Bound by HBM up to some 32 rows a kv head, then by the matrix instructions,
+// of which the second part of q is a third, by the softmax beside them and by the LDS.  Whole calls, bf16, Dh 128, 64 sequences of 2048
+// tokens, 32 / 32 heads: 1 node 5.7 TB/s, 16 nodes 5.3, 64 nodes 4.8 (a copy reaches 5.05); 16 x 4096 tokens, 64 nodes, 64 / 8 heads:
+// 205 us = 0.68 PFLOP/s of the formula's and 1.0 of products issued (a large matrix product 1.23); one sequence of 120001
+// tokens, 60 nodes, 64 / 8 heads: 325 us, matrix pipes busy 51 %, no LDS conflicts.  Four tiles in flight with one workgroup a CU
+// took 127 us where this took 93, 8 waves of 256 rows 275 for 217.
 template <typename T, int KVT, int DP, int RW, int KW, int QT>
 __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP > 128 ? 1 : 2))) void tree_attn_kernel(TreeArgs p)
 {
@@ -891,8 +901,9 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
                 store_tile(stage);
         }
     };
-    // the first tile and the tiles with nodes go through the general step, the history's others through the short one
-    // (with few rows one copy of the step: fetching code costs more there than a mask test)
+    // The first tile and the tiles with nodes go through the general step, the history's others through the short one: 328 us for 352
+    // with the general step alone over 120001 tokens (60 nodes, 64 / 8 heads), 176 for 193 over 16 x 4096 in fp8.  Where the waves
+    // share the keys one copy of the step is enough (16 nodes, 64 x 2048 tokens: 431 us either way).
     const bool has_rows = q0 < n * G; // a wave without rows (a smaller tree than the largest) only loads
     const int plain_end = KW == 1 ? min(tile_hi, past / TREE_KT) : 0;
     while (i < tile_hi)
@@ -1043,7 +1054,7 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
 
 // ---------------------------------------------------------------------------------------------- 3. combine
 // grid (ceil(rows of a (sequence, kv head) / 8), pairs of several parts at most).  Half a wave joins one row; the parts are summed in
-// the keys' order, 4 in flight.
+// the keys' order, 4 in flight.  Bound by the reads of the states: 8.5 us for 18 MB (256 pairs of 20 .. 108 rows), 4.2 us at least.
 template <typename T, int DP>
 __global__ __launch_bounds__(TREE_THREADS) void tree_combine_kernel(TreeArgs p, bool quantised)
 {
@@ -1138,17 +1149,17 @@ TreePlan tree_plan(const mi355q_tree_attention_params& q)
     const int max_tiles = std::max((q.max_past_length + q.max_draft_length + TREE_KT - 1) / TREE_KT, 1);
     const int64_t groups = (int64_t) q.batch * q.num_kv_heads;
     // Few rows: the 4 waves of a workgroup share the keys of a tile instead of the rows.  Whole calls, us, with 16 / 32 / 64 / 128 rows
-    // a workgroup (bf16, Dh 128, 32 sequences of 2048 tokens, 32 heads): 16 nodes 235 / 235 / 238 / 240, 32 nodes 278 / 245 / 253 /
-    // 253, 64 nodes 402 / 290 / 273 / 279, 128 nodes 741 / 460 / 369 / 337.
+    // a workgroup (bf16, Dh 128, 32 sequences of 2048 tokens, 32 heads): 16 nodes 230 / 230 / 232 / 233, 32 nodes 262 / 238 / 242 /
+    // 243, 64 nodes 403 / 291 / 270 / 275, 128 nodes 718 / 453 / 356 / 334.
     // 33 to 64 rows of fewer than 256 (sequence, kv head) pairs go as two tiles of 32: half as many parts, so fewer states to
-    // join (8 nodes x 8 heads over 4096 tokens, 4 / 8 / 16 sequences: 32.8 / 41.1 / 68.7 us, as one tile of 64 34.3 / 46.9 / 70.5)
+    // join (8 nodes x 8 heads over 4096 tokens, 4 / 8 / 16 / 32 sequences: 29.2 / 37.3 / 61.0 / 128 us, as one tile of 64 33.8 / 41.8 /
+    // 64.3 / 127)
     t.rows_per_wg = rows <= 16 ? 16 : (rows <= 32 || (rows <= 64 && t.dp <= 128 && groups < 256) ? 32 : (rows <= 64 || t.dp > 128 ? 64 : 128));
     t.mtiles = (rows + t.rows_per_wg - 1) / t.rows_per_wg;
     // One item per (sequence, kv head), nothing to join, for short histories: up to 512 tokens, and up to 4096 the longer the more
-    // workgroups there are to even the lengths out (64 tiles with the chip's 512).  us whole / in parts, histories of t / 6 .. t
-    // tokens: 128 workgroups (4 sequences, 32 heads, 16 nodes) t = 600 17.5 / 23.3, t = 1000 21.5 / 25.2; 256 (8 of 32 heads, 16 nodes)
-    // 2100 40.6 / 47.5, 3400 66.2 / 62.0; 512 (16 of 32 heads, 64 nodes) 2100 96.9 / 117.9, 4100 167.8 / 188.4; 1024 4100 280.3 / 277.9;
-    // 32 (one sequence) 1000 18.3 / 16.1
+    // workgroups there are to even the lengths out (64 tiles with the chip's 512).  us whole / in parts, equal histories of t tokens:
+    // 32 workgroups (one sequence, 32 heads, 8 nodes) t = 440 13.2 / 15.0, 1000 18.4 / 16.1; 128 (4 sequences, 16 nodes) 600 19.0 / 22.9,
+    // 1000 24.1 / 26.5; 256 (8) 2100 55.1 / 58.3, 3400 101.2 / 100.6 (ragged 66.0 / 60.3); 512 (16, 64 nodes) 4100 235 / 238, 1024 (32) 417 / 430
     const int64_t whole_tiles = std::min<int64_t>(std::max<int64_t>(groups * t.mtiles / 8, 8), 64);
     t.whole = q.multi_block_mode == 1 || (q.multi_block_mode == 0 && max_tiles <= whole_tiles);
     if (t.whole)
@@ -1165,7 +1176,8 @@ TreePlan tree_plan(const mi355q_tree_attention_params& q)
     else
     {
         // two workgroups live on a CU (one with heads beyond 128): about as many items as fill 256 CUs, of at least 2 tiles each (an
-        // item costs its prologue and a partial state), and no pair in more parts than the combine kernel reads.  A pair of nt
+        // item costs its prologue and a partial state; 512 / 1024 items, us: 4 sequences of 4000 tokens, 8 nodes, 32 / 8 heads 28 / 35,
+        // 16 of 4100, 64 nodes, 64 / 8 heads 212 / 230, ragged 132 / 139), and no pair in more parts than the combine kernel reads.  A pair of nt
         // tiles has round(nt / part) parts where that is 2 or more: at most 4 / 3 nt / part
         t.target_items = std::max((t.dp > 128 ? 256 : 512) / t.mtiles, 1);
         t.part_tiles = std::max(2, (max_tiles + TREE_MAX_SPLITS - 1) / TREE_MAX_SPLITS);
