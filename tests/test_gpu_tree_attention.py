@@ -117,6 +117,15 @@ def test_key_splits(cuda, splits, Hq, n):
     check(c, cuda, op_kw=dict(multi_block_mode=splits))
 
 
+@pytest.mark.parametrize("B,splits,bound", [(70, 0, 700), (200, 0, 2600), (256, 4, 700), (257, 4, 700), (300, 0, 2600), (300, 3, 700)])
+def test_many_sequences(cuda, B, splits, bound):
+    # lengths in any order, empty sequences and trees among them; bound: what the host says of the histories
+    rs = np.random.RandomState(B + splits)
+    past = [int(x) for x in rs.choice([0, 5, 63, 64, 130, 400, 600], B, p=[0.1, 0.3, 0.1, 0.1, 0.2, 0.1, 0.1])]
+    c = TreeCase(past, trees([int(n) for n in rs.randint(0, 6, B)]), 2, 1, 64, BF, max_blocks=48, behind=3)
+    check(c, cuda, op_kw=dict(multi_block_mode=splits), max_past_length=bound)
+
+
 def test_masks(cuda):
     # nodes that see nothing (a zero row where there is no history), not themselves, everything, later nodes; bits beyond the
     # tree and rows beyond the sequences are set and must not count
