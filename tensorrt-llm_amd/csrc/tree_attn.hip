@@ -1204,7 +1204,6 @@ template <typename T, int KVT, int DP>
 void tree_launch_attn(const TreeArgs& a, const TreePlan& t, hipStream_t stream)
 {
     const int64_t grid = ((int64_t) t.items_bound + 7) / 8 * 8 * t.mtiles;
-    MQ_CHECK(grid < (1ll << 24), "tree attention grid %lld", (long long) grid); // 2^32 threads
     const dim3 g((unsigned) grid), b(TREE_THREADS);
     // 32 rows a wave; 16 with heads beyond 128, whose accumulators take twice the registers
     constexpr int QT = DP > 128 ? 1 : 2;
@@ -1235,7 +1234,6 @@ void tree_launch(const mi355q_tree_attention_params& q, const TreeArgs& a, const
         tree_launch_attn<T, KVT, 256>(a, t, stream);
     if (!t.whole && t.pairs_bound)
     {
-        MQ_CHECK(t.pairs_bound <= 65535, "tree attention: %d (sequence, kv head) pairs in parts", t.pairs_bound);
         const dim3 g((t.mtiles * t.rows_per_wg + 7) / 8, t.pairs_bound), b(TREE_THREADS);
         if (t.dp == 64)
             hipLaunchKernelGGL((tree_combine_kernel<T, 64>), g, b, 0, stream, a, KVT != 0);
@@ -1303,6 +1301,11 @@ void tree_attention(const mi355q_tree_attention_params& q, hipStream_t stream)
     else if (q.position_embedding_type != 0)
         MQ_UNSUPPORTED("tree attention: position_embedding_type %d is not built (0 - 2)", q.position_embedding_type);
     const TreePlan t = tree_plan(q);
+    MQ_CHECK((int64_t) q.batch * q.num_kv_heads * ((q.max_past_length + q.max_draft_length + TREE_KT - 1) / TREE_KT) < (1 << 30),
+        "tree attention: %d sequences x %d kv heads x %d keys", q.batch, q.num_kv_heads, q.max_past_length);
+    // what the grids hold (2^32 threads, 65535 rows)
+    MQ_CHECK(((int64_t) t.items_bound + 8) * t.mtiles < (1ll << 24) && t.pairs_bound <= 65535,
+        "tree attention: %d sequences x %d kv heads x %d row tiles, up to %d pairs in parts", q.batch, q.num_kv_heads, t.mtiles, t.pairs_bound);
     MQ_CHECK(q.workspace && q.workspace_bytes >= t.total(), "workspace too small: %zu < %zu", q.workspace_bytes, t.total());
     TreeArgs a{};
     a.qkv = static_cast<const uint16_t*>(q.qkv);
@@ -1349,8 +1352,6 @@ void tree_attention(const mi355q_tree_attention_params& q, hipStream_t stream)
     a.items_bound = t.items_bound;
     a.pairs_bound = t.pairs_bound;
     a.whole = t.whole;
-    MQ_CHECK((int64_t) q.batch * q.num_kv_heads * ((q.max_past_length + q.max_draft_length + TREE_KT - 1) / TREE_KT) < (1 << 30),
-        "tree attention: %d sequences x %d kv heads x %d keys", q.batch, q.num_kv_heads, q.max_past_length);
     a.pos_type = q.position_embedding_type;
     a.rot_dim = q.rotary_embedding_dim;
     a.rot_scale_type = q.rotary_embedding_scale_type;

@@ -57,7 +57,11 @@ ROPE = dict(position_embedding_type=2, rotary_embedding_dim=128)
     (dict(ROPE, rotary_embedding_scale_type=3), INVALID, "scale_type"), (dict(ROPE, rotary_embedding_scale_type=1), INVALID, "scale"),
     (dict(ROPE, rotary_embedding_scale_type=2, rotary_embedding_scale=2.0), INVALID, "dynamic"),
     (dict(multi_block_mode=-1), INVALID, "multi_block_mode"), (dict(workspace=None), INVALID, "workspace too small"),
-    (dict(workspace_bytes=1000), INVALID, "workspace too small")])
+    (dict(workspace_bytes=1000), INVALID, "workspace too small"),
+    # more than the grids hold
+    (dict(batch=65535, num_heads=1024, num_kv_heads=512, num_tokens=65535), INVALID, "row tiles"),
+    (dict(batch=65535, multi_block_mode=4), INVALID, "pairs in parts"),
+    (dict(batch=65535, num_heads=2048, num_kv_heads=1024, max_past_length=2048), INVALID, "kv heads")])
 def test_tree_attention_refusals(kw, status, words):
     refused("mi355q_tree_attention", tree_params(**kw), status, words)
 
