@@ -425,8 +425,10 @@ def _ptr(name, t, index, dtype, shape):
     return t.data_ptr()
 
 
-# the handle of a GPU's current stream without a Stream object around it (1 us a call)
+# the handle of a GPU's current stream without a Stream object around it, and the current GPU without the initialisation check
+# (a CUDA tensor is at hand): 1.2 us a call
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+_current_gpu = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 class _On:
@@ -440,10 +442,10 @@ class _On:
         self.index = t.get_device()
 
     def __enter__(self):
-        self.previous = torch.cuda.current_device()
+        self.previous = _current_gpu()
         if self.previous != self.index:
             torch.cuda.set_device(self.index)
-        return C.c_void_p(_raw_stream(self.index))
+        return _raw_stream(self.index)
 
     def __exit__(self, *exc):
         if self.previous != self.index:
@@ -525,7 +527,7 @@ class TreeAttention:
         p.qkv, p.qkv_stride = qkv.data_ptr(), qkv.stride(0) if tokens > 1 else 0
         with on as stream:
             if out is None:
-                out = torch.empty((tokens, self.out_hidden), dtype=self.dtype, device=qkv.device)
+                out = qkv.new_empty((tokens, self.out_hidden))
             p.out = _ptr("out", out, dev, self.dtype, (tokens, self.out_hidden))
             if workspace is None:  # from torch's allocator: ordered on this stream, kept by a graph that captures the call
                 bounds = (batch, tokens, max_draft_length, max_past_length, blocks)
@@ -534,9 +536,11 @@ class TreeAttention:
                     if len(self._sizes) >= 1024:
                         self._sizes.clear()
                     need = self._sizes[bounds] = L.lib().mi355q_tree_attention_workspace_size(C.byref(p))
-                workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=qkv.device)
-            p.workspace = _ptr("workspace", workspace, dev, torch.uint8, workspace.shape)
-            p.workspace_bytes = workspace.numel()
+                workspace = qkv.new_empty(need // 2 + 8)  # (elements of 2 bytes)
+                p.workspace, p.workspace_bytes = workspace.data_ptr(), 2 * workspace.shape[0]
+            else:
+                p.workspace = _ptr("workspace", workspace, dev, torch.uint8, workspace.shape)
+                p.workspace_bytes = workspace.numel()
             L.check(L.lib().mi355q_tree_attention(C.byref(p), stream))
         return out
 
@@ -558,12 +562,11 @@ def kv_block_tables(past_lengths, new_lengths, block_table, block_counts, free_b
     counts_out = block_counts if block_counts_out is None else block_counts_out
     state_out = free_state if free_state_out is None else free_state_out
     with on as stream:
-        where = past_lengths.device
-        pointers = torch.empty((pools, batch, 2, max_blocks), dtype=torch.int64, device=where)
-        slots = torch.empty(num_tokens, dtype=torch.int64, device=where)
+        # (new tensors take the type of one that is checked below)
+        pointers, slots = pool_bases.new_empty((pools, batch, 2, max_blocks)), pool_bases.new_empty(num_tokens)
         # offsets, status and the workspace in one allocation, the workspace first (16-byte aligned)
         need = L.lib().mi355q_kv_block_tables_workspace_size(batch)
-        small = torch.empty(need // 4 + 2 * batch + 1, dtype=i32, device=where)
+        small = past_lengths.new_empty(need // 4 + 2 * batch + 1)
         offsets, status = small[need // 4:need // 4 + batch + 1], small[need // 4 + batch + 1:]
         at = small.data_ptr()
         p = L.KvBlockTablesParams(
@@ -588,8 +591,7 @@ def draft_tree_accept(draft_tokens, parents, target_tokens, draft_offsets, max_p
         raise ValueError("draft_tokens must be [num_tokens], draft_offsets [batch + 1], max_path at least 1")
     flat, batch = draft_tokens.shape, draft_offsets.shape[0] - 1
     with on as stream:
-        both = torch.empty((2, batch, max_path), dtype=i32, device=draft_tokens.device)
-        counts = torch.empty(batch, dtype=i32, device=draft_tokens.device)
+        both, counts = draft_tokens.new_empty((2, batch, max_path)), draft_tokens.new_empty(batch)
         at = both.data_ptr()
         p = L.DraftTreeAcceptParams(
             _ptr("draft_tokens", draft_tokens, dev, i32, flat), _ptr("parents", parents, dev, i32, flat),
@@ -611,7 +613,7 @@ def kv_commit_path(block_pointers, past_lengths, accept_path, accept_counts, *, 
     pools, batch, _, max_blocks = block_pointers.shape
     max_path = accept_path.shape[1]
     with on as stream:
-        lengths = torch.empty(batch, dtype=i32, device=block_pointers.device)
+        lengths = past_lengths.new_empty(batch)
         p = L.KvCommitPathParams(
             _ptr("block_pointers", block_pointers, dev, torch.int64, (pools, batch, 2, max_blocks)),
             _ptr("past_lengths", past_lengths, dev, i32, (batch,)), _ptr("accept_path", accept_path, dev, i32, (batch, max_path)),
