@@ -499,7 +499,7 @@ __device__ __forceinline__ uint64_t tree_mask64(const uint32_t* row, int words, 
 // Softmax in the log2 domain with the running maximum as the C operand of the first product: what comes out is already
 // s - m, and as long as no column grows past m + 8 (p <= 256: harmless in fp16 / bf16 and in the fp32 sums) nothing is rescaled.
 // Whether one does is an integer maximum over the raw bits (negative floats are negative integers).
-// Two workgroups live on a CU (64 KiB of LDS: a tile of K and V that is computed, one that arrives), 2 waves a SIMD at 211 to 247
+// Two workgroups live on a CU (64 KiB of LDS: a tile of K and V that is computed, one that arrives), 2 waves a SIMD at 219 to 249
 // registers; what one waits for the other covers.  Bound by HBM up to some 32 rows a kv head, then by the matrix instructions,
 // of which the second part of q is a third, by the softmax beside them and by the LDS.  Whole calls, bf16, Dh 128, 64 sequences of 2048
 // tokens, 32 / 32 heads: 1 node 5.7 TB/s, 16 nodes 5.3, 64 nodes 4.8 (a copy reaches 5.05); 16 x 4096 tokens, 64 nodes, 64 / 8 heads:
@@ -518,8 +518,8 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
     constexpr int TILE_BYTES = TREE_KT * ROWB, STAGE_BYTES = 2 * TILE_BYTES;
     constexpr int XW = 4 / KW;                      // 16-key subtiles per wave
     constexpr int X2 = XW < 2 ? XW : 2;             // subtiles per compute step: 32 keys, or 16 with four key groups
-    // fragments read from the LDS ahead of their products, as many as the registers hold
-    constexpr bool TIGHT = PARTS == 2 && QT == 2 && DP >= 128;
+    // fragments read from the LDS ahead of their products, as many as the registers hold (8-bit caches hold a tile in them too)
+    constexpr bool TIGHT = KVT && PARTS == 2 && QT == 2 && DP >= 128;
     constexpr int KBATCH = TIGHT && X2 == 2 ? 2 : KS, VBATCH = TIGHT && X2 == 2 ? 4 : (DT < 8 ? DT : 8);
     constexpr int WROWS = TREE_KT / 4;              // a wave loads 16 consecutive keys of a tile
     constexpr int RPD = 1024 / ROWB, DPW = WROWS / RPD; // 16-bit caches: rows per DMA instruction, DMAs per wave
