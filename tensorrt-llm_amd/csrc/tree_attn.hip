@@ -499,6 +499,10 @@ __device__ __forceinline__ uint64_t tree_mask64(const uint32_t* row, int words, 
 // Softmax in the log2 domain with the running maximum as the C operand of the first product: what comes out is already
 // s - m, and as long as no column grows past m + 8 (p <= 256: harmless in fp16 / bf16 and in the fp32 sums) nothing is rescaled.
 // Whether one does is an integer maximum over the raw bits (negative floats are negative integers).
+// Scores that come out NaN: an infinite key element, or products beyond fp32, meet the second part of q, whose sign is either, or
+// the zeros that q is padded with.  The row's sum is then NaN, and the whole item runs again with careful scores; what is still
+// NaN then is so by the definition.  (The check at an item's end costs up to 1 us a call: 92.8 for 91.8 over 16
+// sequences of 300 .. 2048 tokens, 32 / 32 heads, up to 64 nodes; nothing measurable elsewhere.)
 // Two workgroups live on a CU (64 KiB of LDS: a tile of K and V that is computed, one that arrives), 2 waves a SIMD at 219 to 249
 // registers; what one waits for the other covers.  Bound by HBM up to some 32 rows a kv head, then by the matrix instructions,
 // of which the second part of q is a third, by the softmax beside them and by the LDS.  Whole calls, bf16, Dh 128, 64 sequences of 2048
@@ -526,6 +530,7 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
     constexpr int CH8 = DP / 16, RPL = 64 / CH8, LPT = WROWS / RPL; // 8-bit caches: rows per 16-byte load, loads per thread
     __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE_BYTES]; // a tile that is computed, a tile that arrives
     __shared__ uint32_t nonfinite[TREE_MAX_DRAFT / 32]; // nodes whose V row has an infinity or NaN
+    __shared__ int redo;                                // a row's sum is NaN
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -648,8 +653,11 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
         }
     };
 
+    // (the barrier of the first tile comes before the first use)
     if (KVT == 0 && tid < TREE_MAX_DRAFT / 32)
-        nonfinite[tid] = 0; // (the barrier of the first tile comes before the first use)
+        nonfinite[tid] = 0;
+    if (tid == 0)
+        redo = 0;
     find_tile(tile_lo);
     if (!p.seq_ok[b]) // a block is missing: nothing of it is read
         return;
@@ -690,18 +698,9 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
     cf32x4_t minus_m[QT]; // C operand of the scores: minus the running maximum
     bool fresh[QT];       // the column has no maximum yet (minus_m is 0)
     cf32x4_t o[QT][DT];
-#pragma unroll
-    for (int qt = 0; qt < QT; ++qt)
-    {
-        fresh[qt] = true;
-        l_run[qt] = 0.f;
-        minus_m[qt] = cf32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-            o[qt][dt] = cf32x4_t{0.f, 0.f, 0.f, 0.f};
-    }
 
     // One compute step: X2 subtiles from key `kb` of the tile in `stage` on.  GENERAL: columns may still be fresh, keys hidden.
+    bool careful = false;
     auto step = [&](auto general, uint32_t stage, int kb, int t0)
     {
         constexpr bool GENERAL = decltype(general)::value;
@@ -712,25 +711,56 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
 #pragma unroll
             for (int qt = 0; qt < QT; ++qt)
                 s[x][qt] = minus_m[qt];
-#pragma unroll
-        for (int ks0 = 0; ks0 < KS; ks0 += KBATCH)
+        if (GENERAL && careful) // uniform
         {
-            uint4 kf[KBATCH][X2];
+            // the products of the two parts of q apart, the padding of the keys as zeros; the second part counts only where both are
+            // finite, so that an infinite score keeps the sign that the first part gives it
+#pragma unroll 1
+            for (int x = 0; x < X2; ++x)
 #pragma unroll
-            for (int ks = 0; ks < KBATCH; ++ks)
+                for (int qt = 0; qt < QT; ++qt)
+                {
+                    cf32x4_t hi = {0.f, 0.f, 0.f, 0.f}, lo = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int x = 0; x < X2; ++x)
-                    kf[ks][x] = tree_lds16((ka ^ (64 * (ks0 + ks))) + 16 * x * ROWB);
+                    for (int ks = 0; ks < KS; ++ks)
+                    {
+                        uint4 kf = tree_lds16((ka ^ (64 * ks)) + 16 * x * ROWB);
+                        if (32 * ks + 8 * lq >= hs)
+                            kf = make_uint4(0, 0, 0, 0);
+                        hi = ctx_mfma<C>(kf, qf[0][qt][ks], hi);
+                        if constexpr (PARTS == 2)
+                            lo = ctx_mfma<C>(kf, qf[PARTS - 1][qt][ks], lo);
+                    }
 #pragma unroll
-            for (int ks = 0; ks < KBATCH; ++ks)
+                    for (int rr = 0; rr < 4; ++rr)
+                    {
+                        const float z = fabsf(hi[rr]) < HUGE_VALF && fabsf(lo[rr]) < HUGE_VALF ? hi[rr] + lo[rr] : hi[rr];
 #pragma unroll
-                for (int part = PARTS - 1; part >= 0; --part)
-#pragma unroll
-                    for (int x = 0; x < X2; ++x) // consecutive products go to different accumulators
-#pragma unroll
-                        for (int qt = 0; qt < QT; ++qt)
-                            s[x][qt] = ctx_mfma<C>(kf[ks][x], qf[part][qt][ks0 + ks], s[x][qt]);
+                        for (int y = 0; y < X2; ++y)
+                            s[y][qt][rr] = y == x ? z + minus_m[qt][rr] : s[y][qt][rr];
+                    }
+                }
         }
+        else
+#pragma unroll
+            for (int ks0 = 0; ks0 < KS; ks0 += KBATCH)
+            {
+                uint4 kf[KBATCH][X2];
+#pragma unroll
+                for (int ks = 0; ks < KBATCH; ++ks)
+#pragma unroll
+                    for (int x = 0; x < X2; ++x)
+                        kf[ks][x] = tree_lds16((ka ^ (64 * (ks0 + ks))) + 16 * x * ROWB);
+#pragma unroll
+                for (int ks = 0; ks < KBATCH; ++ks)
+#pragma unroll
+                    for (int part = PARTS - 1; part >= 0; --part)
+#pragma unroll
+                        for (int x = 0; x < X2; ++x) // consecutive products go to different accumulators
+#pragma unroll
+                            for (int qt = 0; qt < QT; ++qt)
+                                s[x][qt] = ctx_mfma<C>(kf[ks][x], qf[part][qt][ks0 + ks], s[x][qt]);
+            }
         // the first V fragments are read while the softmax runs
         uint2 vf[VBATCH][X2];
         auto read_v = [&](int d0)
@@ -876,8 +906,6 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
         __syncthreads();
     };
 
-    if constexpr (KVT != 0)
-        store_tile(0);
     uint32_t stage = 0; // of the tile that is computed
     int i = tile_lo;
     auto enter_tile = [&]()
@@ -906,33 +934,64 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
     // share the keys one copy of the step is enough (16 nodes, 64 x 2048 tokens: 431 us either way).
     const bool has_rows = q0 < n * G; // a wave without rows (a smaller tree than the largest) only loads
     const int plain_end = KW == 1 ? min(tile_hi, past / TREE_KT) : 0;
-    while (i < tile_hi)
+    for (;; careful = true)
     {
-        enter_tile();
-        const int t0 = i * TREE_KT;
-        if (t0 + TREE_KT > past)
-            clean_tail(stage, t0);
-#pragma unroll 1
-        for (int kb = has_rows ? 0 : 16 * XW; kb < 16 * XW; kb += 16 * X2)
-            step(std::true_type{}, stage, kb, t0);
-        leave_tile();
-        if constexpr (KW == 1)
-        {
-            // (scores of -inf only, of an overflow in fp32: the column has no maximum yet, the general step goes on)
-            bool open = false;
 #pragma unroll
-            for (int qt = 0; qt < QT; ++qt)
-                open |= fresh[qt];
-            const bool settled = !__any(open);
-            while (settled && i < plain_end)
-            {
-                enter_tile();
+        for (int qt = 0; qt < QT; ++qt)
+        {
+            fresh[qt] = true;
+            l_run[qt] = 0.f;
+            minus_m[qt] = cf32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+                o[qt][dt] = cf32x4_t{0.f, 0.f, 0.f, 0.f};
+        }
+        if constexpr (KVT != 0)
+            store_tile(0);
+        while (i < tile_hi)
+        {
+            enter_tile();
+            const int t0 = i * TREE_KT;
+            if (t0 + TREE_KT > past)
+                clean_tail(stage, t0);
 #pragma unroll 1
-                for (int kb = 0; kb < 16 * XW; kb += 16 * X2)
-                    step(std::false_type{}, stage, kb, 0);
-                leave_tile();
+            for (int kb = has_rows ? 0 : 16 * XW; kb < 16 * XW; kb += 16 * X2)
+                step(std::true_type{}, stage, kb, t0);
+            leave_tile();
+            if constexpr (KW == 1)
+            {
+                // (scores of -inf only, of an overflow in fp32: the column has no maximum yet, the general step goes on)
+                bool open = careful;
+#pragma unroll
+                for (int qt = 0; qt < QT; ++qt)
+                    open |= fresh[qt];
+                const bool settled = !__any(open);
+                while (settled && i < plain_end)
+                {
+                    enter_tile();
+#pragma unroll 1
+                    for (int kb = 0; kb < 16 * XW; kb += 16 * X2)
+                        step(std::false_type{}, stage, kb, 0);
+                    leave_tile();
+                }
             }
         }
+        if (careful)
+            break;
+        bool bad = false;
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt)
+            bad |= l_run[qt] != l_run[qt];
+        if (__any(bad))
+            redo = 1;
+        __syncthreads();
+        if (!__builtin_amdgcn_readfirstlane(redo))
+            break;
+        stage = 0;
+        i = tile_lo;
+        find_tile(tile_lo);
+        load_tile(0);
+        find_tile(min(tile_lo + 1, tile_hi - 1));
     }
 
     // ---- the end of the item: the sum over the 4 lanes of a column; the states of the KW key groups meet in the LDS, and
