@@ -24,6 +24,7 @@ constexpr int TREE_THREADS = 256;   // 4 waves
 constexpr int TREE_MAX_SPLITS = 128; // parts of a (sequence, kv head): what the combine kernel reads
 constexpr int TREE_MAX_DRAFT = 1024;
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr float TREE_NO_MAX = -FLT_MAX; // the maximum of a state without keys: no finite score lies below it
 
 // The type the products run in: the activation type; fp16 for an 8-bit cache, whose codes it holds exactly (int8 and e4m3 have
 // at most 8 significant bits) and in which q and P keep 3 bits more than in bf16.
@@ -1006,7 +1007,7 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt)
     {
-        float m = fresh[qt] ? NEG_BIG : -minus_m[qt][0], l = l_run[qt];
+        float m = fresh[qt] ? TREE_NO_MAX : -minus_m[qt][0], l = l_run[qt];
         l += __shfl_xor(l, 16);
         l += __shfl_xor(l, 32);
         cf32x4_t acc[DTW];
@@ -1125,7 +1126,7 @@ __global__ __launch_bounds__(TREE_THREADS) void tree_combine_kernel(TreeArgs p, 
     const int M = p.rows_per_wg;
     auto record = [&](int s) { return ((size_t) (where.x + s) * p.mtiles + r / M) * M + r % M; };
     constexpr int E = DP / 32, U = 4;
-    float mm = NEG_BIG, l = 0.f;
+    float mm = TREE_NO_MAX, l = 0.f;
     for (int s = lane; s < S; s += 32)
         mm = fmaxf(mm, p.part_ml[record(s)].x);
 #pragma unroll

@@ -34,6 +34,47 @@ def put(c, half, b, t, d, value):
     c.pool[half, c.table[b, t // c.tpb], :, t % c.tpb, d] = value
 
 
+# ------------------------------------------------------------------------------------------------ precision
+@pytest.mark.parametrize("dtype,kv", [(BF, BF), (HF, HF), (BF, I8), (HF, I8), (BF, F8), (HF, F8)])
+@pytest.mark.parametrize("Hq,Hkv,D", [(4, 4, 128), (8, 1, 128), (6, 2, 64), (2, 1, 256), (3, 1, 80)])
+@pytest.mark.parametrize("q_factor", [1.0, 4.0])
+def test_precision(cuda, dtype, kv, Hq, Hkv, D, q_factor):
+    c = TreeCase([300, 130], trees([20, 12]), Hq, Hkv, D, dtype, kv, rope=2, kv_scale=SCALE[kv], seed=D)
+    c.qkv[:, :Hq * D] = (c.qkv[:, :Hq * D].float() * q_factor).to(dtype)
+    holds(c, cuda)
+
+
+@pytest.mark.parametrize("splits", [0, 1, 3, 24])
+@pytest.mark.parametrize("Hq,n", [(1, 7), (4, 8), (8, 16), (8, 40)])  # one workgroup shape each
+def test_precision_over_parts(cuda, splits, Hq, n):
+    c = TreeCase([1500, 64, 700], trees([n, 1, n]), Hq, 1, 128, BF, rope=2)
+    c.qkv[:, :Hq * 128] = (c.qkv[:, :Hq * 128].float() * 4).to(BF)
+    holds(c, cuda, op_kw=dict(multi_block_mode=splits))
+
+
+@pytest.mark.parametrize("dtype,kv", [(BF, BF), (HF, HF), (HF, I8)])
+@pytest.mark.parametrize("splits", [1, 4])
+def test_maxima_that_keep_growing(cuda, dtype, kv, splits):
+    # scores of several hundred whose maximum grows along the keys, and all of them negative: every rescale shows
+    c = TreeCase([400, 100], trees([13, 4]), 2, 1, 64, dtype, kv, kv_scale=1 / 8 if kv == I8 else 1.0)
+    for b, past in enumerate(c.past):
+        for t in range(past):
+            row = c.pool[0, c.table[b, t // c.tpb], :, t % c.tpb]
+            row.copy_((row.float() * (0.1 + 6.0 * t / past)).clamp(-127, 127).to(kv))
+    c.qkv[:, :2 * 64] = (c.qkv[:, :2 * 64].float() * 4).to(dtype)
+    holds(c, cuda, op_kw=dict(multi_block_mode=splits))
+    c.qkv[:, :2 * 64] = -c.qkv[:, :2 * 64].abs()
+    c.pool = c.pool.abs() if kv != I8 else c.pool.float().abs().clamp(max=127).to(kv)
+    holds(c, cuda, op_kw=dict(multi_block_mode=splits))
+
+
+@pytest.mark.parametrize("ns,kv", [([257, 3], BF), ([513, 1], F8), ([1024], HF), ([700, 64], I8)])
+def test_large_trees(cuda, ns, kv):
+    dtype = HF if kv in (HF, I8) else BF
+    c = TreeCase([100, 20][:len(ns)], trees(ns, 5), 2, 1, 64, dtype, kv, tpb=32, kv_scale=SCALE[kv], rope=2)
+    holds(c, cuda)
+
+
 # ------------------------------------------------------------------------------------------------ scores at and beyond the ends of fp32
 @pytest.mark.parametrize("D", [64, 128, 80, 48])
 @pytest.mark.parametrize("dtype", [BF, HF])
@@ -79,3 +120,21 @@ def test_infinite_queries(cuda):
             put(c, 0, 0, t, 5, 1.0 if t in keys else -1.0)
         out, _ = run(c, cuda)
         assert out.isnan().all() if nan else (out == 0).all()
+
+
+@pytest.mark.parametrize("n,splits", [(4, 1), (12, 1), (12, 4), (60, 1), (60, 4)])
+@pytest.mark.parametrize("big", [1e16, 1e18])
+def test_scores_far_below_zero(cuda, n, splits, big):
+    # all scores equal, at -1e31 and -1e35: the weights are equal, whatever the scores' size
+    c = TreeCase([500], trees([n]), 2, 1, 64, BF)
+    c.qkv[:, :192] = 0.0
+    c.qkv[:, [0, 64]] = big
+    c.qkv[:, 128] = -big
+    c.pool[0] = 0.0
+    c.pool[0, ..., 0] = -big
+    out, pool = run(c, cuda, op_kw=dict(multi_block_mode=splits))
+    # equal weights: P is a power of 2 or one number for all keys, so the result is the mean but for the fp32 sums
+    for rows, cols, q, k, v, hidden in S.heads(c, 0, pool):
+        w = (~hidden).double() / (~hidden).sum(1, keepdim=True)
+        # (P's one rounding is in the sums of all keys, 2^-8, and the result's own)
+        assert ((out[rows, cols].double() - w @ v).abs() <= 2 * UNIT[BF] * (w @ v).abs() + 2.0 ** -16 * (w @ v.abs())).all()
