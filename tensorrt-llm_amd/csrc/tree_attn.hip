@@ -497,8 +497,11 @@ __device__ __forceinline__ uint64_t tree_mask64(const uint32_t* row, int words, 
 // the end.
 // S^T = K . Q^T (16x16x32): a lane holds one query column's scores of 4 consecutive keys, and the same registers, rounded
 // to the compute type, are the B operand of O^T += V^T . P^T.
-// Softmax in the log2 domain with the running maximum as the C operand of the first product: what comes out is already
-// s - m, and as long as no column grows past m + 8 (p <= 256: harmless in fp16 / bf16 and in the fp32 sums) nothing is rescaled.
+// Softmax in the log2 domain with the running maximum m as the C operand of the first product: what comes out is already
+// s - m, and as long as no column grows past m + 8 (p <= 256: harmless in bf16 and in the fp32 sums) nothing is rescaled.
+// fp16 has few numbers below 1 and many above: there m lies 10 below the largest score, p goes up to 2^15, and the weights keep
+// their bits down to 2^-24 of the largest and vanish below 2^-35 (with m at the largest 2^-14 and 2^-25: many keys far behind
+// a single one were lost).  It costs nothing: the times of all fp16 and 8-bit cases stayed.
 // Whether one does is an integer maximum over the raw bits (negative floats are negative integers).
 // Scores that come out NaN: an infinite key element, or products beyond fp32, meet the second part of q, whose sign is either, or
 // the zeros that q is padded with.  The row's sum is then NaN, and the whole item runs again with careful scores; what is still
@@ -523,6 +526,8 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
     constexpr int TILE_BYTES = TREE_KT * ROWB, STAGE_BYTES = 2 * TILE_BYTES;
     constexpr int XW = 4 / KW;                      // 16-key subtiles per wave
     constexpr int X2 = XW < 2 ? XW : 2;             // subtiles per compute step: 32 keys, or 16 with four key groups
+    constexpr float LEAD = T16<C>::is_bf16 ? 0.f : 10.f;                       // m below the largest score when it is set
+    constexpr int GROWTH = __builtin_bit_cast(int, T16<C>::is_bf16 ? 8.f : 15.f); // s - m from which on the column is rescaled
     // fragments read from the LDS ahead of their products, as many as the registers hold (8-bit caches hold a tile in them too)
     constexpr bool TIGHT = KVT && PARTS == 2 && QT == 2 && DP >= 128;
     constexpr int KBATCH = TIGHT && X2 == 2 ? 2 : KS, VBATCH = TIGHT && X2 == 2 ? 4 : (DT < 8 ? DT : 8);
@@ -808,7 +813,7 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
                 for (int rr = 0; rr < 4; ++rr)
                     mx = max(mx, __builtin_bit_cast(int, (float) s[x][qt][rr]));
             const bool first = GENERAL && fresh[qt];
-            if (__any(first || mx > 0x41000000 /* 8.0f */)) // wave-uniform
+            if (__any(first || mx > GROWTH)) // wave-uniform
             {
                 // the column's maximum of these keys, over its 4 lanes (a NaN stays out of the comparison and in the scores)
                 float top = -__builtin_inff();
@@ -821,7 +826,7 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
                 top = fmaxf(top, __shfl_xor(top, 32));
                 if (top != -__builtin_inff())
                 {
-                    const float up = first ? top : fmaxf(top, 0.f);
+                    const float up = first ? top - LEAD : fmaxf(top - LEAD, 0.f);
                     const float corr = first ? 0.f : __builtin_amdgcn_exp2f(-up); // (nothing was summed before the first maximum)
                     const float mm = minus_m[qt][0] - up;
                     minus_m[qt] = cf32x4_t{mm, mm, mm, mm};

@@ -75,6 +75,29 @@ def test_large_trees(cuda, ns, kv):
     holds(c, cuda)
 
 
+# ------------------------------------------------------------------------------------------------ far weights
+@pytest.mark.parametrize("kv", [HF, I8, F8, BF])
+@pytest.mark.parametrize("splits", [1, 5])
+def test_a_key_far_ahead_keeps_the_others(cuda, kv, splits):
+    # key 0 is 26 binary orders ahead of about 5000 others and its value is 0: the result is what the others add up to, whose
+    # weights, 2^-26 of the largest, fall below fp16's smallest number where the largest is 1.  A weight held as 2^-16 in fp16
+    # is off by 2^-25 at most (2^-9 of it), in bf16 by 2^-8 of it; a score of 18 by 2^-16 (q in two bf16 parts) and fp32: 2^-11
+    dtype = BF if kv == BF else HF
+    c = TreeCase([5000], trees([8]), 2, 1, 64, dtype, kv, kv_scale=1.0)
+    c.qkv.zero_()
+    c.qkv[:, :128:64] = 8.0   # q: (8, 0, ...), score = k_0
+    c.pool[0] = torch.zeros(1).to(c.kv_dtype)
+    c.pool[1] = torch.full((1,), 64.0).to(c.kv_dtype)
+    c.qkv[:, 3 * 64:] = 64.0  # v of the nodes
+    put(c, 0, 0, 0, 0, 18.0)
+    for d in range(64):
+        put(c, 1, 0, 0, d, 0.0)
+    out, pool = run(c, cuda, op_kw=dict(multi_block_mode=splits))
+    ref = S.definition(c, pool)[0]
+    assert ref.abs().min() > 1e-3
+    assert ((out.double() - ref).abs() <= (2.0 ** -8 + 2.0 ** -11 + UNIT[dtype]) * ref).all(), (out[0, 0].item(), ref[0, 0].item())
+
+
 # ------------------------------------------------------------------------------------------------ scores at and beyond the ends of fp32
 @pytest.mark.parametrize("D", [64, 128, 80, 48])
 @pytest.mark.parametrize("dtype", [BF, HF])
