@@ -67,6 +67,7 @@ struct TreeArgs
     int4* join;          // [pairs_bound][2]: the pairs of several parts: first row, nodes, kv head, parts (0: none) | record, sequence
     float* part_acc;     // partial states: [record][m-tile][row][DP]
     float2* part_ml;     // their (running maximum in the log2 domain, sum)
+    uint8_t* q_shift;    // [tokens][Hq], where the products run in fp16: the query lies in q_ws times 2^-shift
     int64_t qkv_stride;
     int batch, num_heads, num_kv_heads, group, hs;
     int num_tokens, max_draft, max_past, mask_words;
@@ -343,26 +344,46 @@ __global__ __launch_bounds__(TREE_THREADS) void tree_prepare_kernel(TreeArgs p, 
     {
         const int vec = it / cpv, d0 = 8 * (it % cpv);
         uint4* const qdst = reinterpret_cast<uint4*>(p.q_ws + ((size_t) row * Hq + vec) * PARTS * dp + d0);
-        if (d0 >= hs) // the padding of the workspace rows
-        {
-            if (vec < Hq)
-                for (int part = 0; part < PARTS; ++part)
-                    qdst[part * dp / 8] = make_uint4(0, 0, 0, 0);
+        if (vec >= Hq && d0 >= hs)
             continue;
-        }
         if (vec < Hq)
         {
             // q carries the score scale, the K dequantisation and log2(e): the matrix product then IS the exponent
-            float y[8], hi[8], lo[8];
-            tree_chunk8<T>(p, src, vec, d0, half, rope, y, [&](int j, float& c, float& s) { c = q_tab[j].x, s = q_tab[j].y; });
+            float z[8] = {}, hi[8], lo[8]; // (zeros: the padding of the workspace rows)
+            if (d0 < hs)
+            {
+                float y[8];
+                tree_chunk8<T>(p, src, vec, d0, half, rope, y, [&](int j, float& c, float& s) { c = q_tab[j].x, s = q_tab[j].y; });
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    z[e] = y[e] * qscale;
+            }
+            if constexpr (!T16<C>::is_bf16)
+            {
+                // a head whose largest element (infinities apart) fp16 does not hold goes down by a power of 2, which the scores get
+                // back in fp32.  The lanes of a head are neighbours in one wave
+                float top = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    top = fmaxf(top, fabsf(z[e]) < HUGE_VALF ? fabsf(z[e]) : 0.f);
+                int shift = 0;
+                if (__any(top > 65504.f))
+                {
+                    for (int o = 1; o < cpv; o <<= 1)
+                        top = fmaxf(top, __shfl_xor(top, o));
+                    shift = top > 65504.f ? ilogbf(top) - 14 : 0;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        z[e] = ldexpf(z[e], -shift);
+                }
+                if (d0 == 0)
+                    p.q_shift[(size_t) row * Hq + vec] = shift;
+            }
 #pragma unroll
             for (int e = 0; e < 8; ++e)
             {
-                float z = y[e] * qscale;
-                if constexpr (!T16<C>::is_bf16) // a finite query stays finite in fp16
-                    z = fabsf(z) > 65504.f && fabsf(z) < HUGE_VALF ? copysignf(65504.f, z) : z;
-                hi[e] = T16<C>::to_float(T16<C>::from_float(z));
-                lo[e] = fabsf(hi[e]) < HUGE_VALF ? z - hi[e] : 0.f;
+                hi[e] = T16<C>::to_float(T16<C>::from_float(z[e]));
+                lo[e] = fabsf(hi[e]) < HUGE_VALF ? z[e] - hi[e] : 0.f;
             }
             *qdst = make_uint4(pack2<C>(hi[0], hi[1]), pack2<C>(hi[2], hi[3]), pack2<C>(hi[4], hi[5]), pack2<C>(hi[6], hi[7]));
             if constexpr (PARTS == 2)
@@ -505,7 +526,7 @@ __device__ __forceinline__ uint64_t tree_mask64(const uint32_t* row, int words, 
 // Whether one does is an integer maximum over the raw bits (negative floats are negative integers).
 // Scores that come out NaN: an infinite key element, or products beyond fp32, meet the second part of q, whose sign is either, or
 // the zeros that q is padded with.  The row's sum is then NaN, and the whole item runs again with careful scores; what is still
-// NaN then is so by the definition.  (The check at an item's end costs up to 1 us a call: 92.8 for 91.8 over 16
+// NaN then is so by the definition.  So does an item with a query that was shifted into the range of fp16.  (The check at an item's end costs up to 1 us a call: 92.8 for 91.8 over 16
 // sequences of 300 .. 2048 tokens, 32 / 32 heads, up to 64 nodes; nothing measurable elsewhere.)
 // Two workgroups live on a CU (64 KiB of LDS: a tile of K and V that is computed, one that arrives), 2 waves a SIMD at 219 to 249
 // registers; what one waits for the other covers.  Bound by HBM up to some 32 rows a kv head, then by the matrix instructions,
@@ -536,7 +557,7 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
     constexpr int CH8 = DP / 16, RPL = 64 / CH8, LPT = WROWS / RPL; // 8-bit caches: rows per 16-byte load, loads per thread
     __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE_BYTES]; // a tile that is computed, a tile that arrives
     __shared__ uint32_t nonfinite[TREE_MAX_DRAFT / 32]; // nodes whose V row has an infinity or NaN
-    __shared__ int redo;                                // a row's sum is NaN
+    __shared__ int redo;                                // a row's sum is NaN, or its query shifted
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -673,6 +694,7 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
     const int q0 = mt * M + rw * QT * 16;
     uint4 qf[PARTS][QT][KS];
     uint64_t mask_row[QT]; // the first 64 nodes' bits
+    int q_shift[QT];
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt)
     {
@@ -681,7 +703,11 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
         mask_row[qt] = (uint64_t) mrow[p.mask_words > 1 ? 1 : 0] << 32 | mrow[0];
         if (n < 64)
             mask_row[qt] &= (1ull << n) - 1;
-        const uint16_t* q = p.q_ws + ((size_t) (off + r / G) * p.num_heads + head_kv * G + r % G) * PARTS * DP;
+        const size_t head = (size_t) (off + r / G) * p.num_heads + head_kv * G + r % G;
+        const uint16_t* q = p.q_ws + head * PARTS * DP;
+        q_shift[qt] = 0;
+        if constexpr (!T16<C>::is_bf16)
+            q_shift[qt] = p.q_shift[head];
 #pragma unroll
         for (int part = 0; part < PARTS; ++part)
 #pragma unroll
@@ -691,7 +717,7 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
     // end the compiler's own bookkeeping of these loads here, before the loop's (to it invisible) DMAs
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt)
-        asm volatile("" : "+v"(mask_row[qt]));
+        asm volatile("" : "+v"(mask_row[qt]), "+v"(q_shift[qt]));
 #pragma unroll
     for (int part = 0; part < PARTS; ++part)
 #pragma unroll
@@ -720,7 +746,7 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
         if (GENERAL && careful) // uniform
         {
             // the products of the two parts of q apart, the padding of the keys as zeros; the second part counts only where both are
-            // finite, so that an infinite score keeps the sign that the first part gives it
+            // finite, so that an infinite score keeps the sign that the first part gives it; a shifted query's scores shifted back
 #pragma unroll 1
             for (int x = 0; x < X2; ++x)
 #pragma unroll
@@ -743,7 +769,7 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
                         const float z = fabsf(hi[rr]) < HUGE_VALF && fabsf(lo[rr]) < HUGE_VALF ? hi[rr] + lo[rr] : hi[rr];
 #pragma unroll
                         for (int y = 0; y < X2; ++y)
-                            s[y][qt][rr] = y == x ? z + minus_m[qt][rr] : s[y][qt][rr];
+                            s[y][qt][rr] = y == x ? ldexpf(z, q_shift[qt]) + minus_m[qt][rr] : s[y][qt][rr];
                     }
                 }
         }
@@ -987,7 +1013,7 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
         bool bad = false;
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt)
-            bad |= l_run[qt] != l_run[qt];
+            bad |= l_run[qt] != l_run[qt] || q_shift[qt] != 0;
         if (__any(bad))
             redo = 1;
         __syncthreads();
@@ -1175,10 +1201,10 @@ struct TreePlan
 {
     int dp, rows_per_wg, mtiles; // padded head size; query rows per workgroup; m-tiles of a (sequence, kv head)
     int target_items, part_tiles, items_bound, pairs_bound, records, whole;
-    size_t q_bytes, order_bytes, split_bytes, ok_bytes, join_bytes, acc_bytes, ml_bytes;
+    size_t q_bytes, shift_bytes, order_bytes, split_bytes, ok_bytes, join_bytes, acc_bytes, ml_bytes;
     size_t total() const
     {
-        return q_bytes + order_bytes + split_bytes + ok_bytes + join_bytes + acc_bytes + ml_bytes;
+        return q_bytes + shift_bytes + order_bytes + split_bytes + ok_bytes + join_bytes + acc_bytes + ml_bytes;
     }
 };
 size_t round256(size_t x)
@@ -1252,6 +1278,8 @@ TreePlan tree_plan(const mi355q_tree_attention_params& q)
     }
     const bool two_parts = q.kv_type == q.act_type || q.act_type == MI355Q_HALF; // TREE_Q2
     t.q_bytes = round256((size_t) q.num_tokens * q.num_heads * t.dp * 2 * (two_parts ? 2 : 1));
+    if (q.act_type == MI355Q_HALF || q.kv_type != q.act_type) // products in fp16
+        t.shift_bytes = round256((size_t) q.num_tokens * q.num_heads);
     t.order_bytes = round256((size_t) (q.batch + 1) * sizeof(int4));
     t.split_bytes = round256((size_t) q.batch * sizeof(int4));
     t.ok_bytes = round256((size_t) q.batch * sizeof(int32_t));
@@ -1391,6 +1419,7 @@ void tree_attention(const mi355q_tree_attention_params& q, hipStream_t stream)
         return at;
     };
     a.q_ws = reinterpret_cast<uint16_t*>(carve(t.q_bytes));
+    a.q_shift = reinterpret_cast<uint8_t*>(carve(t.shift_bytes));
     a.order = reinterpret_cast<int4*>(carve(t.order_bytes));
     a.split = reinterpret_cast<int4*>(carve(t.split_bytes));
     a.seq_ok = reinterpret_cast<int32_t*>(carve(t.ok_bytes));

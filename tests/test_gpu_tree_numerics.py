@@ -161,3 +161,22 @@ def test_scores_far_below_zero(cuda, n, splits, big):
         w = (~hidden).double() / (~hidden).sum(1, keepdim=True)
         # (P's one rounding is in the sums of all keys, 2^-8, and the result's own)
         assert ((out[rows, cols].double() - w @ v).abs() <= 2 * UNIT[BF] * (w @ v).abs() + 2.0 ** -16 * (w @ v.abs())).all()
+
+
+@pytest.mark.parametrize("dtype,kv,factor", [(BF, I8, 1.0), (BF, F8, 1.0), (BF, F8, 1e6), (HF, HF, 1.0), (HF, F8, 1.0)])
+@pytest.mark.parametrize("n,splits", [(3, 1), (12, 3), (60, 1)])
+def test_queries_beyond_fp16(cuda, dtype, kv, factor, n, splits):
+    # q times its scale is beyond 65504 in two places, of which the larger decides: cut off there both would be equal, and the
+    # other key, with the larger element, would win
+    c = TreeCase([100], trees([n]), 2, 1, 64, dtype, kv, kv_scale=1.0)
+    q_scaling = 1.0 if dtype == BF else 1.0 / 512
+    c.qkv[:, :128] = (c.qkv[:, :128].float() * 0.1).to(dtype)
+    c.qkv[:, [0, 64]] = 3.0e6 * factor if dtype == BF else 30000.0
+    c.qkv[:, [1, 65]] = 1.0e6 * factor if dtype == BF else 10000.0
+    c.qkv[:, 128:192] = 0.0
+    c.pool[0] = torch.zeros(1).to(c.kv_dtype)
+    put(c, 0, 0, 7, 0, 1.0)
+    put(c, 0, 0, 40, 1, 2.0)
+    out = holds(c, cuda, op_kw=dict(multi_block_mode=splits, q_scaling=q_scaling), q_scaling=q_scaling)
+    v = c.pool[1, c.table[0, 0], 0, 7]
+    assert torch.equal(out[:, :64], v.to(dtype).expand(n, -1))
