@@ -507,7 +507,9 @@ extern "C"
      * nodes j whose bit (word j / 32, bit j % 32 of the row of tree_mask) is set -- itself too only if its own bit is.  A row
      * that sees nothing is 0.  What a row does not see does not reach it, infinities and NaN included.  Scores are held in
      * fp32: a key whose score is -inf, or below what fp32 holds, has weight 0 (a row that sees no other is 0), a score of
-     * +inf makes its row NaN.  K / V are read back from the cache, so an 8-bit cache attends to the quantised nodes.
+     * +inf makes its row NaN.  K / V are read back from the cache, so an 8-bit cache attends to the quantised nodes; there, as
+     * in every call that writes such a cache, values beyond its range saturate, infinities too, and a NaN becomes the lowest
+     * value (-128, -448).
      * A sequence whose device-side lengths do not fit (past_lengths outside 0 .. max_past_length, more than
      * max_draft_length nodes, rows outside num_tokens, keys beyond the block table) or whose table lacks a block (pointer 0, or
      * not 16-byte aligned) is skipped: its rows of out stay as they were.  Rows of qkv / out outside every sequence are not touched. */

@@ -180,3 +180,28 @@ def test_queries_beyond_fp16(cuda, dtype, kv, factor, n, splits):
     out = holds(c, cuda, op_kw=dict(multi_block_mode=splits, q_scaling=q_scaling), q_scaling=q_scaling)
     v = c.pool[1, c.table[0, 0], 0, 7]
     assert torch.equal(out[:, :64], v.to(dtype).expand(n, -1))
+
+
+# ------------------------------------------------------------------------------------------------ NaN into 8-bit caches
+@pytest.mark.parametrize("kv,low", [(I8, -128), (F8, -448.0)])
+def test_nan_into_an_8_bit_cache_is_its_lowest_value(cuda, kv, low):
+    # like every kernel of the framework that writes these caches; infinities saturate.  No row but those that see the node changes
+    c = TreeCase([70], trees([9]), 4, 2, 64, BF, kv, kv_scale=1 / 32)
+    k, v = 4 * 64, 6 * 64
+    seen = [0b1, 0b11, 0b101, 0b1001, 0b10001, 0b100001, 0b1000001, 0b10000001, 0b100000001]
+    c.mask[:] = pack_rows(seen, c.words)
+    clean, clean_pool = run(c, cuda)
+    for i, at in ((3, v + 5), (5, k + 70)):
+        c.qkv[i, at] = float("nan")
+    c.qkv[6, v + 9], c.qkv[6, v + 10] = float("inf"), float("-inf")
+    out, pool = run(c, cuda)
+    value = lambda half, node, h, d: pool[half, c.table[0, (70 + node) // c.tpb], h, (70 + node) % c.tpb, d].float().item()
+    assert value(1, 3, 0, 5) == low and value(0, 5, 1, 6) == low
+    assert value(1, 6, 0, 9) == (127 if kv == I8 else 448) and value(1, 6, 0, 10) == low
+    same = [0, 1, 2, 4, 7, 8]
+    assert torch.equal(out[same].view(torch.int16), clean[same].view(torch.int16)) and torch.isfinite(out).all()
+    held = c.qkv.clone()
+    held[held.isnan()] = low / 32
+    c.qkv = held
+    wrong = S.verdict(out, *S.definition(c, pool))
+    assert wrong is None, wrong
