@@ -557,7 +557,7 @@ extern "C"
      * be handed out from the next call on).  status: 0 done; 1 the free blocks did not reach (nor for any later request
      * that asked); 2 more than max_blocks_per_seq blocks; 3 lengths or counts out of range.  A refused request keeps what it
      * has and its slots are -1.  Pointers are 0 where no block is held (all of an ended request's); so are those of a table
-     * or ring entry outside the pool. */
+     * or ring entry outside the pool.  With batch 0 the call writes nothing, token_offsets and free_state_out neither. */
     typedef struct
     {
         const int32_t* past_lengths; /* device [batch] */

@@ -578,6 +578,11 @@ def kv_block_tables(past_lengths, new_lengths, block_table, block_counts, free_b
             at + need + 4 * (batch + 1), at, need, block_bytes, batch, max_blocks, free_blocks.shape[0], pools, num_tokens,
             tokens_per_block)
         L.check(L.lib().mi355q_kv_block_tables(C.byref(p), stream))
+        if batch == 0:  # (the library's call writes nothing then)
+            offsets.zero_()
+            slots.fill_(-1)
+            if state_out is not free_state:
+                state_out.copy_(free_state)
     return pointers, offsets, slots, status
 
 
