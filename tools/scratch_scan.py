@@ -12,6 +12,7 @@ for src in sorted(glob.glob(os.path.join(root, "*.hip"))):
     per_file = ["-fno-slp-vectorize"] if os.path.basename(src) in ("woq_gemm.hip", "woq_gemv_small.hip", "woq_prefill.hip") else []
     with tempfile.TemporaryDirectory() as td:
         r = subprocess.run(["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950", "-ffp-contract=off",
+                            "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
                             "-Rpass-analysis=kernel-resource-usage", *per_file, *extra, "-c", src, "-o", os.path.join(td, "x.o")],
                            capture_output=True, text=True, cwd=root)
     seen = set()
