@@ -1247,12 +1247,16 @@ TreePlan tree_plan(const mi355q_tree_attention_params& q)
     // 64.3 / 127)
     t.rows_per_wg = rows <= 16 ? 16 : (rows <= 32 || (rows <= 64 && t.dp <= 128 && groups < 256) ? 32 : (rows <= 64 || t.dp > 128 ? 64 : 128));
     t.mtiles = (rows + t.rows_per_wg - 1) / t.rows_per_wg;
-    // One item per (sequence, kv head), nothing to join, for short histories: up to 512 tokens, and up to 4096 the longer the more
-    // workgroups there are to even the lengths out (64 tiles with the chip's 512).  us whole / in parts, equal histories of t tokens:
-    // 32 workgroups (one sequence, 32 heads, 8 nodes) t = 440 13.2 / 15.0, 1000 18.4 / 16.1; 128 (4 sequences, 16 nodes) 600 19.0 / 22.9,
-    // 1000 24.1 / 26.5; 256 (8) 2100 55.1 / 58.3, 3400 101.2 / 100.6 (ragged 66.0 / 60.3); 512 (16, 64 nodes) 4100 235 / 238, 1024 (32) 417 / 430
-    const int64_t whole_tiles = std::min<int64_t>(std::max<int64_t>(groups * t.mtiles / 8, 8), 64);
-    t.whole = q.multi_block_mode == 1 || (q.multi_block_mode == 0 && max_tiles <= whole_tiles);
+    // One item per (sequence, kv head), nothing to join, for short histories: up to 512 keys, and up to 4096 tokens of history the
+    // longer the more workgroups there are to even the lengths out (64 tiles with the chip's 512; the nodes on top of a history do
+    // not count, or 4096 tokens would be cut).  us whole / in parts, equal histories of t tokens: 8 workgroups (one sequence, 8 kv heads, 8
+    // nodes) t = 512 16.8 / 15.9; 32 (32 kv heads) 440 13.2 / 15.0, 512 15.5 / 15.9, 1000 18.4 / 16.1; 128 (4 sequences, 16 nodes) 600 19.0 /
+    // 22.9, 1024 24.4 / 27.5 (ragged 23.2 / 24.3); 256 (8) 2048 51.4 / 58.0 (ragged 40.9 / 44.5), 3400 101.2 / 100.6 (ragged 66.0 /
+    // 60.3); 512 (16, 64 nodes, 64 / 8 heads) 4096 190.1 / 192.1 (ragged 126.9 / 130.0), fp8 155.5 / 156.8 (ragged 116.8 / 119.4); 1024 (32)
+    // 4100 417 / 430
+    const int history_tiles = (q.max_past_length + TREE_KT - 1) / TREE_KT;
+    const int64_t whole_tiles = std::min<int64_t>(groups * t.mtiles / 8, 64);
+    t.whole = q.multi_block_mode == 1 || (q.multi_block_mode == 0 && (max_tiles <= 8 || history_tiles <= whole_tiles));
     if (t.whole)
         t.items_bound = (int) std::min<int64_t>(groups, INT32_MAX / 16);
     else if (q.multi_block_mode > 0)
