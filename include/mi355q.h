@@ -503,7 +503,7 @@ extern "C"
     /* Attention of a tree of drafted tokens over the paged cache.  Node i of sequence b is row draft_offsets[b] + i of
      * qkv; its position is past_lengths[b] + position_offsets[row] (NULL: + i), its cache slot past_lengths[b] + i (position
      * t lives in block t / tokens_per_block: no window, no sink tokens, no beams).  The call rotates q and k, rounds K / V
-     * of every node once to the cache's type, stores them, and attends from every node to the past tokens and to the
+     * of every node to the cache's type, stores them, and attends from every node to the past tokens and to the
      * nodes j whose bit (word j / 32, bit j % 32 of the row of tree_mask) is set -- itself too only if its own bit is.  A row
      * that sees nothing is 0.  What a row does not see does not reach it, infinities and NaN included.  Scores are held in
      * fp32: a key whose score is -inf, or below what fp32 holds, has weight 0 (a row that sees no other is 0), a score of

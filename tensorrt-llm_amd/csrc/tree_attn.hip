@@ -5,7 +5,7 @@
 // slot past + i.  For every query head
 //     out[i] = sum_t softmax_t(q_i . k_t / (sqrt(Dh) q_scaling)) v_t   over t < past and the nodes t = past + j of i's mask,
 // and 0 where nothing is visible.  Three launches:
-//   1. tree_prepare_kernel: bias and rotation of q, k, v; K / V of every node rounded ONCE to the cache's type and stored
+//   1. tree_prepare_kernel: bias and rotation of q, k, v; K / V of every node rounded to the cache's type and stored
 //      in its slot; q, times the score scale, to the workspace.  One workgroup per sequence checks its lengths and blocks.
 //   2. tree_attn_kernel: flash attention of the nodes over the cache (K / V of the nodes come from the cache too, so a
 //      later step over the accepted tokens sees the values that were scored).
@@ -268,10 +268,11 @@ __device__ __forceinline__ void tree_chunk8(
 
 // ---------------------------------------------------------------------------------------------- 1. prepare
 // grid (max_draft + 2, batch, parts of the heads).  Angles, and rotation and quantisation of K / V, run in 64 bits: the angle of a
-// far position has few correct digits left in fp32 (position 2^17: error 2^-8 rad), and a value next to a rounding border
-// of the cache's type lands on the side the definition says.  The queries, the larger part, are rotated in fp32.
+// far position has few correct digits left in fp32 (position 2^17: error 2^-8 rad).  From there K / V go through fp32 to the cache's type,
+// as torch's conversion does (int8 codes are rounded in 64 bits): the stored rows equal those of the definition.
+// The queries, the larger part, are rotated in fp32.
 // Bound by memory: rows in, two parts of q and K / V out, in rows of 256 bytes.  708 tokens of 32 + 64 heads of 128: 14 us for 41 MB;
-// 8 tokens: 4.2 us, a launch, three dependent loads and the angles.  (Loading a thread's elements ahead of the angles, values
+// 8 tokens: 4.0 us, a launch, three dependent loads and the angles.  (Loading a thread's elements ahead of the angles, values
 // as plain copies, and more or fewer workgroups than 2048 all cost 1 to 3 us more.)
 template <typename T, int KVT>
 __global__ __launch_bounds__(TREE_THREADS) void tree_prepare_kernel(TreeArgs p, int dp)
@@ -526,14 +527,13 @@ __device__ __forceinline__ uint64_t tree_mask64(const uint32_t* row, int words, 
 // Whether one does is an integer maximum over the raw bits (negative floats are negative integers).
 // Scores that come out NaN: an infinite key element, or products beyond fp32, meet the second part of q, whose sign is either, or
 // the zeros that q is padded with.  The row's sum is then NaN, and the whole item runs again with careful scores; what is still
-// NaN then is so by the definition.  So does an item with a query that was shifted into the range of fp16.  (The check at an item's end costs up to 1 us a call: 92.8 for 91.8 over 16
-// sequences of 300 .. 2048 tokens, 32 / 32 heads, up to 64 nodes; nothing measurable elsewhere.)
-// Two workgroups live on a CU (64 KiB of LDS: a tile of K and V that is computed, one that arrives), 2 waves a SIMD at 219 to 249
+// NaN then is so by the definition.  So does an item with a query that was shifted into the range of fp16.
+// Two workgroups live on a CU (64 KiB of LDS: a tile of K and V that is computed, one that arrives), 2 waves a SIMD at 225 to 255
 // registers; what one waits for the other covers.  Bound by HBM up to some 32 rows a kv head, then by the matrix instructions,
 // of which the second part of q is a third, by the softmax beside them and by the LDS.  Whole calls, bf16, Dh 128, 64 sequences of 2048
 // tokens, 32 / 32 heads: 1 node 5.7 TB/s, 16 nodes 5.3, 64 nodes 4.8 (a copy reaches 5.05); 16 x 4096 tokens, 64 nodes, 64 / 8 heads:
-// 205 us = 0.68 PFLOP/s of the formula's and 1.0 of products issued (a large matrix product 1.23); one sequence of 120001
-// tokens, 60 nodes, 64 / 8 heads: 325 us, matrix pipes busy 51 %, no LDS conflicts.  Four tiles in flight with one workgroup a CU
+// 199 us = 0.70 PFLOP/s of the formula's and 1.05 of products issued (a large matrix product 1.23); one sequence of 120001
+// tokens, 60 nodes, 64 / 8 heads: 308 us, matrix pipes busy 53 %, no LDS conflicts.  Four tiles in flight with one workgroup a CU
 // took 127 us where this took 93, 8 waves of 256 rows 275 for 217.
 template <typename T, int KVT, int DP, int RW, int KW, int QT>
 __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP > 128 ? 1 : 2))) void tree_attn_kernel(TreeArgs p)
@@ -572,8 +572,8 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
 
     // swizzle of the 16-byte chunk index by the row, K and V alike.  The banks see a 16-byte read of 64 lanes in groups of rows
     // 0-3, 12-15 at one chunk with rows 4-11 at its neighbour (K fragments: row = lane & 15), and a transposing read in groups of
-    // 4 rows x 2 chunks (V): both fall on all banks once; so do the writes of every other chunk of two neighbouring rows (8-bit
-    // caches).  It depends on the row modulo 16 only.
+    // 4 rows x 2 chunks (V): both fall on all banks once.  The tile writes of the 8-bit caches, every other chunk of two neighbouring
+    // rows, do not: a quarter of that kernel's LDS cycles are conflicts.  It depends on the row modulo 16 only.
     auto sw = [](int row)
     {
         const int x = (row >> 2) & 3;
@@ -1008,16 +1008,14 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
                 }
             }
         }
-        if (careful)
-            break;
         bool bad = false;
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt)
             bad |= l_run[qt] != l_run[qt] || q_shift[qt] != 0;
         if (__any(bad))
             redo = 1;
-        __syncthreads();
-        if (!__builtin_amdgcn_readfirstlane(redo))
+        __syncthreads(); // (everyone is done with the tiles, too)
+        if (careful || !__builtin_amdgcn_readfirstlane(redo))
             break;
         stage = 0;
         i = tile_lo;
@@ -1052,7 +1050,8 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
         {
             constexpr int STATE = (DT + 1) * 64 * 16; // bytes of one wave's state: float4 per register group and lane
             static_assert(4 * STATE <= 2 * STAGE_BYTES, "states do not fit the tile buffers");
-            __syncthreads(); // everyone is done with the tiles, or with the states before
+            if (qt > 0)
+                __syncthreads(); // everyone is done with the states before
             cf32x4_t* st = reinterpret_cast<cf32x4_t*>(lds + wave * STATE) + lane;
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt)
