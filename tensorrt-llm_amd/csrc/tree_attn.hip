@@ -852,9 +852,14 @@ __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP
                 top = fmaxf(top, __shfl_xor(top, 32));
                 if (top != -__builtin_inff())
                 {
-                    const float up = first ? top - LEAD : fmaxf(top - LEAD, 0.f);
-                    const float corr = first ? 0.f : __builtin_amdgcn_exp2f(-up); // (nothing was summed before the first maximum)
+                    // where fp32 counts in steps of 2 and more the maximum gets no lead, or P would leave fp16 by its rounding; below
+                    // that the sums move by what the maximum moved by, rounding included
+                    const bool coarse = fabsf(minus_m[qt][0] - top) >= 0x1p24f;
+                    const float lead = coarse ? 0.f : LEAD;
+                    float up = first ? top - lead : fmaxf(top - lead, 0.f);
                     const float mm = minus_m[qt][0] - up;
+                    up = coarse ? up : minus_m[qt][0] - mm;
+                    const float corr = first ? 0.f : __builtin_amdgcn_exp2f(-up); // (nothing was summed before the first maximum)
                     minus_m[qt] = cf32x4_t{mm, mm, mm, mm};
                     if constexpr (GENERAL)
                         fresh[qt] = false;

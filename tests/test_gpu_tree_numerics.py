@@ -205,3 +205,44 @@ def test_nan_into_an_8_bit_cache_is_its_lowest_value(cuda, kv, low):
     c.qkv = held
     wrong = S.verdict(out, *S.definition(c, pool))
     assert wrong is None, wrong
+
+
+# ------------------------------------------------------------------------------------------------ maxima whose step is coarse
+@pytest.mark.parametrize("dtype,kv", [(BF, I8), (BF, F8), (HF, HF), (BF, BF)])
+@pytest.mark.parametrize("log2_score", [12, 20, 22.5, 23.5, 24.5, 25.5, 26.5, 27.5, 28.5, 29.5, 31, 40])
+@pytest.mark.parametrize("n,splits", [(3, 1), (60, 1), (60, 3)])
+def test_one_key_far_ahead_of_all_at_any_size(cuda, dtype, kv, log2_score, n, splits):
+    # the largest score is 2^log2_score binary orders, where fp32 counts in steps of up to 2^17; the rest lies as far behind
+    c = TreeCase([200], trees([n]), 2, 1, 64, dtype, kv, kv_scale=1.0)
+    q_scaling = 1.0 if dtype == BF else 2.0 ** -24
+    value = 2.0 ** log2_score / (0.125 * 1.4426950408889634) * q_scaling / 2
+    c.qkv[:, :192] = 0.0
+    c.qkv[:, [0, 64]] = value
+    c.pool[0] = torch.zeros(1).to(c.kv_dtype)
+    put(c, 0, 0, 7, 0, 1.0)
+    put(c, 0, 0, 150, 0, 2.0)  # in another tile: the maximum doubles
+    out, _ = run(c, cuda, op_kw=dict(multi_block_mode=splits, q_scaling=q_scaling))
+    if not torch.isfinite(c.qkv).all():  # (fp16 does not hold the query of the last case: inf * 0 is NaN)
+        assert dtype == HF and log2_score == 40 and out.isnan().all()
+        return
+    v = c.pool[1, c.table[0, 150 // c.tpb], 0, 150 % c.tpb]
+    assert torch.equal(out[:, :64], v.to(dtype).expand(n, -1))
+
+
+@pytest.mark.parametrize("dtype,kv", [(BF, I8), (HF, HF), (BF, BF)])
+@pytest.mark.parametrize("top", [1000, 30000, 500000])
+def test_a_maximum_that_moves_a_little_at_large_scores(cuda, dtype, kv, top):
+    # key 7 at `top` binary orders, key 150 a few above it: the rescale has to move sums and maximum by the same step
+    c = TreeCase([200], trees([12]), 1, 1, 64, dtype, kv, kv_scale=1.0)
+    q_scaling = 2.0 ** -8
+    c.qkv[:, :128] = 0.0
+    unit = 0.125 * 1.4426950408889634 / q_scaling  # of a score per q k
+    c.qkv[:, 0], c.qkv[:, 1] = top / unit / 64, 20.3 / unit
+    c.pool[0] = torch.zeros(1).to(c.kv_dtype)
+    for t, extra in ((7, 0.0), (150, 1.0)):
+        put(c, 0, 0, t, 0, 64.0)
+        put(c, 0, 0, t, 1, extra)
+    out, pool = run(c, cuda, op_kw=dict(q_scaling=q_scaling))
+    ref = S.definition(c, pool, q_scaling)[0]
+    # key 150 is 2^20 ahead; key 7's share, 2^-20, is below the result's rounding
+    assert ((out.double() - ref).abs() <= UNIT[dtype] * ref.abs() + 2.0 ** -18 * ref.abs().max()).all()
