@@ -533,7 +533,7 @@ __device__ __forceinline__ uint64_t tree_mask64(const uint32_t* row, int words, 
 // of which the second part of q is a third, by the softmax beside them and by the LDS.  Whole calls, bf16, Dh 128, 64 sequences of 2048
 // tokens, 32 / 32 heads: 1 node 5.7 TB/s, 16 nodes 5.3, 64 nodes 4.8 (a copy reaches 5.05); 16 x 4096 tokens, 64 nodes, 64 / 8 heads:
 // 199 us = 0.70 PFLOP/s of the formula's and 1.05 of products issued (a large matrix product 1.23); one sequence of 120001
-// tokens, 60 nodes, 64 / 8 heads: 308 us, matrix pipes busy 53 %, no LDS conflicts.  Four tiles in flight with one workgroup a CU
+// tokens, 60 nodes, 64 / 8 heads: 308 to 317 us, matrix pipes busy 53 %, no LDS conflicts.  Four tiles in flight with one workgroup a CU
 // took 127 us where this took 93, 8 waves of 256 rows 275 for 217.
 template <typename T, int KVT, int DP, int RW, int KW, int QT>
 __global__ __launch_bounds__(TREE_THREADS) __attribute__((amdgpu_waves_per_eu(DP > 128 ? 1 : 2))) void tree_attn_kernel(TreeArgs p)
