@@ -103,7 +103,7 @@ def model(c, pool, q_parts=None):
     return out
 
 
-def verdict(out, ref, bound, variance):
+def wrong_with(out, ref, bound, variance):
     """None, or what is wrong with `out` [tokens, Hq * D] against the definition."""
     live = ~bound.isnan().all(1)
     o, r, t, var = out.double()[live], ref[live], bound[live], variance[live]

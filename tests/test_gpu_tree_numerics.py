@@ -24,7 +24,7 @@ def run(c, dev, op_kw=None, **call):
 
 def holds(c, dev, op_kw=None, q_scaling=1.0, **call):
     out, pool = run(c, dev, op_kw, **call)
-    wrong = S.verdict(out, *S.definition(c, pool, q_scaling))
+    wrong = S.wrong_with(out, *S.definition(c, pool, q_scaling))
     assert wrong is None, wrong
     return out
 
@@ -203,7 +203,7 @@ def test_nan_into_an_8_bit_cache_is_its_lowest_value(cuda, kv, low):
     held = c.qkv.clone()
     held[held.isnan()] = low / 32
     c.qkv = held
-    wrong = S.verdict(out, *S.definition(c, pool))
+    wrong = S.wrong_with(out, *S.definition(c, pool))
     assert wrong is None, wrong
 
 

@@ -23,7 +23,7 @@ def case(dtype, kv, D, past=(300, 130), n=(20, 12), q_factor=4.0, **kw):
 def test_limits_accept_the_arithmetic(dtype, kv, D):
     c = case(dtype, kv, D)
     pool = c.reference()[2]
-    assert S.verdict(S.model(c, pool), *S.definition(c, pool)) is None
+    assert S.wrong_with(S.model(c, pool), *S.definition(c, pool)) is None
 
 
 @pytest.mark.parametrize("dtype,kv", [(BF, BF), (HF, HF), (HF, I8), (HF, F8)])
@@ -31,15 +31,15 @@ def test_limits_accept_the_arithmetic(dtype, kv, D):
 def test_limits_reject_a_query_in_one_part(dtype, kv, D):
     c = case(dtype, kv, D)
     pool = c.reference()[2]
-    assert S.verdict(S.model(c, pool, q_parts=1), *S.definition(c, pool)) is not None
+    assert S.wrong_with(S.model(c, pool, q_parts=1), *S.definition(c, pool)) is not None
 
 
 def test_limits_reject_zeros_and_a_lost_rescale():
     c = case(BF, BF, 64, q_factor=40.0)
     pool = c.reference()[2]
     ref, bound, var = S.definition(c, pool)
-    assert S.verdict(S.model(c, pool), ref, bound, var) is None
-    assert S.verdict(torch.zeros_like(ref), ref, bound, var) is not None
+    assert S.wrong_with(S.model(c, pool), ref, bound, var) is None
+    assert S.wrong_with(torch.zeros_like(ref), ref, bound, var) is not None
     assert ((ref.abs() <= bound).double().mean() < 0.05)
 
 
